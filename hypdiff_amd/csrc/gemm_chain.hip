@@ -207,7 +207,7 @@ __device__ __forceinline__ bool dep_ready(const ChainArgs& P, const int* tab, in
 // experiments (-DHD_CHAIN_EXPERIMENT) put the staging + barrier + fragment-read pipeline alone at ~420 us of the 500.
 #ifndef HD_CHAIN_WO
 #define HD_CHAIN_WO 2              // write-out: 0 = bias loads per column pair, scalar GELU; 1 = a tile's bias loads in one batch;
-                                   // 2 = 1 + GELU on the packed fp32 pipe (same bits).  Same-box A/B in the bench step
+                                   // 2 = 1 + GELU on two values at a time (same bits).  Same-box A/B in the bench step
                                    // (tools/probes/bench_ab.sh, twice): 183.6 / 184.1 -> 184.3 / 185.1 -> 185.5 / 184.9 TF
 #endif
 #ifndef HD_CHAIN_PRIO

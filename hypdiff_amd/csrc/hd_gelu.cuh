@@ -30,9 +30,8 @@ __device__ __forceinline__ float erf_fast(float a) {
     return t > 0.927734375f ? r : q;
 }
 __device__ __forceinline__ float gelu_erf(float x) { return 0.5f * x * (1.0f + erf_fast(x * 0.70710678118654752440f)); }
-// Two at a time on the packed fp32 pipe (v_pk_fma_f32 / v_pk_mul_f32 / v_pk_add_f32: two lanes' worth of
-// FMAs per issue): the same operations in the same order as erf_fast / gelu_erf, so the results are bit
-// identical; only exp and the selects stay scalar.  The GEMM write-outs are VALU-bound on this.
+// Two values at a time: the same operations per element in the same order as erf_fast / gelu_erf, so the same bits (the
+// build scalarises them: packed fp32 instructions are off).
 typedef float hd_f32x2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ hd_f32x2 gelu_erf2(hd_f32x2 x) {
     const hd_f32x2 a = x * 0.70710678118654752440f;
@@ -77,8 +76,7 @@ __device__ __forceinline__ float gelu_erfc(float x) {
     const float e = __builtin_amdgcn_exp2f(r * t);                       // erfc(|a|)
     return x * (x >= 0.f ? fmaf(-0.5f, e, 1.0f) : 0.5f * e);
 }
-// gelu_erfc on two values at a time (v_pk_mul_f32 / v_pk_fma_f32: the same operations per element in the same order, so
-// the same bits; exp2 and the select stay per element)
+// gelu_erfc on two values at a time (the same operations per element in the same order, so the same bits)
 __device__ __forceinline__ hd_f32x2 gelu_erfc2(hd_f32x2 x) {
     const hd_f32x2 a = x * 0.70710678118654752440f;
     const hd_f32x2 t = {fabsf(a.x), fabsf(a.y)};
