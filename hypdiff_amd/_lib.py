@@ -40,6 +40,11 @@ class HdAdamJob(ctypes.Structure):
     _fields_ = [("param", c_void_p), ("offset", c_int64), ("count", c_int64)]
 
 
+class HdAdamWJob(ctypes.Structure):
+    """struct hd_adamw_job of include/hypdiff.h"""
+    _fields_ = [("param", c_void_p), ("grad", c_void_p), ("first", c_int64), ("count", c_int64), ("row", c_int64)]
+
+
 class HdTnJob(ctypes.Structure):
     """struct hd_tn_job of include/hypdiff.h"""
     _fields_ = [("a_img", c_void_p), ("b_img", c_void_p), ("c", c_void_p), ("colsum_a", c_void_p), ("P", c_int64),
@@ -76,6 +81,7 @@ SIZE_QUERIES = {
     "hd_chain_image_bytes": [I64, I64],
     "hd_chain_workspace_bytes": [],
     "hd_mlp_chain_workspace_bytes": [I64, c_int],
+    "hd_adamw_max_jobs": [],
 }
 
 # name -> argtypes; names ending in "*" exist as _f32 and _f64
@@ -146,6 +152,8 @@ SIGNATURES = {
     "hd_transpose_f32": [P, P, I64, I64, I64, I64, P],
     "hd_transpose_multi_f32": [POINTER(HdTransposeJob), c_int, P],
     "hd_adam_step_f32": [POINTER(HdAdamJob), c_int, P, P, P, c_double, c_double, c_double, c_double, I64, P, P],
+    "hd_adamw_step": [P, c_int, c_int, c_int, P, P, P, P, P, I64, c_double, c_double, c_double, c_double, c_double, I64, P,
+                      I64, P],
     "hd_colsum_f32": [P, P, I64, I64, I64, P, P],
     "hd_bias_gelu_f32": [P, P, P, P, I64, I64, c_int, P],
     "hd_gelu_bwd_f32": [P, P, P, I64, P],

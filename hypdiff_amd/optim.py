@@ -1,0 +1,257 @@
+"""AdamW over many parameter tensors in one launch, moments in 32 bits or in 8 (csrc/adamw.hip).
+
+Stands beside dist.BucketAdam (Adam over the fp32 bucket of the data-parallel trainer): the same kind of one-launch step for
+parameters in fp32, bf16 or fp16 with gradients of their own type, with decoupled weight decay and parameter groups.  The
+reference trains with optim.Adam(params, lr) (diff.py:107, diff_graphset.py:66, lp_train.py:41-46).
+"""
+import numpy as np
+import torch
+
+from . import _lib, ops
+
+BLOCK = 256                 # elements of one scale of the 8-bit moments; every tensor's state starts on a multiple of it
+_DT = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_JOB = np.dtype([("param", np.uint64), ("grad", np.uint64), ("first", np.int64), ("count", np.int64), ("row", np.int64)])
+_OPTIONS = ("lr", "betas", "eps", "weight_decay", "state_bits", "master_weights")
+
+
+class _Flat:
+    """The state of one parameter group: flat arrays with a segment of whole 256-element blocks for every parameter."""
+
+    def __init__(self, group):
+        self.params = list(group["params"])
+        self.bits, self.with_master = int(group["state_bits"]), bool(group["master_weights"])
+        dev = self.params[0].device
+        self.numels = [p.numel() for p in self.params]
+        self.first, at = [], 0
+        for n in self.numels:
+            self.first.append(at)
+            at += (n + BLOCK - 1) // BLOCK * BLOCK
+        self.total = at
+        self.steps = [0] * len(self.params)              # steps taken by each parameter, as the host counts them
+        self.table = torch.zeros(len(self.params), 3, dtype=torch.float64, device=dev)     # the device's count
+        self.device_count = False                        # True once a step was captured: the device's count is the true one
+        self.buffers = {}
+        if self.bits == 32:
+            self.buffers["exp_avg"] = torch.zeros(at, dtype=torch.float32, device=dev)
+            self.buffers["exp_avg_sq"] = torch.zeros(at, dtype=torch.float32, device=dev)
+        else:
+            for k in ("exp_avg", "exp_avg_sq_root"):
+                self.buffers[k] = torch.zeros(at, dtype=torch.uint8, device=dev).view(torch.float8_e4m3fn)
+                self.buffers[k + "_scale"] = torch.zeros(at // BLOCK, dtype=torch.float32, device=dev)
+        if self.with_master:
+            m = self.buffers["master"] = torch.zeros(at, dtype=torch.float32, device=dev)
+            for p, a, n in zip(self.params, self.first, self.numels):
+                m[a:a + n].copy_(p.detach().reshape(-1))
+
+    def view(self, key, i):
+        """parameter i's part of a buffer: its shape, or one value per block for the scales"""
+        a, n, buf = self.first[i], self.numels[i], self.buffers[key]
+        if key.endswith("_scale"):
+            return buf[a // BLOCK:(a + n + BLOCK - 1) // BLOCK]
+        return buf[a:a + n].view(self.params[i].shape)
+
+    def refresh_steps(self):
+        if self.device_count:                            # replays of a captured step counted on the device alone
+            self.steps = [int(t) for t in self.table[:, 0].tolist()]
+
+    def set_step(self, i, t):
+        self.steps[i] = int(t)
+        self.table[i, 0] = float(int(t))
+
+
+class AdamW(torch.optim.Optimizer):
+    """torch.optim.AdamW's update
+
+        m = b1 m + (1 - b1) g;  v = b2 v + (1 - b2) g^2;  p = p (1 - lr wd) - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+
+    in fp32 arithmetic over parameters in fp32, bf16 or fp16 (contiguous, on the current GPU), one launch per 88 tensors of
+    a group.
+
+    state_bits=32: moments in fp32, also for 16-bit parameters.
+    state_bits=8: m and sqrt(v) as e4m3 codes with one fp32 scale per 256 elements (2.03 bytes per parameter instead of 8).
+        sqrt(v) is rounded up or down so that it is right on average over steps (round-to-nearest would never let it decay);
+        the rounding depends on the element and the step alone, so a run repeats bit for bit.
+    master_weights=True: 16-bit parameters keep fp32 weights in the state and receive their rounding (an update below half a
+        step of the type is lost otherwise).  fp32 parameters are their own.  The masters are taken from the parameters at
+        the first step (or from a loaded state): parameters changed by hand afterwards are overwritten.
+
+    Sparse, complex and fp64 parameters, lr as a tensor, amsgrad and maximize are not offered.  A parameter whose gradient
+    is None is skipped and does not count the step.  Inside a captured HIP graph the step count lives on the device, so a
+    replay has the right bias corrections; lr and the other options are the captured ones.  Run one step (or load a state)
+    before the capture.  state_dict / load_state_dict keep the state's own types; with state_bits=32 a state saved by
+    torch.optim.AdamW loads."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32, master_weights=False):
+        defaults = dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits,
+                        master_weights=bool(master_weights))
+        self._flats = {}
+        super().__init__(params, defaults)
+
+    @staticmethod
+    def _check_options(g):
+        for k in ("lr", "eps", "weight_decay"):
+            if torch.is_tensor(g[k]):
+                raise TypeError(f"AdamW: {k} is a number here, not a tensor (it is a launch argument)")
+            if not 0.0 <= float(g[k]) < float("inf"):
+                raise ValueError(f"AdamW: {k} = {g[k]} is not a finite number >= 0")
+        if len(g["betas"]) != 2 or not all(0.0 <= float(b) < 1.0 for b in g["betas"]):
+            raise ValueError(f"AdamW: betas = {g['betas']} are not two numbers in [0, 1)")
+        if g["state_bits"] not in (32, 8):
+            raise ValueError(f"AdamW: state_bits is 32 or 8, not {g['state_bits']}")
+
+    def add_param_group(self, group):
+        super().add_param_group(group)
+        g = self.param_groups[-1]
+        try:
+            self._check_options(g)
+            for p in g["params"]:
+                if p.dtype not in _DT:
+                    raise TypeError(f"AdamW: parameters in float32, bfloat16 or float16, not {p.dtype}")
+                if p.layout != torch.strided or not p.is_contiguous():
+                    raise ValueError("AdamW: a parameter is not contiguous")
+        except Exception:
+            self.param_groups.pop()
+            raise
+
+    def _flat(self, gi):
+        fl = self._flats.get(gi)
+        if fl is None:
+            group = self.param_groups[gi]
+            if not group["params"]:
+                return None
+            ops._dev(*group["params"])
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("AdamW: the state does not exist yet: run one step or load a state before capturing a graph")
+            fl = self._flats[gi] = _Flat(group)
+            for i, p in enumerate(fl.params):
+                # an fp32 parameter is its own master
+                self.state[p] = {"step": 0, **{k: fl.view(k, i) for k in fl.buffers
+                                               if k != "master" or p.dtype != torch.float32}}
+        return fl
+
+    def state_buffers(self, group=0):
+        """The flat state arrays of a parameter group, the ones that the step updates: exp_avg, exp_avg_sq (fp32), or exp_avg,
+        exp_avg_sq_root (float8_e4m3fn) with their _scale arrays (fp32, one per 256 elements); master (fp32) where kept.  The
+        parameters follow each other in the group's order, each from a multiple of 256 on, with zeros behind it."""
+        fl = self._flat(group)
+        return {} if fl is None else dict(fl.buffers)
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        for gi, group in enumerate(self.param_groups):
+            fl = self._flat(gi)
+            if fl is not None:
+                self._step_group(group, fl)
+        return loss
+
+    def _step_group(self, group, fl):
+        self._check_options(group)
+        if len(group["params"]) != len(fl.params):
+            raise RuntimeError("AdamW: the parameters of a group changed after its first step")
+        if int(group["state_bits"]) != fl.bits or bool(group["master_weights"]) != fl.with_master:
+            raise RuntimeError("AdamW: state_bits and master_weights cannot change after a group's first step")
+        capturing = torch.cuda.is_current_stream_capturing()
+        if capturing:
+            fl.device_count = True
+        cur = torch.cuda.current_device()
+        batches, keep, touched = {}, [], []
+        for i, p in enumerate(group["params"]):
+            g = p.grad
+            if g is None:
+                continue
+            dt = p.dtype
+            if g.dtype is not dt or g.layout is not torch.strided or g.get_device() != cur or p.get_device() != cur \
+                    or p.numel() != fl.numels[i] or g.shape != p.shape or not p.is_contiguous():
+                self._refuse(i, p, g, fl, cur)
+            if not g.is_contiguous():
+                g = g.contiguous()
+                keep.append(g)                            # lives until the launch is enqueued; its memory is stream-ordered
+            touched.append(p)
+            if fl.numels[i]:
+                batches.setdefault((dt, 0 if fl.device_count else fl.steps[i] + 1), []).append(
+                    (p.data_ptr(), g.data_ptr(), fl.first[i], fl.numels[i], i))
+            fl.steps[i] += 1
+            self.state[p]["step"] = fl.steps[i]
+        b = fl.buffers
+        second = b["exp_avg_sq"] if fl.bits == 32 else b["exp_avg_sq_root"]
+        most = _lib.load().hd_adamw_max_jobs()
+        (b1, b2), lr, eps, wd = group["betas"], float(group["lr"]), float(group["eps"]), float(group["weight_decay"])
+        for (dt, t), jobs in batches.items():
+            master = b["master"] if fl.with_master and dt != torch.float32 else None
+            for k in range(0, len(jobs), most):
+                part = np.array(jobs[k:k + most], dtype=_JOB)
+                _lib.call("hd_adamw_step", part.ctypes.data, len(part), _DT[dt], fl.bits, ops._p(b["exp_avg"]), ops._p(second),
+                          ops._p(b.get("exp_avg_scale")), ops._p(b.get("exp_avg_sq_root_scale")), ops._p(master), fl.total,
+                          lr, float(b1), float(b2), eps, wd, t, ops._p(fl.table), len(fl.params), ops._stream())
+        # the kernel wrote behind autograd's back: the versions key the caches of weight copies, and a saved tensor must notice
+        torch.autograd.graph.increment_version(touched)
+
+    @staticmethod
+    def _refuse(i, p, g, fl, cur):
+        if p.get_device() != cur or g.get_device() != cur:
+            raise RuntimeError("AdamW: parameter %d is on %s, its gradient on %s, but the current device is cuda:%d"
+                               % (i, p.device, g.device, cur))
+        if g.layout is not torch.strided:
+            raise RuntimeError("AdamW: sparse gradients are not offered")
+        if g.dtype is not p.dtype:
+            raise TypeError("AdamW: parameter %d is %s, its gradient %s" % (i, p.dtype, g.dtype))
+        if g.shape != p.shape or p.numel() != fl.numels[i]:
+            raise ValueError("AdamW: parameter %d changed its size" % i)
+        raise ValueError("AdamW: parameter %d is not contiguous" % i)
+
+    # ---- replays of a captured step (dist.DataParallelTrainer.capture) ----
+    def replayed(self):
+        """To be called after a replay of a graph that holds step(): the parameters changed without the host's doing."""
+        torch.autograd.graph.increment_version([p for g in self.param_groups for p in g["params"] if p.grad is not None])
+
+    # ---- saving and loading: the state's own types, not the parameters' ----
+    def state_dict(self):
+        for fl in self._flats.values():
+            fl.refresh_steps()
+            for p, t in zip(fl.params, fl.steps):
+                self.state[p]["step"] = t
+        return super().state_dict()
+
+    def load_state_dict(self, state_dict):
+        saved = state_dict["state"]
+        ids = [i for g in state_dict["param_groups"] for i in g["params"]]
+        mine = [p for g in self.param_groups for p in g["params"]]
+        options = [{k: g[k] for k in _OPTIONS} for g in self.param_groups]
+        super().load_state_dict({**state_dict, "state": {}})
+        for g, o in zip(self.param_groups, options):
+            for k in _OPTIONS:
+                g.setdefault(k, o[k])                     # a state saved by torch.optim.AdamW has no state_bits
+            self._check_options(g)
+        self._flats = {}
+        at = 0
+        for gi, group in enumerate(self.param_groups):
+            part, at = list(zip(ids[at:], mine[at:]))[:len(group["params"])], at + len(group["params"])
+            if not any(pid in saved for pid, _ in part):
+                continue
+            fl = self._flat(gi)
+            for i, (pid, p) in enumerate(part):
+                st = saved.get(pid)
+                if not st:
+                    continue
+                for k in fl.buffers:
+                    if k == "master" and (k not in st or p.dtype == torch.float32):
+                        continue                          # taken from the parameter when the flat state was made
+                    if k not in st:
+                        raise ValueError(f"AdamW: the saved state has no {k} (state_bits={fl.bits})")
+                    dst, src = fl.view(k, i), st[k]
+                    if src.numel() != dst.numel():
+                        raise ValueError(f"AdamW: the saved {k} has {src.numel()} elements, not {dst.numel()}")
+                    if (src.dtype == torch.float8_e4m3fn) != (dst.dtype == torch.float8_e4m3fn):
+                        raise ValueError(f"AdamW: the saved {k} is {src.dtype}, not {dst.dtype}")
+                    with torch.no_grad():
+                        if dst.dtype == torch.float8_e4m3fn:
+                            dst.view(torch.uint8).copy_(src.to(dst.device).view(torch.uint8).reshape(dst.shape))
+                        else:
+                            dst.copy_(src.reshape(dst.shape))
+                fl.set_step(i, float(st["step"]))
+                self.state[p]["step"] = fl.steps[i]

@@ -35,6 +35,9 @@ typedef struct hd_curv {
     double c, sqrt_c, K, sqrt_K;
 } hd_curv;
 
+/* element types of the mixed-precision training operators */
+enum { HD_DT_F32 = 0, HD_DT_BF16 = 1, HD_DT_F16 = 2 };
+
 /* activation codes for the tangent-space activation of HypAct */
 enum { HD_ACT_IDENTITY = 0, HD_ACT_RELU = 1, HD_ACT_TANH = 2, HD_ACT_SIGMOID = 3, HD_ACT_ELU = 4,
        HD_ACT_LEAKY_RELU = 5 };
@@ -443,6 +446,25 @@ typedef struct hd_adam_job {
 } hd_adam_job;
 int hd_adam_step_f32(const hd_adam_job* jobs, int n_jobs, const void* grad_flat, void* exp_avg_flat, void* exp_avg_sq_flat,
                      double lr, double beta1, double beta2, double eps, int64_t step, void* step_state, void* stream);
+/* One step of AdamW (decoupled weight decay) over up to hd_adamw_max_jobs() parameter tensors in ONE launch:
+ *   m = b1 m + (1-b1) g;  v = b2 v + (1-b2) g^2;  p = p (1 - lr wd) - lr/(1-b1^t) * m / (sqrt(v)/sqrt(1-b2^t) + eps)   (fp32)
+ * Job i: `count` elements of type `dtype` (HD_DT_*) at param / grad, contiguous, aligned to the element; its state is the
+ * segment [first, first + count) of the flat state arrays of state_elems elements, `first` and state_elems multiples of 256
+ * and segments of whole 256-element blocks (the padding holds zeros and keeps them).  state_bits 32: exp_avg = m and
+ * exp_avg_sq = v in fp32 (the scales NULL).  state_bits 8: exp_avg = m and exp_avg_sq = sqrt(v) as e4m3 bytes, with one fp32
+ * scale per block in exp_avg_scale / exp_avg_sq_scale.  master (fp32, flat like the state, or NULL; 16-bit types only): the
+ * weights themselves, param receives their rounding.  step >= 1: the step being taken, and row `row` of step_table
+ * (step_rows x 3 doubles, or NULL) receives it; step 0: the count is step_table[row][0], advanced by this call (a captured
+ * call replays with the right bias corrections).  No two jobs of a call may share a row or a segment. */
+typedef struct hd_adamw_job {
+    void* param;
+    const void* grad;
+    int64_t first, count, row;
+} hd_adamw_job;
+int64_t hd_adamw_max_jobs(void);
+int hd_adamw_step(const hd_adamw_job* jobs, int n_jobs, int dtype, int state_bits, void* exp_avg, void* exp_avg_sq,
+                  void* exp_avg_scale, void* exp_avg_sq_scale, void* master, int64_t state_elems, double lr, double beta1,
+                  double beta2, double eps, double weight_decay, int64_t step, void* step_table, int64_t step_rows, void* stream);
 /* The same weight gradient (and bias gradient) from bf16x3 limb IMAGES of A (R x P) and B (R x Q) -- the images the
  * forward and input-gradient launches of hd_gemm_limbs_train_f32 write anyway, so training keeps no fp32 copies of dz or
  * of the layer inputs.  The contraction runs over image rows (LDS-DMA + ds_read_b64_tr_b16 transposing reads); the pad
