@@ -31,6 +31,9 @@ class _Flat:
         self.steps = [0] * len(self.params)              # steps taken by each parameter, as the host counts them
         self.table = torch.zeros(len(self.params), 3, dtype=torch.float64, device=dev)     # the device's count
         self.device_count = False                        # True once a step was captured: the device's count is the true one
+        self.jobs = np.zeros(len(self.params), dtype=_JOB)     # the launch arguments; a step fills in the pointers
+        self.jobs["first"], self.jobs["count"], self.jobs["row"] = self.first, self.numels, range(len(self.params))
+        self.checked, self.states = None, []
         self.buffers = {}
         if self.bits == 32:
             self.buffers["exp_avg"] = torch.zeros(at, dtype=torch.float32, device=dev)
@@ -41,8 +44,8 @@ class _Flat:
                 self.buffers[k + "_scale"] = torch.zeros(at // BLOCK, dtype=torch.float32, device=dev)
         if self.with_master:
             m = self.buffers["master"] = torch.zeros(at, dtype=torch.float32, device=dev)
-            for p, a, n in zip(self.params, self.first, self.numels):
-                m[a:a + n].copy_(p.detach().reshape(-1))
+            torch._foreach_copy_([m[a:a + n] for a, n in zip(self.first, self.numels)],
+                                 [p.detach().reshape(-1) for p in self.params])
 
     def view(self, key, i):
         """parameter i's part of a buffer: its shape, or one value per block for the scales"""
@@ -53,11 +56,14 @@ class _Flat:
 
     def refresh_steps(self):
         if self.device_count:                            # replays of a captured step counted on the device alone
-            self.steps = [int(t) for t in self.table[:, 0].tolist()]
+            self.set_steps([int(t) for t in self.table[:, 0].tolist()], False)
 
-    def set_step(self, i, t):
-        self.steps[i] = int(t)
-        self.table[i, 0] = float(int(t))
+    def set_steps(self, steps, device=True):
+        self.steps = steps
+        for st, t in zip(self.states, steps):
+            st["step"] = t
+        if device:
+            self.table[:, 0] = torch.tensor(steps, dtype=torch.float64)
 
 
 class AdamW(torch.optim.Optimizer):
@@ -126,8 +132,9 @@ class AdamW(torch.optim.Optimizer):
             fl = self._flats[gi] = _Flat(group)
             for i, p in enumerate(fl.params):
                 # an fp32 parameter is its own master
-                self.state[p] = {"step": 0, **{k: fl.view(k, i) for k in fl.buffers
-                                               if k != "master" or p.dtype != torch.float32}}
+                fl.states.append(self.state[p])
+                fl.states[-1].update({"step": 0, **{k: fl.view(k, i) for k in fl.buffers
+                                                      if k != "master" or p.dtype != torch.float32}})
         return fl
 
     def state_buffers(self, group=0):
@@ -150,46 +157,60 @@ class AdamW(torch.optim.Optimizer):
         return loss
 
     def _step_group(self, group, fl):
-        self._check_options(group)
-        if len(group["params"]) != len(fl.params):
+        # the host's part is most of a small model's step: about 0.9 us a tensor and 15 us besides
+        options = (group["lr"], group["betas"], group["eps"], group["weight_decay"], group["state_bits"], group["master_weights"])
+        if fl.checked != options:
+            self._check_options(group)
+            if int(group["state_bits"]) != fl.bits or bool(group["master_weights"]) != fl.with_master:
+                raise RuntimeError("AdamW: state_bits and master_weights cannot change after a group's first step")
+            fl.checked = options
+        params = group["params"]
+        if len(params) != len(fl.params):
             raise RuntimeError("AdamW: the parameters of a group changed after its first step")
-        if int(group["state_bits"]) != fl.bits or bool(group["master_weights"]) != fl.with_master:
-            raise RuntimeError("AdamW: state_bits and master_weights cannot change after a group's first step")
-        capturing = torch.cuda.is_current_stream_capturing()
-        if capturing:
+        if torch.cuda.is_current_stream_capturing():
             fl.device_count = True
+        counted = fl.device_count
         cur = torch.cuda.current_device()
+        steps, states, numels = fl.steps, fl.states, fl.numels
         batches, keep, touched = {}, [], []
-        for i, p in enumerate(group["params"]):
+        for i, p in enumerate(params):
             g = p.grad
             if g is None:
                 continue
-            dt = p.dtype
-            if g.dtype is not dt or g.layout is not torch.strided or g.get_device() != cur or p.get_device() != cur \
-                    or p.numel() != fl.numels[i] or g.shape != p.shape or not p.is_contiguous():
+            dt, n = p.dtype, numels[i]
+            if g.dtype is not dt or g.get_device() != cur or p.get_device() != cur or g.layout is not torch.strided \
+                    or p.numel() != n or g.numel() != n or not p.is_contiguous():
                 self._refuse(i, p, g, fl, cur)
             if not g.is_contiguous():
                 g = g.contiguous()
                 keep.append(g)                            # lives until the launch is enqueued; its memory is stream-ordered
-            touched.append(p)
-            if fl.numels[i]:
-                batches.setdefault((dt, 0 if fl.device_count else fl.steps[i] + 1), []).append(
-                    (p.data_ptr(), g.data_ptr(), fl.first[i], fl.numels[i], i))
-            fl.steps[i] += 1
-            self.state[p]["step"] = fl.steps[i]
+            t = steps[i] + 1
+            touched.append((i, p, t))
+            if n:
+                # one launch has one element type and one step count
+                b = batches.get((dt, 0 if counted else t))
+                if b is None:
+                    b = batches[(dt, 0 if counted else t)] = ([], [], [])
+                b[0].append(i)
+                b[1].append(p.data_ptr())
+                b[2].append(g.data_ptr())
         b = fl.buffers
         second = b["exp_avg_sq"] if fl.bits == 32 else b["exp_avg_sq_root"]
         most = _lib.load().hd_adamw_max_jobs()
         (b1, b2), lr, eps, wd = group["betas"], float(group["lr"]), float(group["eps"]), float(group["weight_decay"])
-        for (dt, t), jobs in batches.items():
+        for (dt, t), (rows, ptrs, grads) in batches.items():
             master = b["master"] if fl.with_master and dt != torch.float32 else None
-            for k in range(0, len(jobs), most):
-                part = np.array(jobs[k:k + most], dtype=_JOB)
-                _lib.call("hd_adamw_step", part.ctypes.data, len(part), _DT[dt], fl.bits, ops._p(b["exp_avg"]), ops._p(second),
-                          ops._p(b.get("exp_avg_scale")), ops._p(b.get("exp_avg_sq_root_scale")), ops._p(master), fl.total,
-                          lr, float(b1), float(b2), eps, wd, t, ops._p(fl.table), len(fl.params), ops._stream())
+            jobs = fl.jobs if len(rows) == len(params) else fl.jobs[rows]
+            jobs["param"], jobs["grad"] = ptrs, grads
+            for k in range(0, len(rows), most):
+                _lib.call("hd_adamw_step", jobs.ctypes.data + k * _JOB.itemsize, min(most, len(rows) - k), _DT[dt], fl.bits,
+                          ops._p(b["exp_avg"]), ops._p(second), ops._p(b.get("exp_avg_scale")),
+                          ops._p(b.get("exp_avg_sq_root_scale")), ops._p(master), fl.total, lr, float(b1), float(b2), eps, wd, t,
+                          ops._p(fl.table), len(params), ops._stream())
+        for i, _, t in touched:                           # counted once the launches are under way
+            steps[i] = states[i]["step"] = t
         # the kernel wrote behind autograd's back: the versions key the caches of weight copies, and a saved tensor must notice
-        torch.autograd.graph.increment_version(touched)
+        torch.autograd.graph.increment_version([p for _, p, _ in touched])
 
     @staticmethod
     def _refuse(i, p, g, fl, cur):
@@ -200,7 +221,7 @@ class AdamW(torch.optim.Optimizer):
             raise RuntimeError("AdamW: sparse gradients are not offered")
         if g.dtype is not p.dtype:
             raise TypeError("AdamW: parameter %d is %s, its gradient %s" % (i, p.dtype, g.dtype))
-        if g.shape != p.shape or p.numel() != fl.numels[i]:
+        if g.numel() != p.numel() or p.numel() != fl.numels[i]:
             raise ValueError("AdamW: parameter %d changed its size" % i)
         raise ValueError("AdamW: parameter %d is not contiguous" % i)
 
@@ -210,11 +231,12 @@ class AdamW(torch.optim.Optimizer):
         torch.autograd.graph.increment_version([p for g in self.param_groups for p in g["params"] if p.grad is not None])
 
     # ---- saving and loading: the state's own types, not the parameters' ----
+    def __getstate__(self):
+        raise TypeError("AdamW: save or copy state_dict(), not the optimizer (its state lives in shared flat arrays)")
+
     def state_dict(self):
         for fl in self._flats.values():
             fl.refresh_steps()
-            for p, t in zip(fl.params, fl.steps):
-                self.state[p]["step"] = t
         return super().state_dict()
 
     def load_state_dict(self, state_dict):
@@ -227,6 +249,8 @@ class AdamW(torch.optim.Optimizer):
             for k in _OPTIONS:
                 g.setdefault(k, o[k])                     # a state saved by torch.optim.AdamW has no state_bits
             self._check_options(g)
+            if g.get("amsgrad") or g.get("maximize"):
+                raise ValueError("AdamW: the saved options ask for amsgrad or maximize, which are not offered")
         self._flats = {}
         at = 0
         for gi, group in enumerate(self.param_groups):
@@ -234,6 +258,7 @@ class AdamW(torch.optim.Optimizer):
             if not any(pid in saved for pid, _ in part):
                 continue
             fl = self._flat(gi)
+            steps, to, frm = list(fl.steps), [], []
             for i, (pid, p) in enumerate(part):
                 st = saved.get(pid)
                 if not st:
@@ -248,10 +273,12 @@ class AdamW(torch.optim.Optimizer):
                         raise ValueError(f"AdamW: the saved {k} has {src.numel()} elements, not {dst.numel()}")
                     if (src.dtype == torch.float8_e4m3fn) != (dst.dtype == torch.float8_e4m3fn):
                         raise ValueError(f"AdamW: the saved {k} is {src.dtype}, not {dst.dtype}")
-                    with torch.no_grad():
-                        if dst.dtype == torch.float8_e4m3fn:
-                            dst.view(torch.uint8).copy_(src.to(dst.device).view(torch.uint8).reshape(dst.shape))
-                        else:
-                            dst.copy_(src.reshape(dst.shape))
-                fl.set_step(i, float(st["step"]))
-                self.state[p]["step"] = fl.steps[i]
+                    if dst.dtype == torch.float8_e4m3fn:
+                        dst, src = dst.view(torch.uint8), src.view(torch.uint8)
+                    to.append(dst)
+                    frm.append(src.detach().to(dst.device).reshape(dst.shape))
+                steps[i] = int(st["step"])
+            if to:
+                with torch.no_grad():
+                    torch._foreach_copy_(to, frm)
+            fl.set_steps(steps)

@@ -314,6 +314,11 @@ def test_refusals_on_the_host():
     p.grad = torch.ones(4)
     with pytest.raises(RuntimeError, match="no CPU fallback"):
         AdamW([p]).step()
+    with pytest.raises(TypeError, match="state_dict"):
+        copy.deepcopy(AdamW([p]))
+    sd = torch.optim.AdamW([p], amsgrad=True).state_dict()
+    with pytest.raises(ValueError, match="amsgrad"):
+        AdamW([p]).load_state_dict(sd)
 
 
 def test_refusals_of_the_entry_point():
