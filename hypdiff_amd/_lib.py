@@ -82,6 +82,7 @@ SIZE_QUERIES = {
     "hd_chain_workspace_bytes": [],
     "hd_mlp_chain_workspace_bytes": [I64, c_int],
     "hd_adamw_max_jobs": [],
+    "hd_embedding_sum_workspace_bytes": [I64, I64, I64, c_int],
 }
 
 # name -> argtypes; names ending in "*" exist as _f32 and _f64
@@ -173,6 +174,8 @@ SIGNATURES = {
     "hd_ddpm_step": [P, P, P, c_double, c_double, c_double, P, I64, P],
     "hd_embedding_add": [P, P, P, I64, I64, I64, P],
     "hd_embedding_grad_f32": [P, P, P, I64, I64, I64, P, P],
+    "hd_embedding_lookup": [P, I64, P, c_int, P, I64, c_double, c_int, I64, I64, I64, P, P],
+    "hd_embedding_sum": [P, I64, P, c_int, I64, c_double, c_int, I64, I64, I64, P, P, I64, P],
     "hd_generate_adj_f32": [P, P, P, I64, I64, P],
     "hd_hkm_to_hyperboloid": [P, P, I64, I64, P],
     "hd_hkm_mean_step": [P, P, P, I64, I64, I64, c_double, P, P],

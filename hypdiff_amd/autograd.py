@@ -18,6 +18,7 @@ PyTorch owns memory, the autograd graph and RNG (and the optimizer unless dist.B
 import os
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib, ops
 
@@ -496,6 +497,24 @@ class EmbeddingAdd(torch.autograd.Function):
         _lib.call("hd_embedding_grad_f32", ops._p(g), ops._p(order.values), ops._p(order.indices.contiguous()), g.shape[0],
                   g.shape[1], ctx.T, ops._p(gt), ops._stream())
         return g, gt, None
+
+
+class Embedding(torch.autograd.Function):
+    """add + scale * table[idx] in the table's type (ops.embedding).  Backward: hd_embedding_sum for the table, the
+    incoming gradient itself for add."""
+
+    @staticmethod
+    def forward(ctx, table, add, idx, scale, padding):
+        ctx.save_for_backward(idx)
+        ctx.scale, ctx.padding, ctx.T = scale, padding, table.shape[0]
+        return ops._embedding_lookup(table, idx, scale, add)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        (idx,) = ctx.saved_tensors
+        gt = ops._embedding_sum(g, idx, ctx.T, ctx.scale, ctx.padding) if ctx.needs_input_grad[0] else None
+        return gt, g if ctx.needs_input_grad[1] else None, None, None, None
 
 
 class MSELoss(torch.autograd.Function):

@@ -1,0 +1,533 @@
+// Embedding lookup  out[r] = add[r] + scale * table[idx[r]]  and its table gradient  dT[v] = scale * sum_{idx[r] = v} g[r],
+// in fp32, bf16 or fp16 (the sums in fp32, rounded once).  The time embedding of the graph-level denoiser (ddpm.py:36-41)
+// is such a lookup; hd_embedding_add / hd_embedding_grad_f32 are its fp32 form for a caller that sorts by itself.
+//
+// The gradient is a segment sum over the rows of g in the order of a stable sort by token: every table row is written once,
+// by one lane per column, so there are no atomics on floats, the sums run in ascending row order inside fixed chunks, and
+// a repeated call gives the same bits.
+//   sort    key = token (the padding token and tokens outside the table become T, behind all others), value = row.  Up to
+//           4096 rows: one workgroup, bitonic on (key, row) in LDS.  More: least-significant-digit radix passes of at most
+//           8 bits; a workgroup counts its own digits' places from the counts of all workgroups (at most 256 of them, one
+//           read of 256 KB) and the scatter of a pass counts the next pass's digits, so p passes are p + 1 launches.
+//   sum     the sorted rows are cut into chunks of P; a lane owns VEC columns, walks a chunk and writes a table row
+//           whenever a run ends.  A run that crosses a chunk's border leaves a partial sum there, which the next launch
+//           adds up in chunk order: a hot token (18 000 of 75 000 rows) is spread over hundreds of wavefronts.  Further
+//           workgroups of the same launch write the zeros of the table rows that no row names.
+// Bound by HBM: one read of g and one write of the table's gradient (the lookup: one read of the named rows, one write).
+#include <type_traits>
+#include "hd_common.cuh"
+#include "hd_half.cuh"
+#include "../../include/hypdiff.h"
+
+using namespace hd;
+
+namespace {
+
+constexpr int kSmallRows = 4096;                    // rows that one workgroup sorts
+constexpr int kSortWg = 1024;
+constexpr int kMaxSortWgs = 256;
+constexpr int kZeroRows = 64;                       // table rows of one zero-writing workgroup
+
+// ---- lookup ---------------------------------------------------------------------------------------------------------------
+template <typename T, int VEC, typename I>
+__global__ __launch_bounds__(256) void lookup_k(const T* __restrict__ table, long long ldt, const I* __restrict__ idx,
+                                                const T* __restrict__ add, long long lda, float scale, long long n_table,
+                                                long long rows, int dim, int log2_lanes, T* __restrict__ out) {
+    const int lanes = 1 << log2_lanes;                                        // lanes of a row (a power of two up to 256)
+    const long long r = (long long)blockIdx.x * (256 >> log2_lanes) + (threadIdx.x >> log2_lanes);
+    if (r >= rows) return;
+    const long long t = (long long)idx[r];
+    const bool inside = t >= 0 && t < n_table;                                // outside the table: a row of NaN
+    const T* src = table + (inside ? t : 0) * ldt;
+    for (int c = (threadIdx.x & (lanes - 1)) * VEC; c < dim; c += lanes * VEC) {
+        if (c + VEC <= dim) {
+            const Pack<T, VEC> a = load_pack<T, VEC>(src + c);
+            Pack<T, VEC> o;
+            if (add) {
+                const Pack<T, VEC> b = load_pack<T, VEC>(add + r * lda + c);
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) o.v[e] = (T)(inside ? (float)b.v[e] + scale * (float)a.v[e] : __builtin_nanf(""));
+            } else {
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) o.v[e] = (T)(inside ? scale * (float)a.v[e] : __builtin_nanf(""));
+            }
+            store_pack<T, VEC>(out + r * dim + c, o);
+        } else {
+            for (int k = c; k < dim; ++k) {
+                float v = scale * (float)src[k];
+                if (add) v = (float)add[r * lda + k] + v;
+                out[r * dim + k] = (T)(inside ? v : __builtin_nanf(""));
+            }
+        }
+    }
+}
+
+// ---- sort -----------------------------------------------------------------------------------------------------------------
+template <typename I>
+__device__ __forceinline__ unsigned key_of(I t, long long padding, unsigned n_table) {
+    const long long v = (long long)t;
+    return v >= 0 && v < (long long)n_table && v != padding ? (unsigned)v : n_table;
+}
+
+template <typename I>
+__global__ __launch_bounds__(kSortWg) void sort_small_k(const I* __restrict__ idx, long long padding, unsigned n_table, int n, int n2,
+                                                        unsigned* __restrict__ keys, unsigned* __restrict__ pos) {
+    __shared__ unsigned long long s[kSmallRows];
+    for (int i = threadIdx.x; i < n2; i += kSortWg)
+        s[i] = i < n ? ((unsigned long long)key_of(idx[i], padding, n_table) << 32) | (unsigned)i : ~0ull;
+    __syncthreads();
+    for (int k = 2; k <= n2; k <<= 1)
+        for (int j = k >> 1; j > 0; j >>= 1) {
+            for (int i = threadIdx.x; i < n2 >> 1; i += kSortWg) {
+                const int a = ((i & ~(j - 1)) << 1) | (i & (j - 1)), b = a | j;
+                const unsigned long long x = s[a], y = s[b];
+                if ((x > y) == ((a & k) == 0)) { s[a] = y; s[b] = x; }
+            }
+            __syncthreads();
+        }
+    for (int i = threadIdx.x; i < n; i += kSortWg) {
+        keys[i] = (unsigned)(s[i] >> 32);
+        pos[i] = (unsigned)s[i];
+    }
+}
+
+// digit counts of the first pass, [workgroup][256]; clears the counts of the further passes
+template <typename I>
+__global__ __launch_bounds__(kSortWg) void radix_count_k(const I* __restrict__ idx, long long padding, unsigned n_table, unsigned n,
+                                                         unsigned per_wg, unsigned mask, unsigned* __restrict__ hist,
+                                                         unsigned more_words) {
+    __shared__ unsigned h[256];
+    if (threadIdx.x < 256) h[threadIdx.x] = 0;
+    __syncthreads();
+    const unsigned i0 = blockIdx.x * per_wg, i1 = n - i0 < per_wg ? n : i0 + per_wg;
+    for (unsigned i = i0 + threadIdx.x; i < i1; i += kSortWg) atomicAdd(&h[key_of(idx[i], padding, n_table) & mask], 1u);
+    __syncthreads();
+    if (threadIdx.x < 256) hist[blockIdx.x * 256 + threadIdx.x] = h[threadIdx.x];
+    unsigned* more = hist + gridDim.x * 256;
+    for (unsigned i = blockIdx.x * kSortWg + threadIdx.x; i < more_words; i += gridDim.x * kSortWg) more[i] = 0;
+}
+
+// One stable scatter by the digit (key >> shift) & mask.  FIRST: keys come from idx.  next: the counts of the next pass
+// ([workgroup][256], integers: the order of the additions does not matter), or NULL after the last.
+template <typename I, bool FIRST>
+__global__ __launch_bounds__(kSortWg) void radix_scatter_k(const I* __restrict__ idx, long long padding, unsigned n_table,
+                                                           const unsigned* __restrict__ keys_in, const unsigned* __restrict__ pos_in,
+                                                           unsigned n, unsigned per_wg, int shift, unsigned mask, int next_shift,
+                                                           unsigned next_mask, const unsigned* __restrict__ hist,
+                                                           unsigned* __restrict__ next, unsigned* __restrict__ keys_out,
+                                                           unsigned* __restrict__ pos_out) {
+    __shared__ unsigned part_all[4][256], part_before[4][256], place[256], wave_count[16][256];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, digit = tid & 255, quarter = tid >> 8;
+    // where this workgroup's rows of each digit go: all rows of smaller digits, then the earlier workgroups' of this digit
+    unsigned all = 0, before = 0;
+#pragma unroll 8
+    for (unsigned b = quarter; b < gridDim.x; b += 4) {
+        const unsigned c = hist[b * 256 + digit];
+        all += c;
+        before += b < blockIdx.x ? c : 0u;
+    }
+    part_all[quarter][digit] = all;
+    part_before[quarter][digit] = before;
+    __syncthreads();
+    if (tid < 64) {                                                           // exclusive scan over 256 digits, 4 a lane
+        unsigned c[4], sum = 0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int d = tid * 4 + k;
+            c[k] = part_all[0][d] + part_all[1][d] + part_all[2][d] + part_all[3][d];
+            sum += c[k];
+        }
+        unsigned run = sum;
+        for (int o = 1; o < 64; o <<= 1) {
+            const unsigned up = (unsigned)__shfl_up((int)run, o);
+            if (tid >= o) run += up;
+        }
+        run -= sum;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int d = tid * 4 + k;
+            place[d] = run + part_before[0][d] + part_before[1][d] + part_before[2][d] + part_before[3][d];
+            run += c[k];
+        }
+    }
+    const unsigned i0 = blockIdx.x * per_wg, i1 = n - i0 < per_wg ? n : i0 + per_wg;
+    for (unsigned r = i0; r < i1; r += kSortWg) {                              // rounds of 1024 rows in order
+        for (int k = tid; k < 16 * 256; k += kSortWg) (&wave_count[0][0])[k] = 0;
+        __syncthreads();                                                      // (also: place is complete / was advanced)
+        const unsigned i = r + tid;
+        const bool live = i < i1;
+        unsigned key = 0, row = i;
+        if (live) {
+            if constexpr (FIRST) key = key_of(idx[i], padding, n_table);
+            else { key = keys_in[i]; row = pos_in[i]; }
+        }
+        const unsigned d = (key >> shift) & mask;
+        // the lanes of this wavefront with the same digit
+        unsigned long long same = __ballot(live);
+#pragma unroll
+        for (int bit = 0; bit < 8; ++bit) {
+            const unsigned long long m = __ballot(live && ((d >> bit) & 1));
+            same &= (d >> bit) & 1 ? m : ~m;
+        }
+        const unsigned rank = (unsigned)__popcll(same & ((1ull << lane) - 1));
+        if (live && rank == 0) wave_count[wave][d] = (unsigned)__popcll(same);
+        __syncthreads();
+        if (tid < 256) {                                                      // first place of every wavefront's rows of a digit
+            unsigned p = place[tid];
+#pragma unroll
+            for (int w = 0; w < 16; ++w) {
+                const unsigned c = wave_count[w][tid];
+                wave_count[w][tid] = p;
+                p += c;
+            }
+            place[tid] = p;
+        }
+        __syncthreads();
+        if (live) {
+            const unsigned to = wave_count[wave][d] + rank;
+            keys_out[to] = key;
+            pos_out[to] = row;
+            if (next) atomicAdd(&next[to / per_wg * 256 + ((key >> next_shift) & next_mask)], 1u);
+        }
+        __syncthreads();
+    }
+}
+
+// ---- sum ------------------------------------------------------------------------------------------------------------------
+__device__ __forceinline__ unsigned lower_bound(const unsigned* keys, unsigned n, unsigned v) {
+    unsigned lo = 0, hi = n;
+    while (lo < hi) {
+        const unsigned mid = lo + ((hi - lo) >> 1);
+        if (keys[mid] < v) lo = mid + 1; else hi = mid;
+    }
+    return lo;
+}
+
+template <int VEC>
+__device__ __forceinline__ void store_part(float* p, const float (&acc)[VEC], int c, int dim) {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e)
+        if (c + e < dim) p[c + e] = acc[e];
+}
+template <typename T, int VEC>
+__device__ __forceinline__ void store_row(T* p, const float (&acc)[VEC], float scale, int c, int dim) {
+    if (c + VEC <= dim) {
+        Pack<T, VEC> o;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) o.v[e] = (T)(acc[e] * scale);
+        store_pack<T, VEC>(p + c, o);
+    } else {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e)
+            if (c + e < dim) p[c + e] = (T)(acc[e] * scale);
+    }
+}
+
+// head[chunk]: the sum of the chunk's rows that continue the run of the chunk before; tail[chunk]: of the run that begins in
+// the chunk and goes on in the next.  A lane owns the columns c .. c + VEC - 1 of one chunk.
+template <typename T, int VEC>
+__global__ __launch_bounds__(256) void segment_sum_k(const T* __restrict__ g, long long ldg, const unsigned* __restrict__ keys,
+                                                     const unsigned* __restrict__ pos, unsigned n, int dim, unsigned n_table,
+                                                     float scale, int chunk, int log2_lanes, int tiles, unsigned sum_wgs,
+                                                     T* __restrict__ out, float* __restrict__ head, float* __restrict__ tail) {
+    if (blockIdx.x >= sum_wgs) {                                              // zeros of the table rows that nothing names
+        __shared__ unsigned present[kZeroRows];
+        __shared__ unsigned range[2];
+        const unsigned t0 = (blockIdx.x - sum_wgs) * kZeroRows;
+        const unsigned t1 = n_table - t0 < kZeroRows ? n_table : t0 + kZeroRows;
+        if (threadIdx.x < kZeroRows) present[threadIdx.x] = 0;
+        if (threadIdx.x < 2) range[threadIdx.x] = lower_bound(keys, n, threadIdx.x ? t1 : t0);
+        __syncthreads();
+        const unsigned a = range[0], b = range[1];
+        for (unsigned i = a + threadIdx.x; i < b; i += 256) present[keys[i] - t0] = 1;
+        __syncthreads();
+        const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+        const float zero[VEC] = {};
+        for (unsigned t = t0 + wave; t < t1; t += 4)
+            if (!present[t - t0])
+                for (int c = lane * VEC; c < dim; c += 64 * VEC) store_row<T, VEC>(out + (long long)t * dim, zero, 1.f, c, dim);
+        return;
+    }
+    const unsigned item = blockIdx.x * (256u >> log2_lanes) + (threadIdx.x >> log2_lanes);
+    const unsigned ch = item / (unsigned)tiles;
+    const int c = ((int)(item - ch * tiles) * (1 << log2_lanes) + (int)(threadIdx.x & ((1 << log2_lanes) - 1))) * VEC;
+    const unsigned i0 = ch * chunk;
+    if (i0 >= n || c >= dim) return;
+    const unsigned i1 = n - i0 < (unsigned)chunk ? n : i0 + chunk;
+    const bool whole = c + VEC <= dim;
+    const unsigned after = i1 < n ? keys[i1] : ~0u;
+    unsigned cur = keys[i0];
+    bool cont = i0 > 0 && keys[i0 - 1] == cur;                                // the run began in an earlier chunk
+    float acc[VEC] = {};
+    constexpr int U = 8;                                                      // rows in flight
+    for (unsigned i = i0; i < i1; i += U) {
+        unsigned k[U], p[U];
+        Pack<T, VEC> x[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const unsigned j = i + u < i1 ? i + u : i1 - 1;
+            k[u] = i + u < i1 ? keys[j] : ~0u;
+            p[u] = pos[j];
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const T* src = g + (long long)p[u] * ldg + c;
+            if (whole) {
+                x[u] = load_pack<T, VEC>(src);
+            } else {
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) x[u].v[e] = c + e < dim ? src[e] : (T)0.f;
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (k[u] == ~0u) break;
+            if (k[u] != cur) {                                                // the run of cur is over
+                if (cont) store_part<VEC>(head + (long long)ch * dim, acc, c, dim);
+                else if (cur < n_table) store_row<T, VEC>(out + (long long)cur * dim, acc, scale, c, dim);
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) acc[e] = 0.f;
+                cur = k[u];
+                cont = false;
+            }
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) acc[e] += (float)x[u].v[e];
+        }
+    }
+    if (cont) store_part<VEC>(head + (long long)ch * dim, acc, c, dim);
+    else if (after == cur) store_part<VEC>(tail + (long long)ch * dim, acc, c, dim);
+    else if (cur < n_table) store_row<T, VEC>(out + (long long)cur * dim, acc, scale, c, dim);
+}
+
+// Runs that cross chunks: tail of the chunk where the run begins, then the heads up to the chunk where it ends, in order;
+// four wavefronts take a quarter of the heads each.  One workgroup per (chunk, 64 columns); chunks without a tail leave at once.
+template <typename T>
+__global__ __launch_bounds__(256) void segment_join_k(const unsigned* __restrict__ keys, unsigned n, int dim, unsigned n_table,
+                                                      float scale, int chunk, int tiles, const float* __restrict__ head,
+                                                      const float* __restrict__ tail, T* __restrict__ out) {
+    __shared__ float red[4][64];
+    __shared__ unsigned last;
+    const unsigned ch = blockIdx.x / (unsigned)tiles;
+    const unsigned i0 = ch * chunk, i1 = i0 + chunk;                          // the last chunk has no tail: not launched for it
+    const unsigned cur = keys[i1 - 1];
+    if (cur >= n_table || keys[i1] != cur || (keys[i0] == cur && i0 > 0 && keys[i0 - 1] == cur)) return;
+    if (threadIdx.x == 0) last = (lower_bound(keys, n, cur + 1) - 1) / (unsigned)chunk;
+    __syncthreads();
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const int c = (int)(blockIdx.x - ch * tiles) * 64 + lane;
+    const unsigned heads = last - ch, per = (heads + 3) / 4;
+    const unsigned a = ch + 1 + wave * per, b = a + per < last + 1 ? a + per : last + 1;
+    float acc = 0.f;
+    if (c < dim) {
+        if (wave == 0) acc = tail[(long long)ch * dim + c];
+#pragma unroll 8
+        for (unsigned k = a; k < b; ++k) acc += head[(long long)k * dim + c];
+    }
+    red[wave][lane] = acc;
+    __syncthreads();
+    if (wave == 0 && c < dim)
+        out[(long long)cur * dim + c] = (T)((((red[0][lane] + red[1][lane]) + red[2][lane]) + red[3][lane]) * scale);
+}
+
+// ---- host side ------------------------------------------------------------------------------------------------------------
+inline int ceil_log2(int64_t v) {
+    int l = 0;
+    while ((int64_t(1) << l) < v) ++l;
+    return l;
+}
+
+// columns of a lane: the widest load (16 bytes at most) that leaves at most a quarter of the lanes without columns
+inline int pick_vec(int64_t dim, int most) {
+    for (int v = most; v > 1; v >>= 1) {
+        const int64_t used = (dim + v - 1) / v, lanes = used > 64 ? (used + 63) / 64 * 64 : int64_t(1) << ceil_log2(used);
+        if (4 * used >= 3 * lanes && dim >= v) return v;
+    }
+    return 1;
+}
+
+struct Plan {
+    int vec, log2_lanes, tiles, chunk;
+    int64_t chunks;
+    int passes, width, sort_wgs;
+    int64_t per_wg;
+    int64_t off_pos, off_keys2, off_pos2, off_hist, off_head, off_tail, bytes;
+};
+
+Plan make_plan(int64_t rows, int64_t dim, int64_t n_table, int dt) {
+    Plan p;
+    p.vec = pick_vec(dim, dt == HD_DT_F32 ? 4 : 8);
+    const int64_t used = (dim + p.vec - 1) / p.vec;
+    p.log2_lanes = used >= 64 ? 6 : ceil_log2(used);
+    p.tiles = (int)((used + (1 << p.log2_lanes) - 1) >> p.log2_lanes);
+    // chunks long enough that the partial sums are a small part of the traffic (2 / 64 at the border of every chunk) and
+    // short enough that a small batch still fills the chip
+    const int64_t lanes_per_row = (int64_t)p.tiles << p.log2_lanes;
+    p.chunk = 8;
+    while (p.chunk < 64 && rows * lanes_per_row / (2 * p.chunk) >= 4096 * 64) p.chunk *= 2;
+    p.chunks = (rows + p.chunk - 1) / p.chunk;
+    const int bits = ceil_log2(n_table + 1) > 0 ? ceil_log2(n_table + 1) : 1;     // keys are 0 .. n_table
+    p.passes = (bits + 7) / 8;
+    p.width = (bits + p.passes - 1) / p.passes;
+    int64_t per = (rows + kMaxSortWgs - 1) / kMaxSortWgs;
+    per = (per + kSortWg - 1) / kSortWg * kSortWg;
+    p.per_wg = per < kSortWg ? kSortWg : per;
+    p.sort_wgs = (int)((rows + p.per_wg - 1) / p.per_wg);
+    const bool small = rows <= kSmallRows;
+    auto up = [](int64_t b) { return (b + 255) / 256 * 256; };
+    int64_t at = up(rows * 4);                                                   // the sorted keys come first
+    p.off_pos = at;
+    at += up(rows * 4);
+    p.off_keys2 = at;
+    at += small ? 0 : up(rows * 4);
+    p.off_pos2 = at;
+    at += small ? 0 : up(rows * 4);
+    p.off_hist = at;
+    at += small ? 0 : up((int64_t)p.passes * p.sort_wgs * 256 * 4);
+    p.off_head = at;
+    at += up(p.chunks * dim * 4);
+    p.off_tail = at;
+    at += up(p.chunks * dim * 4);
+    p.bytes = at > 256 ? at : 256;
+    return p;
+}
+
+template <typename I>
+void sort_rows(const I* idx, long long padding, unsigned n_table, int64_t rows, const Plan& p, unsigned char* ws, hipStream_t st) {
+    unsigned *keys = (unsigned*)ws, *pos = (unsigned*)(ws + p.off_pos);
+    if (rows <= kSmallRows) {
+        int n2 = 2;
+        while (n2 < rows) n2 <<= 1;
+        sort_small_k<I><<<1, kSortWg, 0, st>>>(idx, padding, n_table, (int)rows, n2, keys, pos);
+        return;
+    }
+    unsigned* buf_k[2] = {keys, (unsigned*)(ws + p.off_keys2)};
+    unsigned* buf_p[2] = {pos, (unsigned*)(ws + p.off_pos2)};
+    unsigned* hist = (unsigned*)(ws + p.off_hist);
+    const unsigned mask = (1u << p.width) - 1, words = (unsigned)p.sort_wgs * 256;
+    radix_count_k<I><<<p.sort_wgs, kSortWg, 0, st>>>(idx, padding, n_table, (unsigned)rows, (unsigned)p.per_wg, mask, hist,
+                                                     words * (p.passes - 1));
+    int to = (p.passes - 1) & 1;                                                 // so that the last pass writes buffer 0
+    for (int k = 0; k < p.passes; ++k, to ^= 1) {
+        unsigned* next = k + 1 < p.passes ? hist + (size_t)(k + 1) * words : nullptr;
+        if (k == 0)
+            radix_scatter_k<I, true><<<p.sort_wgs, kSortWg, 0, st>>>(idx, padding, n_table, nullptr, nullptr, (unsigned)rows,
+                                                                     (unsigned)p.per_wg, 0, mask, p.width, mask, hist, next, buf_k[to],
+                                                                     buf_p[to]);
+        else
+            radix_scatter_k<I, false><<<p.sort_wgs, kSortWg, 0, st>>>(idx, padding, n_table, buf_k[to ^ 1], buf_p[to ^ 1],
+                                                                      (unsigned)rows, (unsigned)p.per_wg, k * p.width, mask,
+                                                                      (k + 1) * p.width, mask, hist + (size_t)k * words, next,
+                                                                      buf_k[to], buf_p[to]);
+    }
+}
+
+template <typename T, int VEC>
+void sum_rows(const T* g, int64_t ldg, int64_t rows, int64_t dim, int64_t n_table, float scale, const Plan& p, unsigned char* ws, T* out,
+              hipStream_t st) {
+    const unsigned *keys = (const unsigned*)ws, *pos = (const unsigned*)(ws + p.off_pos);
+    float *head = (float*)(ws + p.off_head), *tail = (float*)(ws + p.off_tail);
+    const int64_t per_wg = 256 >> p.log2_lanes;
+    const unsigned sum_wgs = (unsigned)((p.chunks * p.tiles + per_wg - 1) / per_wg);
+    const unsigned zero_wgs = (unsigned)((n_table + kZeroRows - 1) / kZeroRows);
+    segment_sum_k<T, VEC><<<sum_wgs + zero_wgs, 256, 0, st>>>(g, ldg, keys, pos, (unsigned)rows, (int)dim, (unsigned)n_table, scale, p.chunk,
+                                                              p.log2_lanes, p.tiles, sum_wgs, out, head, tail);
+    if (p.chunks > 1) {
+        const int tiles = (int)((dim + 63) / 64);
+        segment_join_k<T><<<(unsigned)((p.chunks - 1) * tiles), 256, 0, st>>>(keys, (unsigned)rows, (int)dim, (unsigned)n_table, scale,
+                                                                              p.chunk, tiles, head, tail, out);
+    }
+}
+
+template <typename T>
+void sum_any(const T* g, int64_t ldg, int64_t rows, int64_t dim, int64_t n_table, float scale, const Plan& p, unsigned char* ws, T* out,
+             hipStream_t st) {
+    if constexpr (sizeof(T) == 2) {
+        if (p.vec == 8) return sum_rows<T, 8>(g, ldg, rows, dim, n_table, scale, p, ws, out, st);
+    }
+    if (p.vec == 4) return sum_rows<T, 4>(g, ldg, rows, dim, n_table, scale, p, ws, out, st);
+    if (p.vec == 2) return sum_rows<T, 2>(g, ldg, rows, dim, n_table, scale, p, ws, out, st);
+    return sum_rows<T, 1>(g, ldg, rows, dim, n_table, scale, p, ws, out, st);
+}
+
+template <typename T, typename I>
+void lookup_any(const T* table, int64_t ldt, const I* idx, const T* add, int64_t lda, float scale, int64_t n_table, int64_t rows,
+                int64_t dim, T* out, hipStream_t st) {
+    constexpr int MOST = 16 / sizeof(T);
+    const int vec = pick_vec(dim, MOST);
+    const int64_t used = (dim + vec - 1) / vec;
+    const int l2 = used >= 256 ? 8 : ceil_log2(used);
+    const unsigned wgs = (unsigned)((rows + (256 >> l2) - 1) / (256 >> l2));
+    auto go = [&](auto tag) {
+        constexpr int VEC = decltype(tag)::value;
+        lookup_k<T, VEC, I><<<wgs, 256, 0, st>>>(table, ldt, idx, add, lda, scale, n_table, rows, (int)dim, l2, out);
+    };
+    if constexpr (MOST == 8) {
+        if (vec == 8) return go(std::integral_constant<int, 8>{});
+    }
+    if (vec == 4) go(std::integral_constant<int, 4>{});
+    else if (vec == 2) go(std::integral_constant<int, 2>{});
+    else go(std::integral_constant<int, 1>{});
+}
+
+bool known_dt(int dt) { return dt == HD_DT_F32 || dt == HD_DT_BF16 || dt == HD_DT_F16; }
+
+}  // namespace
+
+extern "C" int hd_embedding_lookup(const void* table, int64_t ldt, const void* idx, int idx_bits, const void* add, int64_t lda,
+                                   double scale, int dtype, int64_t T, int64_t rows, int64_t dim, void* out, void* st) {
+    HD_REQUIRE(known_dt(dtype), "hd_embedding_lookup: unknown element type %d", dtype);
+    HD_REQUIRE(idx_bits == 32 || idx_bits == 64, "hd_embedding_lookup: indices of 32 or 64 bits, not %d", idx_bits);
+    HD_REQUIRE(rows >= 0 && rows < (1LL << 31) && dim >= 1 && dim < (1LL << 30) && T >= 1 && T < (1LL << 31) - 1 && ldt >= 0 && lda >= 0,
+               "hd_embedding_lookup: bad shape");
+    if (rows == 0) return HD_OK;
+    HD_REQUIRE(table && idx && out, "hd_embedding_lookup: null pointer");
+    const int es = dt_size(dtype);
+    HD_REQUIRE((uintptr_t)table % es == 0 && (uintptr_t)out % es == 0 && (uintptr_t)add % es == 0 && (uintptr_t)idx % (idx_bits / 8) == 0,
+               "hd_embedding_lookup: pointer not aligned to the element");
+    hipStream_t s = (hipStream_t)st;
+    auto go = [&](auto tag) {
+        using E = decltype(tag);
+        if (idx_bits == 64) lookup_any<E, long long>((const E*)table, ldt, (const long long*)idx, (const E*)add, lda, (float)scale, T, rows, dim, (E*)out, s);
+        else lookup_any<E, int>((const E*)table, ldt, (const int*)idx, (const E*)add, lda, (float)scale, T, rows, dim, (E*)out, s);
+    };
+    if (dtype == HD_DT_F32) go(float{});
+    else if (dtype == HD_DT_BF16) go(bf16{});
+    else go(f16{});
+    return check_launch("hd_embedding_lookup");
+}
+
+extern "C" int64_t hd_embedding_sum_workspace_bytes(int64_t rows, int64_t dim, int64_t T, int dtype) {
+    if (rows < 0 || dim < 1 || T < 1 || rows >= (1LL << 31) || T >= (1LL << 31) - 1 || dim >= (1LL << 30) || !known_dt(dtype)) return 0;
+    return make_plan(rows, dim, T, dtype).bytes;
+}
+
+extern "C" int hd_embedding_sum(const void* g, int64_t ldg, const void* idx, int idx_bits, int64_t padding, double scale, int dtype,
+                                int64_t T, int64_t rows, int64_t dim, void* out, void* workspace, int64_t workspace_bytes, void* st) {
+    HD_REQUIRE(known_dt(dtype), "hd_embedding_sum: unknown element type %d", dtype);
+    HD_REQUIRE(idx_bits == 32 || idx_bits == 64, "hd_embedding_sum: indices of 32 or 64 bits, not %d", idx_bits);
+    HD_REQUIRE(rows >= 0 && rows < (1LL << 31) && dim >= 1 && dim < (1LL << 30) && T >= 1 && T < (1LL << 31) - 1 && ldg >= 0,
+               "hd_embedding_sum: bad shape");
+    HD_REQUIRE(out && workspace && (rows == 0 || (g && idx)), "hd_embedding_sum: null pointer");
+    const int es = dt_size(dtype);
+    HD_REQUIRE((uintptr_t)g % es == 0 && (uintptr_t)out % es == 0 && (uintptr_t)idx % (idx_bits / 8) == 0 && (uintptr_t)workspace % 16 == 0,
+               "hd_embedding_sum: misaligned pointer");
+    const Plan p = make_plan(rows, dim, T, dtype);
+    HD_REQUIRE(workspace_bytes >= p.bytes, "hd_embedding_sum: workspace of %lld bytes required, got %lld", (long long)p.bytes,
+               (long long)workspace_bytes);
+    HD_REQUIRE(p.chunks * ((dim + 63) / 64) < (1LL << 31) && p.chunks * p.tiles + T / kZeroRows < (1LL << 31) - 256,
+               "hd_embedding_sum: too many workgroups");
+    hipStream_t s = (hipStream_t)st;
+    unsigned char* ws = (unsigned char*)workspace;
+    if (rows > 0) {
+        if (idx_bits == 64) sort_rows<long long>((const long long*)idx, padding, (unsigned)T, rows, p, ws, s);
+        else sort_rows<int>((const int*)idx, padding, (unsigned)T, rows, p, ws, s);
+    }
+    auto go = [&](auto tag) {
+        using E = decltype(tag);
+        sum_any<E>((const E*)g, ldg, rows, dim, T, (float)scale, p, ws, (E*)out, s);
+    };
+    if (dtype == HD_DT_F32) go(float{});
+    else if (dtype == HD_DT_BF16) go(bf16{});
+    else go(f16{});
+    return check_launch("hd_embedding_sum");
+}

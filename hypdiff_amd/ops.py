@@ -755,6 +755,73 @@ def linear_chain_small(x, layers, emb_after=None, emb=None, emb_idx=None):
     return out
 
 
+# ---- embedding in fp32 / bf16 / fp16 (csrc/embedding.hip) --------------------------------------------------
+DT_CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def embedding(idx, table, scale=1.0, add=None, padding_idx=None):
+    """add + scale * table[idx]: table (T, D) in fp32, bf16 or fp16, idx int32 / int64 of any shape, add (idx.shape + (D,),
+    the table's type) or None; computed in fp32, rounded once.  Differentiable in table and add: the table's gradient sums
+    the rows by token in a fixed order (the same bits on every run), in fp32, and is dense.  The row padding_idx gets no
+    gradient (it is looked up like any other, as nn.Embedding does); an index outside [0, T) gives a row of NaN and no
+    gradient.  The time embedding of ddpm.py:36-41 is embedding(idx, weight, add=h)."""
+    if table.dtype not in DT_CODES:
+        raise TypeError(f"embedding: a table in float32, bfloat16 or float16, not {table.dtype}")
+    if table.dim() != 2 or table.shape[0] < 1 or table.shape[1] < 1:
+        raise ValueError(f"embedding: a table of shape (T, D), not {tuple(table.shape)}")
+    if idx.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"embedding: indices in int32 or int64, not {idx.dtype}")
+    if add is not None:
+        if add.dtype != table.dtype:
+            raise TypeError(f"embedding: add is {add.dtype}, the table {table.dtype}")
+        if tuple(add.shape) != tuple(idx.shape) + (table.shape[1],):
+            raise ValueError(f"embedding: add has shape {tuple(add.shape)}, not {tuple(idx.shape) + (table.shape[1],)}")
+    if padding_idx is not None:
+        if not -table.shape[0] <= padding_idx < table.shape[0]:
+            raise ValueError(f"embedding: padding_idx {padding_idx} is outside a table of {table.shape[0]} rows")
+        padding_idx = int(padding_idx) % table.shape[0]
+    scale = float(scale)
+    _dev(table, idx, add)
+    if torch.is_grad_enabled() and (table.requires_grad or (add is not None and add.requires_grad)):
+        from . import autograd as hag
+        return hag.Embedding.apply(table, add, idx, scale, padding_idx)
+    return _embedding_lookup(table, idx, scale, add)
+
+
+def _pitched(x2):
+    """(2-D tensor with unit column stride, its row pitch): x2 itself unless its columns are strided"""
+    if (x2.stride(1) != 1 and x2.shape[1] > 1) or x2.stride(0) < 0:
+        x2 = x2.contiguous()
+    return x2, x2.stride(0)
+
+
+def _embedding_lookup(table, idx, scale, add):
+    T, D = table.shape
+    tab, ldt = _pitched(table.detach())
+    ix = idx.reshape(-1)
+    ix = ix if ix.is_contiguous() else ix.contiguous()
+    a2, lda = (None, 0) if add is None else _pitched(add.detach().reshape(-1, D))
+    out = torch.empty(tuple(idx.shape) + (D,), dtype=table.dtype, device=table.device)
+    _lib.call("hd_embedding_lookup", _p(tab), ldt, _p(ix), ix.element_size() * 8, _p(a2), lda, scale, DT_CODES[table.dtype], T,
+              ix.numel(), D, _p(out), _stream())
+    return out
+
+
+def _embedding_sum(g, idx, T, scale, padding_idx):
+    D = g.shape[-1]
+    _dev(g, idx)
+    g2, ldg = _pitched(g.detach().reshape(-1, D))
+    ix = idx.reshape(-1)
+    ix = ix if ix.is_contiguous() else ix.contiguous()
+    dt = DT_CODES[g.dtype]
+    nbytes = _lib.load().hd_embedding_sum_workspace_bytes(ix.numel(), D, T, dt)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=g.device)
+    out = torch.empty(T, D, dtype=g.dtype, device=g.device)
+    _lib.call("hd_embedding_sum", _p(g2), ldg, _p(ix), ix.element_size() * 8, -1 if padding_idx is None else padding_idx, scale,
+              dt, T, ix.numel(), D, _p(out), _p(ws), nbytes, _stream())
+    return out
+
+
 # ---- adjacency -------------------------------------------------------------------
 class CSR:
     """Device CSR (int32 rowptr/col, values in the COO's dtype and entry order)."""

@@ -589,6 +589,19 @@ int hd_embedding_add(float* h, const float* table, const int64_t* idx, int64_t T
  * gradients per node in the backward pass of LPModel.decode (models/base_models.py:152-159). */
 int hd_embedding_grad_f32(const float* g, const int64_t* sorted_idx, const int64_t* sorted_rows, int64_t rows, int64_t dim,
                           int64_t T, float* out, void* stream);
+/* Lookup in fp32 / bf16 / fp16 (dtype HD_DT_*): out[r] = add[r] + scale * table[idx[r]], (rows, dim) contiguous, computed in
+ * fp32 and rounded once.  table has row pitch ldt, add (NULL: none) row pitch lda, in elements (0: one row for all); idx holds
+ * int32 or int64 (idx_bits).  An index outside [0, T) gives a row of NaN. */
+int hd_embedding_lookup(const void* table, int64_t ldt, const void* idx, int idx_bits, const void* add, int64_t lda, double scale,
+                        int dtype, int64_t T, int64_t rows, int64_t dim, void* out, void* stream);
+/* Its table gradient: out (T, dim), contiguous, gets scale * (sum of the rows r of g with idx[r] == t), fp32 sums rounded
+ * once; every row of out is written (zeros where no index names it).  The rows of index `padding` (a negative value: none)
+ * and of indices outside [0, T) contribute nothing.  g has row pitch ldg.  The library sorts by itself; the order of the
+ * sums is fixed by the indices alone: the same bits on every call.  workspace: hd_embedding_sum_workspace_bytes bytes,
+ * 16-byte aligned, contents arbitrary, not shared between calls in flight. */
+int64_t hd_embedding_sum_workspace_bytes(int64_t rows, int64_t dim, int64_t T, int dtype);
+int hd_embedding_sum(const void* g, int64_t ldg, const void* idx, int idx_bits, int64_t padding, double scale, int dtype,
+                     int64_t T, int64_t rows, int64_t dim, void* out, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* ---- latent -> graph decoding, diff.py:327-378 --------------------------------------------------
  * The tensor part of generate (:334-349) and decode_adj (:355-378) for a set of graphs: h (n_graphs, n, n) fp32
