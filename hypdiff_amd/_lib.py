@@ -82,6 +82,7 @@ SIZE_QUERIES = {
     "hd_chain_workspace_bytes": [],
     "hd_mlp_chain_workspace_bytes": [I64, c_int],
     "hd_adamw_max_jobs": [],
+    "hd_linear_act_bwd_workspace_bytes": [I64, I64, I64, c_int],
     "hd_embedding_sum_workspace_bytes": [I64, I64, I64, c_int],
 }
 
@@ -153,6 +154,8 @@ SIGNATURES = {
     "hd_transpose_f32": [P, P, I64, I64, I64, I64, P],
     "hd_transpose_multi_f32": [POINTER(HdTransposeJob), c_int, P],
     "hd_adam_step_f32": [POINTER(HdAdamJob), c_int, P, P, P, c_double, c_double, c_double, c_double, I64, P, P],
+    "hd_linear_act_fwd": [P, I64, P, I64, P, P, I64, c_int, I64, I64, I64, c_int, P, P, P],
+    "hd_linear_act_bwd": [P, I64, P, P, I64, P, I64, c_int, I64, I64, I64, c_int, P, P, P, P, I64, P],
     "hd_adamw_step": [P, c_int, c_int, c_int, P, P, P, P, P, I64, c_double, c_double, c_double, c_double, c_double, I64, P,
                       I64, P],
     "hd_colsum_f32": [P, P, I64, I64, I64, P, P],

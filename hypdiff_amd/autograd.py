@@ -499,6 +499,28 @@ class EmbeddingAdd(torch.autograd.Function):
         return g, gt, None
 
 
+class LinearAct(torch.autograd.Function):
+    """resid + act(x W^T + b) on 16-bit operands (ops.linear_act).  The pre-activation is kept in 16 bits (nothing for the
+    identity); backward: hd_linear_act_bwd, and the incoming gradient itself for resid."""
+
+    @staticmethod
+    def forward(ctx, x, w, b, resid, act):
+        y, z = ops._linear_act_fwd(x, w, b, resid, act, want_z=act != 0)
+        ctx.save_for_backward(x, w, z)
+        ctx.act = act
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        x, w, z = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        dx, dw, db = (None, None, None)
+        if any(need[:3]):
+            dx, dw, db = ops._linear_act_bwd(g, z, x, w, ctx.act, *need[:3])
+        return dx, dw, db, g if need[3] else None, None
+
+
 class Embedding(torch.autograd.Function):
     """add + scale * table[idx] in the table's type (ops.embedding).  Backward: hd_embedding_sum for the table, the
     incoming gradient itself for add."""

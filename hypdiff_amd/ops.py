@@ -755,6 +755,87 @@ def linear_chain_small(x, layers, emb_after=None, emb=None, emb_idx=None):
     return out
 
 
+# ---- Linear layers on 16-bit operands (csrc/gemm_half.hip) ---------------------------------------------------
+LINEAR_ACTS = {"identity": 0, "relu": 1, "gelu": 6}
+
+
+def linear_act(x, weight, bias=None, act="identity", resid=None):
+    """resid + act(x @ weight.T + bias) for bf16 or fp16 operands: products accumulated in fp32 on the matrix cores, bias,
+    activation ("identity", "relu", "gelu": the exact-erf one) and residual added in fp32, one rounding at the end.
+
+    x (..., K), weight (N, K), bias (N) or None, resid (..., N) or None, all of one type; the result has that type.
+    Differentiable in all four: one fused pass for dL/dz and the bias gradient, then the two products; the pre-activation is
+    kept in the operands' type, dL/dz is rounded to it for the products, sums are in fp32 and in a fixed order (the same
+    bits on every run).  The 16-bit form of the layers that linear_chain / autograd.linear_stack run in fp32
+    (models/direction_diffusion.py:47-69, ddpm.py:9-27)."""
+    if x.dtype not in (torch.bfloat16, torch.float16):
+        raise TypeError(f"linear_act: operands in bfloat16 or float16, not {x.dtype}")
+    if act not in LINEAR_ACTS:
+        raise ValueError(f"linear_act: act is one of {sorted(LINEAR_ACTS)}, not {act!r}")
+    if weight.dim() != 2 or weight.shape[0] < 1 or weight.shape[1] < 1:
+        raise ValueError(f"linear_act: a weight of shape (N, K), not {tuple(weight.shape)}")
+    if x.dim() < 1 or x.shape[-1] != weight.shape[1]:
+        raise ValueError(f"linear_act: x has shape {tuple(x.shape)}, the weight {tuple(weight.shape)}")
+    N = weight.shape[0]
+    if bias is not None and tuple(bias.shape) != (N,):
+        raise ValueError(f"linear_act: bias has shape {tuple(bias.shape)}, not ({N},)")
+    if resid is not None and tuple(resid.shape) != tuple(x.shape[:-1]) + (N,):
+        raise ValueError(f"linear_act: resid has shape {tuple(resid.shape)}, not {tuple(x.shape[:-1]) + (N,)}")
+    for name, t in (("weight", weight), ("bias", bias), ("resid", resid)):
+        if t is not None and t.dtype != x.dtype:
+            raise TypeError(f"linear_act: {name} is {t.dtype}, x {x.dtype}")
+    _dev(x, weight, bias, resid)
+    code = LINEAR_ACTS[act]
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, resid)):
+        from . import autograd as hag
+        return hag.LinearAct.apply(x, weight, bias, resid, code)
+    return _linear_act_fwd(x, weight, bias, resid, code)[0]
+
+
+def _matrix(t):
+    """(t as a 2-D matrix with unit column stride and rows that do not overlap, its row pitch)"""
+    t = t.detach()
+    if t.dim() != 2:
+        t = t.reshape(-1, t.shape[-1])
+    rows, cols = t.shape
+    if (cols > 1 and t.stride(1) != 1) or (rows > 1 and t.stride(0) < cols):
+        t = t.contiguous()
+    return t, (t.stride(0) if rows > 1 else cols)
+
+
+def _linear_act_fwd(x, w, b, resid, act, want_z=False):
+    x2, ldx = _matrix(x)
+    w2, ldw = _matrix(w)
+    M, (N, K) = x2.shape[0], w2.shape
+    y = torch.empty(x.shape[:-1] + (N,), dtype=x.dtype, device=x.device)
+    z = torch.empty(M, N, dtype=x.dtype, device=x.device) if want_z else None
+    if M == 0:
+        return y, z
+    r2, ldr = (None, 0) if resid is None else _pitched(resid.detach().reshape(M, N))
+    b = None if b is None else b.detach().contiguous()
+    _lib.call("hd_linear_act_fwd", _p(x2), ldx, _p(w2), ldw, _p(b), _p(r2), ldr, DT_CODES[x.dtype], M, N, K, act, _p(y), _p(z),
+              _stream())
+    return y, z
+
+
+def _linear_act_bwd(g, z, x, w, act, need_x, need_w, need_b):
+    _dev(g, x, w)
+    g2, ldg = _matrix(g)
+    x2, ldx = _matrix(x)
+    w2, ldw = _matrix(w)
+    M, (N, K) = x2.shape[0], w2.shape
+    new = torch.zeros if M == 0 else torch.empty
+    dx = new(x.shape, dtype=x.dtype, device=x.device) if need_x else None
+    dw = new(N, K, dtype=x.dtype, device=x.device) if need_w else None
+    db = new(N, dtype=x.dtype, device=x.device) if need_b else None
+    if M > 0:
+        nbytes = _lib.load().hd_linear_act_bwd_workspace_bytes(M, N, K, act)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+        _lib.call("hd_linear_act_bwd", _p(g2), ldg, _p(z), _p(x2), ldx, _p(w2), ldw, DT_CODES[x.dtype], M, N, K, act, _p(dx), _p(dw),
+                  _p(db), _p(ws), nbytes, _stream())
+    return dx, dw, db
+
+
 # ---- embedding in fp32 / bf16 / fp16 (csrc/embedding.hip) --------------------------------------------------
 DT_CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 

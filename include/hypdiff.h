@@ -40,7 +40,7 @@ enum { HD_DT_F32 = 0, HD_DT_BF16 = 1, HD_DT_F16 = 2 };
 
 /* activation codes for the tangent-space activation of HypAct */
 enum { HD_ACT_IDENTITY = 0, HD_ACT_RELU = 1, HD_ACT_TANH = 2, HD_ACT_SIGMOID = 3, HD_ACT_ELU = 4,
-       HD_ACT_LEAKY_RELU = 5 };
+       HD_ACT_LEAKY_RELU = 5, HD_ACT_GELU = 6 };   /* GELU (exact erf): hd_linear_act_* only */
 
 int hd_version(void);
 /* copies the calling thread's last error message (NUL-terminated) into buf */
@@ -446,6 +446,22 @@ typedef struct hd_adam_job {
 } hd_adam_job;
 int hd_adam_step_f32(const hd_adam_job* jobs, int n_jobs, const void* grad_flat, void* exp_avg_flat, void* exp_avg_sq_flat,
                      double lr, double beta1, double beta2, double eps, int64_t step, void* step_state, void* stream);
+/* Linear layer on 16-bit operands (dtype HD_DT_BF16 / HD_DT_F16), fp32 accumulation on the matrix cores:
+ *   z = x W^T + bias,  y = resid + act(z)
+ * x (M, K) with row pitch ldx, W (N, K) with row pitch ldw, bias (N) or NULL, resid (M, N) with row pitch ldr (0: one row for
+ * all) or NULL, y (M, N) contiguous; act HD_ACT_IDENTITY, HD_ACT_RELU or HD_ACT_GELU.  z (M, N) contiguous or NULL: the
+ * pre-activation, rounded, for the backward pass.  y is rounded once, from fp32.  Any sizes, pitches and element-aligned
+ * pointers; rows that start on 16-byte borders and hold a multiple of 8 elements are fastest.  y and z overlap nothing. */
+int hd_linear_act_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, const void* resid, int64_t ldr,
+                      int dtype, int64_t M, int64_t N, int64_t K, int act, void* y, void* z, void* stream);
+/* Its gradients from g = dL/dy (M, N) with row pitch ldg:  dz = g * act'(z);  dx (M, K) = dz W,  dw (N, K) = dz^T x,
+ * db (N) = colsum(dz); each contiguous, of the operands' type, or NULL.  z may be NULL for HD_ACT_IDENTITY.  M >= 1.
+ * workspace: hd_linear_act_bwd_workspace_bytes bytes, 16-byte aligned, contents arbitrary, not shared between calls in
+ * flight.  No atomics: the same bits on every call. */
+int64_t hd_linear_act_bwd_workspace_bytes(int64_t M, int64_t N, int64_t K, int act);
+int hd_linear_act_bwd(const void* g, int64_t ldg, const void* z, const void* x, int64_t ldx, const void* w, int64_t ldw, int dtype,
+                      int64_t M, int64_t N, int64_t K, int act, void* dx, void* dw, void* db, void* workspace,
+                      int64_t workspace_bytes, void* stream);
 /* One step of AdamW (decoupled weight decay) over up to hd_adamw_max_jobs() parameter tensors in ONE launch:
  *   m = b1 m + (1-b1) g;  v = b2 v + (1-b2) g^2;  p = p (1 - lr wd) - lr/(1-b1^t) * m / (sqrt(v)/sqrt(1-b2^t) + eps)   (fp32)
  * Job i: `count` elements of type `dtype` (HD_DT_*) at param / grad, contiguous, aligned to the element; its state is the

@@ -1,0 +1,306 @@
+"""ops.linear_act (csrc/gemm_half.hip): forward and gradients of resid + act(x W^T + b) on 16-bit operands against 64 bits,
+over sizes, layouts and types; NaN and infinities; the same bits on every call; refusals; captured and replayed."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+gpu = pytest.mark.gpu
+U = 2.0 ** -24
+HALF = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}       # half a step, relative
+TINY = {torch.bfloat16: 0.0, torch.float16: 2.0 ** -25}             # half of fp16's smallest step
+
+
+def _gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def _act64(z, act):
+    if act == "relu":
+        return z.clamp(min=0), (z > 0).double()
+    if act == "gelu":
+        phi = 0.5 * torch.erfc(-z / math.sqrt(2.0))
+        return z * phi, phi + z * torch.exp(-0.5 * z * z) / math.sqrt(2 * math.pi)
+    return z, torch.ones_like(z)
+
+
+def _reference(x, w, b, r, g, act, dtype):
+    """Results in 64 bits and what each may be off by, from arithmetic:
+
+    z     K products of 16-bit numbers are exact in fp32; their sum in any order is off by K u sum|x w|, the bias by one
+          more rounding: ez.
+    y     act is 1.13-Lipschitz (GELU) and evaluated to 3e-7 |z|, the residual one rounding, storage half a step.
+    dz    z was stored with a relative half step h (and fp16's smallest step), g times a slope that moves by at most 0.8 per
+          unit of z, except at ReLU's border, where an element within the error of 0 may count or not; the product and the
+          slope's evaluation: 4e-7 |g|; storage of dz another h.
+    dx dw db   sums of those errors against |W|, |x|, 1, and the sum's own roundings."""
+    h, tiny = HALF[dtype], TINY[dtype]
+    K = x.shape[1]
+    z = x @ w.t()
+    ez = (K + 1) * U * (x.abs() @ w.abs().t())
+    if b is not None:
+        z = z + b
+        ez = ez + U * b.abs()
+    a, slope = _act64(z, act)
+    y = a if r is None else a + r
+    ey = 1.13 * ez + 3e-7 * z.abs() + U * y.abs()
+    out = {"y": (y, ey * (1 + h) + h * y.abs() + tiny)}
+    if g is None:
+        return out
+    moved = ez * (1 + h) + (0.0 if act == "identity" else h) * z.abs() + tiny
+    if act == "relu":
+        ds = (z.abs() <= moved).double()
+    else:
+        ds = (0.8 * moved) if act == "gelu" else torch.zeros_like(z)
+    dz = g * slope
+    ed = g.abs() * (ds + (4e-7 if act == "gelu" else 0.0))
+    ed16 = ed + h * (dz.abs() + ed) + tiny
+    n = lambda k: (k + 1) * U  # noqa: E731
+    for key, val, err, size, k in (("dx", dz @ w, ed16 @ w.abs(), (dz.abs() + ed16) @ w.abs(), w.shape[0]),
+                                   ("dw", dz.t() @ x, ed16.t() @ x.abs(), (dz.abs() + ed16).t() @ x.abs(), x.shape[0]),
+                                   ("db", dz.sum(0), ed.sum(0), (dz.abs() + ed).sum(0), x.shape[0])):
+        e = err + n(k) * size
+        out[key] = (val, e * (1 + h) + h * val.abs() + tiny)
+    return out
+
+
+def _check(got, want, bound, what):
+    got = got.detach().double()
+    assert got.shape == want.shape, what
+    over = (got - want).abs() - bound
+    assert not bool((over > 0).any()) and not bool(torch.isnan(got).any()), \
+        (what, float(over.max()), float(((got - want).abs() / bound.clamp(min=1e-300)).max()))
+
+
+def _run(M, N, K, dtype, act, bias, resid, seed, pitch=0, lead=None, w_pitch=0, g_kind="dense"):
+    from hypdiff_amd import ops
+    gen = _gen(seed)
+    x = torch.randn(M, K + pitch, device="cuda", generator=gen).to(dtype)[:, pitch // 2:pitch // 2 + K]
+    w = (torch.randn(N, K + w_pitch, device="cuda", generator=gen) / math.sqrt(K)).to(dtype)[:, :K]
+    b = torch.randn(N, device="cuda", generator=gen).to(dtype) if bias else None
+    r = torch.randn(M, N, device="cuda", generator=gen).to(dtype) if resid else None
+    g = torch.randn(M, N, device="cuda", generator=gen).to(dtype)
+    if g_kind == "slice":
+        g = torch.randn(M, N + 3, device="cuda", generator=gen).to(dtype)[:, 2:N + 2]
+    elif g_kind == "row":
+        g = g[:1].expand(M, N)
+    if lead is not None:
+        x, g = x.reshape(lead + (K,)), g.reshape(lead + (N,))
+        r = None if r is None else r.reshape(lead + (N,))
+    leaves = {"dx": x, "dw": w}
+    if bias:
+        leaves["db"] = b
+    if resid:
+        leaves["dr"] = r
+    leaves = {k: t.detach().requires_grad_(True) for k, t in leaves.items()}
+    y0 = ops.linear_act(x, w, b, act=act, resid=r)
+    y = ops.linear_act(leaves["dx"], leaves["dw"], leaves.get("db"), act=act, resid=leaves.get("dr"))
+    assert torch.equal(y0, y) and y.dtype == dtype
+    grads = dict(zip(leaves, torch.autograd.grad(y, list(leaves.values()), g)))
+    d = lambda t, c: None if t is None else t.reshape(-1, c).double()  # noqa: E731
+    want = _reference(d(x, K), w.double(), None if b is None else b.double(), d(r, N), d(g, N), act, dtype)
+    _check(y.reshape(-1, N), *want["y"], "y")
+    for k in ("dx", "dw") + (("db",) if bias else ()):
+        assert grads[k].dtype == dtype and grads[k].shape == leaves[k].shape
+        _check(grads[k].reshape(want[k][0].shape), *want[k], k)
+    if resid:
+        assert torch.equal(grads["dr"], g)
+    y2 = ops.linear_act(leaves["dx"], leaves["dw"], leaves.get("db"), act=act, resid=leaves.get("dr"))
+    for k, t in zip(leaves, torch.autograd.grad(y2, list(leaves.values()), g)):
+        assert torch.equal(t, grads[k]), k               # no order of sums to differ in
+
+
+SIZES = [(1, 1, 1), (1, 512, 512), (2, 7, 5), (15, 16, 17), (16, 8, 8), (33, 40, 24), (64, 64, 64), (127, 129, 72), (128, 128, 128),
+         (130, 136, 264), (200, 512, 512), (200, 64, 512), (200, 512, 64), (257, 300, 513), (1000, 14, 15), (300, 900, 800),
+         (2049, 72, 88), (4100, 260, 136)]
+
+
+@gpu
+@pytest.mark.parametrize("M,N,K", SIZES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_sizes(M, N, K, dtype):
+    k = SIZES.index((M, N, K))
+    _run(M, N, K, dtype, ("gelu", "relu", "identity")[k % 3], k % 4 != 3, k % 2 == 0, k)
+
+
+@gpu
+@pytest.mark.parametrize("act", ["gelu", "relu", "identity"])
+@pytest.mark.parametrize("bias,resid", [(False, False), (True, True)])
+def test_activations_and_epilogues(act, bias, resid):
+    _run(300, 200, 160, torch.bfloat16, act, bias, resid, 5)
+    _run(70, 99, 161, torch.float16, act, bias, resid, 6)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_layouts(dtype):
+    """pitched rows (aligned, odd, starting off a 16-byte border), pitched weights, leading axes, gradients that are slices
+    or one row for all"""
+    _run(140, 136, 128, dtype, "gelu", True, True, 1, pitch=8)
+    _run(140, 136, 128, dtype, "gelu", True, False, 2, pitch=16)
+    _run(140, 136, 128, dtype, "relu", True, True, 3, pitch=37, w_pitch=1)
+    _run(140, 136, 128, dtype, "gelu", True, True, 4, w_pitch=24, g_kind="slice")
+    _run(140, 136, 128, dtype, "identity", True, True, 5, g_kind="row")
+    _run(140, 133, 120, dtype, "gelu", True, True, 6, lead=(4, 5, 7))
+    _run(140, 136, 128, dtype, "identity", True, False, 7, pitch=3, g_kind="slice")
+
+
+@gpu
+def test_transposed_and_strided_operands():
+    from hypdiff_amd import ops
+    gen = _gen(9)
+    x = torch.randn(96, 50, device="cuda", generator=gen).bfloat16()
+    w = torch.randn(96, 80, device="cuda", generator=gen).bfloat16()
+    for xs, wsx in ((x.t(), w.t()), (x.t()[::2], w.t()[::3])):
+        got = ops.linear_act(xs, wsx)
+        assert torch.equal(got, ops.linear_act(xs.contiguous(), wsx.contiguous()))
+    row = torch.randn(96, device="cuda", generator=gen).bfloat16()
+    assert torch.equal(ops.linear_act(row, w.t()), ops.linear_act(row[None], w.t())[0])
+    one = ops.linear_act(row.expand(40, 96), w.t(), resid=row[:80].expand(40, 80))
+    assert torch.equal(one, one[:1].expand_as(one))
+
+
+@gpu
+def test_no_rows():
+    from hypdiff_amd import ops
+    x = torch.zeros(0, 24, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+    w = torch.randn(16, 24, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+    b = torch.randn(16, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+    y = ops.linear_act(x, w, b, act="gelu", resid=torch.zeros(0, 16, device="cuda", dtype=torch.bfloat16))
+    assert y.shape == (0, 16)
+    dx, dw, db = torch.autograd.grad(y, [x, w, b], torch.zeros(0, 16, device="cuda", dtype=torch.bfloat16))
+    assert dx.shape == (0, 24) and not dw.any() and not db.any()
+
+
+@gpu
+@pytest.mark.parametrize("K", [64, 65, 200])
+def test_nonfinite_values_stay_in_their_row_and_column(K):
+    from hypdiff_amd import ops
+    gen = _gen(11)
+    x = torch.randn(150, K, device="cuda", generator=gen).bfloat16()
+    w = torch.randn(140, K, device="cuda", generator=gen).bfloat16()
+    clean = ops.linear_act(x, w, act="relu")
+    x[149, K - 1], x[3, 0] = float("nan"), float("inf")
+    w[139, 1] = float("nan")
+    got = ops.linear_act(x, w, act="relu")
+    hit = torch.zeros(150, 140, dtype=torch.bool, device="cuda")
+    hit[149] = True
+    hit[3] = True
+    hit[:, 139] = True
+    assert bool(torch.isnan(got[149]).all()) and bool(torch.isnan(got[:, 139]).all())
+    assert torch.equal(got[~hit], clean[~hit])
+
+
+@gpu
+def test_gradient_against_differences():
+    """L = sum(g * y) along a random direction in x, W, b: central differences in 64 bits of the formula against the
+    kernel's gradients: what the gradients may be off by (see _reference) summed along the direction."""
+    from hypdiff_amd import ops
+    gen = _gen(12)
+    x = torch.randn(40, 24, device="cuda", generator=gen).half()
+    w = (torch.randn(32, 24, device="cuda", generator=gen) / 5).half()
+    b = torch.randn(32, device="cuda", generator=gen).half()
+    g = torch.randn(40, 32, device="cuda", generator=gen).half()
+    ls = [t.detach().requires_grad_(True) for t in (x, w, b)]
+    grads = torch.autograd.grad(ops.linear_act(*ls, act="gelu"), ls, g)
+    want = _reference(x.double(), w.double(), b.double(), None, g.double(), "gelu", torch.float16)
+    for k, (t, gr) in enumerate(zip((x, w, b), grads)):
+        d = torch.randn(t.shape, device="cuda", generator=gen, dtype=torch.float64)
+        h = 1e-4
+
+        def loss(s):
+            ops64 = [v.double() for v in (x, w, b)]
+            ops64[k] = ops64[k] + s * d
+            return float((_act64(ops64[0] @ ops64[1].t() + ops64[2], "gelu")[0] * g.double()).sum())
+        diff = (loss(h) - loss(-h)) / (2 * h)
+        bound = float((want[("dx", "dw", "db")[k]][1] * d.abs()).sum())
+        assert abs(diff - float((gr.double() * d).sum())) <= bound + 1e-5 * abs(diff) + 1e-5
+
+
+@gpu
+@pytest.mark.parametrize("M,N,K", [(200, 136, 128), (70, 33, 41)])
+def test_captured_and_replayed(M, N, K):
+    from hypdiff_amd import ops
+    gen = _gen(13)
+    new = lambda *s: torch.randn(*s, device="cuda", generator=gen).bfloat16()  # noqa: E731
+    x, w, b, g = new(M, K), new(N, K), new(N), new(M, N)
+
+    def both():
+        y, z = ops._linear_act_fwd(x, w, b, None, 6, want_z=True)
+        return (y,) + ops._linear_act_bwd(g, z, x, w, 6, True, True, True)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        both()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = both()
+    for _ in range(3):
+        for t in (x, w, b, g):
+            t.copy_(new(*t.shape))
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, c in zip(out, both()):
+            assert torch.equal(a, c)
+
+
+@gpu
+def test_two_streams_at_once():
+    from hypdiff_amd import ops
+    gen = _gen(14)
+    new = lambda *s: torch.randn(*s, device="cuda", generator=gen).bfloat16()  # noqa: E731
+    sets = [(new(3000, 512), new(512, 512), new(512), new(3000, 512)) for _ in range(2)]
+
+    def step(x, w, b, g):
+        y, z = ops._linear_act_fwd(x, w, b, None, 6, want_z=True)
+        return (y,) + ops._linear_act_bwd(g, z, x, w, 6, True, True, True)
+    want = [step(*s) for s in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    got = []
+    for st, s in zip(streams, sets):
+        with torch.cuda.stream(st):
+            got.append([step(*s) for _ in range(5)])
+    torch.cuda.synchronize()
+    for outs, w in zip(got, want):
+        for o in outs:
+            assert all(torch.equal(a, c) for a, c in zip(o, w))
+
+
+def test_refusals_on_the_host():
+    from hypdiff_amd import ops
+    x, w = torch.zeros(3, 4).bfloat16(), torch.zeros(5, 4).bfloat16()
+    for args, kw, err in (((x.float(), w.float()), {}, TypeError), ((x, w.half()), {}, TypeError), ((x, w[0]), {}, ValueError),
+                          ((x, w[:, :3]), {}, ValueError), ((x, w[:0]), {}, ValueError), ((x, w), dict(act="silu"), ValueError),
+                          ((x, w, torch.zeros(4).bfloat16()), {}, ValueError), ((x, w, torch.zeros(5)), {}, TypeError),
+                          ((x, w), dict(resid=torch.zeros(5).bfloat16()), ValueError),
+                          ((x, w), dict(resid=torch.zeros(3, 5)), TypeError)):
+        with pytest.raises(err, match="linear_act"):
+            ops.linear_act(*args, **kw)
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        ops.linear_act(x, w)
+
+
+def test_refusals_of_the_entry_points():
+    from hypdiff_amd import _lib
+
+    def fwd(x=256, ldx=16, w=256, ldw=16, bias=None, resid=None, ldr=0, dt=1, M=4, N=8, K=16, act=0, y=256, z=None):
+        _lib.call("hd_linear_act_fwd", x, ldx, w, ldw, bias, resid, ldr, dt, M, N, K, act, y, z, None)
+
+    def bwd(g=256, ldg=8, z=256, x=256, ldx=16, w=256, ldw=16, dt=1, M=4, N=8, K=16, act=6, dx=256, dw=256, db=256, ws=256,
+            nbytes=1 << 30):
+        _lib.call("hd_linear_act_bwd", g, ldg, z, x, ldx, w, ldw, dt, M, N, K, act, dx, dw, db, ws, nbytes, None)
+    for fn in (fwd, bwd):
+        for bad, what in ((dict(dt=0), "element type"), (dict(act=2), "activation"), (dict(M=-1), "shape"), (dict(N=0), "shape"),
+                          (dict(K=0), "shape"), (dict(M=1 << 30), "shape"), (dict(ldx=15), "pitch"), (dict(ldw=15), "pitch"),
+                          (dict(x=257), "aligned"), (dict(x=None), "null|needs")):
+            with pytest.raises(RuntimeError, match=what):
+                fn(**bad)
+    for bad, what in ((dict(ws=None), "workspace"), (dict(nbytes=16), "workspace of"), (dict(M=0), "no rows"), (dict(z=None), "null"),
+                      (dict(ldg=7), "pitch"), (dict(w=None), "needs")):
+        with pytest.raises(RuntimeError, match=what):
+            bwd(**bad)
+    assert _lib.load().hd_linear_act_bwd_workspace_bytes(1 << 30, 8, 8, 6) == 0
