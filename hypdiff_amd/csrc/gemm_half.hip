@@ -8,20 +8,27 @@
 // in fp32 and are rounded once each.  dz is rounded to the operands' type, as the matrix instruction needs it; db is
 // summed from the unrounded products.
 //
-// One tile kernel does the three products C[m][n] = sum_k A(m, k) B(n, k).  They differ in which index of an operand is
-// contiguous: k (x and W forward, dz for dx) or the other one (W for dx, dz and x for dW).  In the second case a tile
-// lies in LDS as it does in memory, k rows of m or n, and gfx950's transposing LDS read (ds_read_b64_tr_b16) hands a lane
-// four consecutive k of its own column, so nothing is transposed in memory.
+// Three products C[m][n] = sum_k A(m, k) B(n, k): forward (A = x, B = W), dx (A = dz, B = W^T, which the launch that makes dz
+// also writes), dW (A = dz, B = x, both with k -- the rows of the batch -- as the slow index).
 //
+//   tiles     128 x 192 (4 wavefronts of 64 x 96), slabs of 32 k in two LDS buffers of 20 KB, so that three or four workgroups
+//             share a CU and one's epilogue runs beside another's products; 64 x 64 where that gives too few tiles to fill the
+//             chip; 32 x 32 with the contraction split over the wavefronts where even those are few (small_gemm).
 //   staging   16-byte chunks go from memory to LDS without passing registers where every row starts on a 16-byte border and
 //             holds whole chunks; otherwise (an odd width, a sliced matrix) through registers, with the tail masked.  Chunks
 //             beyond the contraction's end come from a page of zeros, rows and columns beyond the matrix from a valid one
 //             (their results are not stored).
-//   LDS       a k-contiguous tile has rows of BK elements whose chunks are permuted by row (c ^ f(row)) so that the 16-byte
-//             reads of a fragment meet 128 bytes of distinct banks per clock (measured: 7.8 clocks per 1 KB read, 16 without);
-//             the rows of B are dealt to the fragment so that a lane ends with 8 consecutive n: 16-byte stores.
-//   split     the contraction of dW (the rows of the batch) is cut into slices, one workgroup each; fp32 partial tiles are
-//             summed in slice order by a second launch, which also finishes db: the same bits on every call.
+//   LDS       a slab with k fast has rows of 64 bytes whose chunks are permuted by row (c ^ f(row)): a fragment's 16-byte reads
+//             then meet distinct banks (measured 8 clocks per 1 KB, the port's width).  B's rows are dealt to the fragments
+//             so that a lane ends with 6 neighbouring n and 16 neighbouring lanes with one row's 96: whole runs of 192 bytes
+//             leave with one store (per-lane 16-byte pieces of 16 rows cost 60 us more at 74750 x 800 -> 900).  A slab with
+//             k slow lies in LDS as it does in memory; gfx950's transposing read (ds_read_b64_tr_b16) hands a lane four
+//             consecutive k of its own column, so nothing is transposed in memory.
+//   split     the contraction of dW is cut into slices, one workgroup each; fp32 partial tiles are summed in slice order by
+//             the last launch, which also finishes db: the same bits on every call.
+// What bounds the large forward (74750 x 800 -> 900, bf16): bytes from L2 into the CUs.  A CU takes 64 bytes a clock in whole
+// 128-byte lines (34 TB/s for the chip), 16 TB/s in the 64-byte runs of a 32-k slab; the products alone take 72 us, the loads
+// alone 100, the stores and the GELU 25 more than they hide.
 #include <stdlib.h>
 #include "hd_common.cuh"
 #include "hd_half.cuh"
@@ -52,43 +59,31 @@ __device__ __forceinline__ void dma16(const void* g, char* l) {              // 
     __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)g, (__attribute__((address_space(3))) void*)l, 16, 0, 0);
 }
 
-// ---- one operand's tile in LDS ----------------------------------------------------------------------------------------------
-// k-contiguous: MN rows of BK elements.  k-strided (TR): BK rows of MN elements.  Addresses in bytes.
-template <int MN, int BK, bool TR, bool PERM>
-struct Tile16 {
+// ---- one operand's slab in LDS ----------------------------------------------------------------------------------------------
+// k fast: MN rows of BK elements.  k slow (TR): BK rows of MN elements.  Chunks of 8 elements, addresses in bytes.
+template <int MN, int BK, bool TR>
+struct Slab {
     static constexpr int kRowChunks = (TR ? MN : BK) / 8;
     static constexpr int kChunks = MN * BK / 8;
     static constexpr int kBytes = MN * BK * 2;
-    static_assert(!TR || MN >= 32, "a k-strided row holds at least two 16-column groups");
     // chunk c of row r lies at position c ^ swz(r)
     static __device__ __forceinline__ int swz(int r) {
-        if constexpr (TR) {
-            const int g = (r & 3) | ((r >> 3) & 1) << 2;
-            return (g << 1) & (kRowChunks - 2);                              // pairs of chunks (one 16-column group) move together
-        } else if constexpr (PERM) {
-            return (((r >> 1) & 1) | ((r >> 3) & 3) << 1) & (kRowChunks - 1);
-        } else {
-            return (r >> 1) & (kRowChunks - 1);
-        }
+        if constexpr (!TR) return (r >> 1) & (kRowChunks - 1);
+        // pairs of chunks (16 columns) move together; rows r and r + 8 of a half-wavefront must not meet
+        else if constexpr (MN % 128 == 0) return ((r & 3) | ((r >> 3) & 1) << 2) << 1;
+        else return (((r >> 1) & 1) | ((r >> 3) & 1) << 1) << 1;               // 192, 64: rows are 128 bytes off a 256-byte border
     }
-    // fragment f (16 of MN) for k = 32 s .. + 31: lane (r16, kq) gets k = 8 kq .. + 7 of its row / column.  PERM deals the
-    // rows so that fragments 2 p and 2 p + 1 hold 8 consecutive ones per group of four accumulators.
-    static __device__ __forceinline__ int frag_row(int f, int r16) {
-        if constexpr (PERM) return 32 * (f >> 1) + 8 * (r16 >> 2) + 4 * (f & 1) + (r16 & 3);
-        else return 16 * f + r16;
-    }
-    // the lane's part of a fragment's address; the rest (frag_off) is a constant of (f, s)
+    // fragment f (16 of MN from base_mn on), k = 32 s .. + 31: lane (r16, kq) gets k = 8 kq .. + 7 of row / column r16
     static __device__ __forceinline__ uint4 read(const char* lds, int base_mn, int f, int s, int lane) {
         const int r16 = lane & 15, kq = lane >> 4;
         if constexpr (!TR) {
-            const int r = base_mn + frag_row(f, r16);
+            const int r = base_mn + 16 * f + r16;
             return *reinterpret_cast<const uint4*>(lds + r * (BK * 2) + (((s * 4 + kq) ^ swz(r)) << 4));
         } else {
             // this lane names 4 columns of k row `rho` of its group; it receives column r16 of 4 rows, twice
             const int rho = r16 >> 2, gam = r16 & 3;
-            const int col = base_mn + (PERM ? 32 * (f >> 1) + 8 * gam + 4 * (f & 1) : 16 * f + 4 * gam);
+            const int col = base_mn + 16 * f + 4 * gam, c = col >> 3, b = (col & 4) << 1;
             const int k0 = 32 * s + 8 * kq + rho;
-            const int c = col >> 3, b = (col & 4) << 1;
             const char* p0 = lds + k0 * (MN * 2) + ((c ^ swz(k0)) << 4) + b;
             const char* p1 = lds + (k0 + 4) * (MN * 2) + ((c ^ swz(k0 + 4)) << 4) + b;
             const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p0);
@@ -99,35 +94,41 @@ struct Tile16 {
     }
 };
 
-// What a workgroup stages of one operand: chunk q (0 .. kChunks - 1) of every k slab
-template <typename T, typename L, int NT, int MN, int BK, bool TR, bool DIRECT>
+// What a workgroup stages of one operand: chunk q (0 .. kChunks - 1) of every slab.  DEAL > 0: the rows of a wavefront's DEAL rows
+// lie in LDS in the order in which the fragments take them (fragment f, row r16 = row r16 * DEAL / 16 + f).
+template <typename T, int MN, int BK, bool TR, bool DIRECT, int DEAL>
 struct Stager {
-    static constexpr int kPer = L::kChunks / NT;                              // chunks of a thread
-    static_assert(L::kChunks % NT == 0, "whole rounds");
+    using L = Slab<MN, BK, TR>;
+    static constexpr int kPer = L::kChunks / 256;                             // chunks of a thread
+    static_assert(L::kChunks % 256 == 0, "whole rounds");
     const T* p[kPer];                                                         // the chunk of the slab at hand
-    int k[kPer];                                                              // its first k (k-contiguous) or its k (k-strided)
-    int n_ok[kPer];                                                           // registers path: elements inside the row (k-strided)
+    int k[kPer];                                                              // its first k (k fast) or its k (k slow)
+    int ok[kPer];                                                             // registers path, k slow: elements inside the matrix
     uint4 reg[DIRECT ? 1 : kPer];
     long long step;
     int k_end;
 
+    static __device__ __forceinline__ int row_of(int r) {
+        if constexpr (DEAL == 0) return r;
+        else return r / DEAL * DEAL + (r % 16) * (DEAL / 16) + (r % DEAL) / 16;
+    }
     __device__ __forceinline__ void init(const T* base, long long ld, int mn0, int mn_end, int k0, int k_end_, int tid) {
         k_end = k_end_;
         step = TR ? (long long)BK * ld : BK;
 #pragma unroll
         for (int q = 0; q < kPer; ++q) {
-            const int at = q * NT + tid, r = at / L::kRowChunks, c = (at % L::kRowChunks) ^ L::swz(r);
+            const int at = q * 256 + tid, r = at / L::kRowChunks, c = (at % L::kRowChunks) ^ L::swz(r);
             if constexpr (TR) {
                 k[q] = k0 + r;
                 int col = mn0 + c * 8;
-                n_ok[q] = mn_end - col;
-                if (n_ok[q] <= 0) { col = 0; n_ok[q] = 0; }                   // beyond the matrix: any column
+                ok[q] = mn_end - col;
+                if (ok[q] <= 0) { col = 0; ok[q] = 0; }                       // beyond the matrix: any column
                 p[q] = base + (long long)k[q] * ld + col;
             } else {
                 k[q] = k0 + c * 8;
-                int row = mn0 + r;
+                int row = mn0 + row_of(r);
                 if (row >= mn_end) row = mn_end - 1;                          // beyond the matrix: any row
-                n_ok[q] = 0;
+                ok[q] = 0;
                 p[q] = base + (long long)row * ld + k[q];
             }
         }
@@ -142,15 +143,15 @@ struct Stager {
         for (int q = 0; q < kPer; ++q) {
             if constexpr (DIRECT) {
                 const void* src = k[q] < k_end ? (const void*)p[q] : (const void*)zero_page;   // whole chunks (k_end % 8 == 0, or a k row)
-                dma16(src, lds + (q * NT + wave * 64) * 16);
+                dma16(src, lds + (q * 256 + wave * 64) * 16);
             } else {
                 Pack<T, 8> v;
-                const int ok = TR ? (k[q] < k_end ? n_ok[q] : 0) : k_end - k[q];
-                if (ok >= 8) {
+                const int n = TR ? (k[q] < k_end ? ok[q] : 0) : k_end - k[q];
+                if (n >= 8) {
                     v = load_pack<T, 8>(p[q]);
                 } else {
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) v.v[e] = e < ok ? p[q][e] : (T)0.f;
+                    for (int e = 0; e < 8; ++e) v.v[e] = e < n ? p[q][e] : (T)0.f;
                 }
                 reg[q] = __builtin_bit_cast(uint4, v);
             }
@@ -159,120 +160,163 @@ struct Stager {
     __device__ __forceinline__ void store(char* lds, int tid) {
         if constexpr (!DIRECT) {
 #pragma unroll
-            for (int q = 0; q < kPer; ++q) *reinterpret_cast<uint4*>(lds + (q * NT + tid) * 16) = reg[q];
+            for (int q = 0; q < kPer; ++q) *reinterpret_cast<uint4*>(lds + (q * 256 + tid) * 16) = reg[q];
         }
     }
 };
 
-__device__ __forceinline__ float act_value(float z, int act) {
-    return act == HD_ACT_GELU ? gelu_erfc(z) : (act == HD_ACT_RELU ? (z > 0.f ? z : (z != z ? z : 0.f)) : z);
+// 0.5 erfc(a / sqrt 2) for a = |x|, as 2^(a P(a) - 1): a weighted minimax fit of log2 erfc, of degree 4 because the result is
+// rounded to 16 bits: GELU comes out within 2e-6 |x| (relative 8e-5 down to x = -3, a sixth of fp16's half step); the fp32 path's
+// degree 7 costs three more operations an element, and the epilogue shares the vector unit with the products' issue.
+// Beyond 30 it is 0 in any case; the clamp keeps infinities out of the products.
+__device__ __forceinline__ float half_erfc16(float x) {
+    const float a = fminf(fabsf(x), 30.f);
+    float r = fmaf(-4.9161474e-04f, a, 7.2239037e-03f);
+    r = fmaf(r, a, -5.2209500e-02f);
+    r = fmaf(r, a, -4.5953175e-01f);
+    r = fmaf(r, a, -1.1510228f);
+    return __builtin_amdgcn_exp2f(fmaf(r, a, -1.0f));
 }
-__device__ __forceinline__ float act_slope(float z, int act) {
-    return act == HD_ACT_GELU ? gelu_erf_grad(z) : (act == HD_ACT_RELU ? (z > 0.f ? 1.f : 0.f) : 1.f);
+// GELU(x) = (x + |x|) / 2 - |x| * (0.5 erfc(|x| / sqrt 2)); the first term passes a NaN on and +inf through
+__device__ __forceinline__ float gelu16(float x) {
+    return fmaf(-fminf(fabsf(x), 30.f), half_erfc16(x), fmaf(0.5f, fabsf(x), 0.5f * x));
+}
+// Phi(x) + x phi(x)
+__device__ __forceinline__ float gelu16_slope(float x) {
+    const float Phi = 0.5f + copysignf(0.5f - half_erfc16(x), x);
+    return fmaf(x, __builtin_amdgcn_exp2f(fmaf(x * -0.72134752044448170368f, x, -1.32574806473615f)), Phi);   // log2(1 / sqrt(2 pi))
+}
+template <int ACT>
+__device__ __forceinline__ float act_value(float z) {
+    if constexpr (ACT == HD_ACT_GELU) return gelu16(z);
+    else if constexpr (ACT == HD_ACT_RELU) return z > 0.f ? z : (z == z ? 0.f : z);
+    else return z;
+}
+template <int ACT>
+__device__ __forceinline__ float act_slope(float z) {
+    if constexpr (ACT == HD_ACT_GELU) return gelu16_slope(z);
+    else if constexpr (ACT == HD_ACT_RELU) return z > 0.f ? 1.f : 0.f;
+    else return 1.f;
 }
 
 struct Prod {
     const void *A, *B;
     long long lda, ldb;
     int M, N, K;
-    void* C;                        // T (M, N) with pitch ldc, or fp32 partial tiles [slice][M][N]
-    long long ldc;
+    void* C;                        // T (M, N) contiguous, or fp32 partial tiles [slice][M][N]
     const void *bias, *resid;
-    void* z;                        // (M, N) contiguous
+    void* z;                        // (M, N) contiguous, or null
     long long ldr;
     int act;
     int tiles_n, tiles, total;      // total = tiles * slices
     int slabs, slabs_rem;           // slice s covers slabs + (s < slabs_rem) slabs of BK
 };
 
-// 8 consecutive n of one row m leave: bias, z, activation, residual, rounding
-template <typename T>
-__device__ __forceinline__ void write8(const Prod& g, int m, int n, const float (&acc)[8]) {
-    float v[8];
-    const bool whole = n + 8 <= g.N;
-    const T* bias = (const T*)g.bias;
-    const T* resid = (const T*)g.resid;
-    const long long o = (long long)m * g.ldc + n;
-    if (whole) {
+// V neighbouring n of row m leave: bias, z, activation, residual, one rounding.  yb / zb: the tile's first element, off: this lane's
+// byte offset in the tile.  z is not read before the backward pass: stored past the caches (8 % of the training forward).
+template <typename T, int V, int ACT>
+__device__ __forceinline__ void write_row(const Prod& g, char* yb, char* zb, unsigned off, int m, int n, const float (&acc)[V],
+                                          const float (&bias)[V]) {
+    float v[V];
+    const T* resid = (const T*)g.resid + (long long)m * g.ldr + n;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = acc[e];
-        if (bias) {
-            const Pack<T, 8> b = load_pack<T, 8>(bias + n);
+    for (int e = 0; e < V; ++e) v[e] = acc[e] + bias[e];
+    if (n + V <= g.N) {
+        if (zb) {
+            Pack<T, V> zz;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] += (float)b.v[e];
+            for (int e = 0; e < V; ++e) zz.v[e] = (T)v[e];
+            if constexpr (V % 2 == 0) {
+                typedef unsigned words __attribute__((ext_vector_type(V / 2), aligned(2)));
+                words w;
+                __builtin_memcpy(&w, &zz, sizeof(zz));
+                __builtin_nontemporal_store(w, (words*)(zb + off));
+            } else {
+                store_pack<T, V>((T*)(zb + off), zz);
+            }
         }
-        if (g.z) {
-            Pack<T, 8> zz;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) zz.v[e] = (T)v[e];
-            store_pack<T, 8>((T*)g.z + (long long)m * g.N + n, zz);
+        for (int e = 0; e < V; ++e) v[e] = act_value<ACT>(v[e]);
+        if (g.resid) {
+            const Pack<T, V> r = load_pack<T, V>(resid);
+#pragma unroll
+            for (int e = 0; e < V; ++e) v[e] += (float)r.v[e];
         }
+        Pack<T, V> y;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = act_value(v[e], g.act);
-        if (resid) {
-            const Pack<T, 8> r = load_pack<T, 8>(resid + (long long)m * g.ldr + n);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] += (float)r.v[e];
-        }
-        Pack<T, 8> y;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) y.v[e] = (T)v[e];
-        store_pack<T, 8>((T*)g.C + o, y);
+        for (int e = 0; e < V; ++e) y.v[e] = (T)v[e];
+        store_pack<T, V>((T*)(yb + off), y);
     } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
+        for (int e = 0; e < V; ++e) {
             if (n + e >= g.N) break;
-            float s = acc[e] + (bias ? (float)bias[n + e] : 0.f);
-            if (g.z) ((T*)g.z)[(long long)m * g.N + n + e] = (T)s;
-            s = act_value(s, g.act);
-            if (resid) s += (float)resid[(long long)m * g.ldr + n + e];
-            ((T*)g.C)[o + e] = (T)s;
+            if (zb) ((T*)(zb + off))[e] = (T)v[e];
+            float s = act_value<ACT>(v[e]);
+            if (g.resid) s += (float)resid[e];
+            ((T*)(yb + off))[e] = (T)s;
         }
     }
 }
 
-__device__ __forceinline__ void write8_f32(float* c, int N, int m, int n, const float (&acc)[8]) {
-    float* o = c + (long long)m * N + n;
-    if (n + 8 <= N) {
-        Pack<float, 4> a, b;
+template <typename T, int V>
+__device__ __forceinline__ void load_bias(const Prod& g, int n, float (&bias)[V]) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) { a.v[e] = acc[e]; b.v[e] = acc[4 + e]; }
-        store_pack<float, 4>(o, a);
-        store_pack<float, 4>(o + 4, b);
-    } else {
+    for (int e = 0; e < V; ++e) bias[e] = g.bias && n + e < g.N ? (float)((const T*)g.bias)[n + e] : 0.f;
+}
+
+// a wavefront's accumulators: D rows (4 kq + e) = m, D columns (r16), fragment by fragment = neighbouring n of lane r16
+template <typename T, int FI, int FJ, int ACT>
+__device__ __forceinline__ void write_tile(const Prod& g, const f32x4 (&acc)[FI][FJ], int m0, int n0, int lane) {
+    const int r16 = lane & 15, kq = lane >> 4, n = n0 + r16 * FJ;
+    float bias[FJ];
+    load_bias<T, FJ>(g, n, bias);
+    char* yb = (char*)g.C + ((long long)m0 * g.N + n0) * 2;
+    char* zb = g.z ? (char*)g.z + ((long long)m0 * g.N + n0) * 2 : nullptr;
+    const unsigned off = (unsigned)(kq * 4 * g.N + r16 * FJ) * 2;             // below 2^32: at most 128 rows, N < 2^23
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-            if (n + e < N) o[e] = acc[e];
-    }
+    for (int i = 0; i < FI; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int m = m0 + 16 * i + 4 * kq + e;
+            float v[FJ];
+#pragma unroll
+            for (int j = 0; j < FJ; ++j) v[j] = acc[i][j][e];
+            if (m < g.M && n < g.N) write_row<T, FJ, ACT>(g, yb, zb, off + (unsigned)((16 * i + e) * g.N) * 2, m, n, v, bias);
+        }
 }
 
 // ---- the tile kernel: 4 wavefronts as 2 x 2, two LDS buffers, one barrier a slab ------------------------------------------------
-template <typename T, bool TA, bool TB, bool DIRECT, int BM, int BN, int BK, bool PARTIAL>
-__device__ __forceinline__ void tile_item(const Prod& g, int vid, char* lds) {
-    using LA = Tile16<BM, BK, TA, false>;
-    using LB = Tile16<BN, BK, TB, true>;
-    constexpr int kStage = LA::kBytes + LB::kBytes;
-    constexpr int FI = BM / 32, FJ = BN / 32;                                 // fragments of a wavefront
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+template <typename T, bool TR, bool DIRECT, int BM, int BN, int BK>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void half_gemm(const Prod g) {
+    constexpr int WM = BM / 2, WN = BN / 2, FI = WM / 16, FJ = WN / 16;       // a wavefront's part, its fragments
+    using SA = Stager<T, BM, BK, TR, DIRECT, 0>;
+    using SB = Stager<T, BN, BK, TR, DIRECT, TR ? 0 : WN>;
+    constexpr int kA = SA::L::kBytes, kStage = kA + SB::L::kBytes;
+    __shared__ __attribute__((aligned(1024))) char lds[2 * kStage];
+    // workgroup b runs on XCD b % 8: every XCD a contiguous run of (slice, tile) pairs, so that tiles sharing rows meet in one L2
+    const int per_xcd = (gridDim.x + 7) >> 3;
+    const int vid = (blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3);
+    if (vid >= g.total) return;                                               // uniform: the grid is rounded up to a multiple of 8
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int tile = vid % g.tiles, slice = vid / g.tiles;
     const int tm = tile / g.tiles_n, tn = tile - tm * g.tiles_n;
     const int m0 = tm * BM, n0 = tn * BN;
     const int nslab = g.slabs + (slice < g.slabs_rem ? 1 : 0);
     const int k0 = (slice * g.slabs + (slice < g.slabs_rem ? slice : g.slabs_rem)) * BK;
-    Stager<T, LA, 256, BM, BK, TA, DIRECT> sa;
-    Stager<T, LB, 256, BN, BK, TB, DIRECT> sb;
+    SA sa;
+    SB sb;
     sa.init((const T*)g.A, g.lda, m0, g.M, k0, g.K, tid);
     sb.init((const T*)g.B, g.ldb, n0, g.N, k0, g.K, tid);
-    const int wr = wave >> 1, wc = wave & 1;
+    const int wm = (wave >> 1) * WM, wn = (wave & 1) * WN;
     f32x4 acc[FI][FJ];
 #pragma unroll
     for (int i = 0; i < FI; ++i)
 #pragma unroll
         for (int j = 0; j < FJ; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
     sa.load(lds, wave);
-    sb.load(lds + LA::kBytes, wave);
+    sb.load(lds + kA, wave);
     sa.store(lds, tid);
-    sb.store(lds + LA::kBytes, tid);
+    sb.store(lds + kA, tid);
     for (int t = 0; t < nslab; ++t) {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();                                                      // slab t is in LDS; the other buffer is free
@@ -282,59 +326,54 @@ __device__ __forceinline__ void tile_item(const Prod& g, int vid, char* lds) {
             sa.advance();
             sb.advance();
             sa.load(nxt, wave);
-            sb.load(nxt + LA::kBytes, wave);
+            sb.load(nxt + kA, wave);
         }
 #pragma unroll
         for (int s = 0; s < BK / 32; ++s) {
             uint4 fa[FI], fb[FJ];
 #pragma unroll
-            for (int i = 0; i < FI; ++i) fa[i] = LA::read(cur, wr * (BM / 2), i, s, lane);
+            for (int i = 0; i < FI; ++i) fa[i] = SA::L::read(cur, wm, i, s, lane);
 #pragma unroll
-            for (int j = 0; j < FJ; ++j) fb[j] = LB::read(cur + LA::kBytes, wc * (BN / 2), j, s, lane);
+            for (int j = 0; j < FJ; ++j) fb[j] = SB::L::read(cur + kA, wn, j, s, lane);
 #pragma unroll
             for (int i = 0; i < FI; ++i)
 #pragma unroll
-                for (int j = 0; j < FJ; ++j) acc[i][j] = mfma<T>(fb[j], fa[i], acc[i][j]);   // D rows = n, D columns = m
+                for (int j = 0; j < FJ; ++j) acc[i][j] = mfma<T>(fa[i], fb[j], acc[i][j]);   // D rows = m, D columns = n
         }
         if (t + 1 < nslab) {
             sa.store(nxt, tid);
-            sb.store(nxt + LA::kBytes, tid);
+            sb.store(nxt + kA, tid);
         }
     }
-    const int r16 = lane & 15, kq = lane >> 4;
+    if constexpr (TR) {                                                       // fp32 partial tile of this slice
+        const int r16 = lane & 15, kq = lane >> 4;
+        float* o = (float*)g.C + (long long)slice * g.M * g.N;
 #pragma unroll
-    for (int i = 0; i < FI; ++i) {
-        const int m = m0 + wr * (BM / 2) + 16 * i + r16;
-        if (m >= g.M) continue;
+        for (int i = 0; i < FI; ++i)
 #pragma unroll
-        for (int j = 0; j < FJ; j += 2) {
-            const int n = n0 + wc * (BN / 2) + 16 * j + 8 * kq;
-            if (n >= g.N) continue;
-            float v[8];
+            for (int e = 0; e < 4; ++e) {
+                const int m = m0 + wm + 16 * i + 4 * kq + e;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) { v[e] = acc[i][j][e]; v[4 + e] = acc[i][j + 1][e]; }
-            if constexpr (PARTIAL) write8_f32((float*)g.C + (long long)slice * g.M * g.N, g.N, m, n, v);
-            else write8<T>(g, m, n, v);
-        }
+                for (int j = 0; j < FJ; ++j) {
+                    const int n = n0 + wn + 16 * j + r16;
+                    if (m < g.M && n < g.N) o[(long long)m * g.N + n] = acc[i][j][e];
+                }
+            }
+    } else {
+        if (g.act == HD_ACT_GELU) write_tile<T, FI, FJ, HD_ACT_GELU>(g, acc, m0 + wm, n0 + wn, lane);
+        else if (g.act == HD_ACT_RELU) write_tile<T, FI, FJ, HD_ACT_RELU>(g, acc, m0 + wm, n0 + wn, lane);
+        else write_tile<T, FI, FJ, HD_ACT_IDENTITY>(g, acc, m0 + wm, n0 + wn, lane);
     }
 }
 
-template <typename T, bool TA, bool TB, bool DIRECT, int BM, int BN, int BK, bool PARTIAL>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void half_gemm(const Prod g) {
-    __shared__ __attribute__((aligned(1024))) char lds[2 * (BM + BN) * BK * 2];
-    // workgroup b runs on XCD b % 8: every XCD a contiguous run of (slice, tile) pairs, so that tiles sharing rows meet in one L2
-    const int per_xcd = (gridDim.x + 7) >> 3;
-    const int vid = (blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3);
-    if (vid >= g.total) return;                                               // uniform: the grid is rounded up to a multiple of 8
-    tile_item<T, TA, TB, DIRECT, BM, BN, BK, PARTIAL>(g, vid, lds);
-}
-
-// ---- dz = g * act'(z) and the column sums of the unrounded products --------------------------------------------------------------
-// A thread owns 8 columns and every (256 / lanes)-th row of the workgroup's rows; part[workgroup][N] gets the sums.
-template <typename T>
-__global__ __launch_bounds__(256) void act_bwd_k(const T* __restrict__ g, long long ldg, const T* __restrict__ z, int M, int N, int act,
-                                                 int log2_lanes, int rows_wg, int col_tiles, T* __restrict__ dz, float* __restrict__ part) {
-    __shared__ float red[256 * 8];
+// ---- dz = g * act'(z), the column sums of the unrounded products, and W^T ---------------------------------------------------------
+// A thread owns 8 columns and every (256 / lanes)-th row of the workgroup's rows, four rows in flight; part[row block][N] gets
+// the sums.  dz has the row pitch lddz, a multiple of 64, and zeros up to the next multiple of 8 columns, so that the products
+// take whole chunks.  The workgroups behind transpose W (N, K) into wt (K, N) with the same pitch and padding.
+template <typename T, int ACT>
+__device__ __forceinline__ void dz_block(const T* __restrict__ g, long long ldg, const T* __restrict__ z, int M, int N, int log2_lanes,
+                                         int rows_wg, int col_tiles, T* __restrict__ dz, long long lddz, float* __restrict__ part,
+                                         float* red) {
     const int lanes = 1 << log2_lanes, slots = 256 >> log2_lanes;
     const int rb = blockIdx.x / col_tiles, ct = blockIdx.x - rb * col_tiles;
     const int n = (ct * lanes + (threadIdx.x & (lanes - 1))) * 8;
@@ -343,36 +382,37 @@ __global__ __launch_bounds__(256) void act_bwd_k(const T* __restrict__ g, long l
     float s[8] = {};
     if (n < N) {
         const bool whole = n + 8 <= N;
-        for (int m = m0 + slot; m < m1; m += slots) {
-            Pack<T, 8> a, b;
-            const T* gp = g + (long long)m * ldg + n;
-            const T* zp = z + (long long)m * N + n;
-            if (whole) {
-                a = load_pack<T, 8>(gp);
-                if (act != HD_ACT_IDENTITY) b = load_pack<T, 8>(zp);
-            } else {
+        constexpr int U = 4;
+        for (int m = m0 + slot; m < m1; m += U * slots) {
+            Pack<T, 8> a[U], b[U];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    a.v[e] = n + e < N ? gp[e] : (T)0.f;
-                    b.v[e] = act != HD_ACT_IDENTITY && n + e < N ? zp[e] : (T)0.f;
-                }
-            }
-            Pack<T, 8> o;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const float d = act != HD_ACT_IDENTITY ? (float)a.v[e] * act_slope((float)b.v[e], act) : (float)a.v[e];
-                s[e] += d;
-                o.v[e] = (T)d;
-            }
-            if (dz) {
-                T* p = dz + (long long)m * N + n;
+            for (int u = 0; u < U; ++u) {
+                const int r = m + u * slots < m1 ? m + u * slots : m;          // a row that is not there: read another, count none
+                const T* gp = g + (long long)r * ldg + n;
+                const T* zp = z + (long long)r * N + n;
                 if (whole) {
-                    store_pack<T, 8>(p, o);
+                    a[u] = load_pack<T, 8>(gp);
+                    if constexpr (ACT != HD_ACT_IDENTITY) b[u] = load_pack<T, 8>(zp);
                 } else {
 #pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        if (n + e < N) p[e] = o.v[e];
+                    for (int e = 0; e < 8; ++e) {
+                        a[u].v[e] = n + e < N ? gp[e] : (T)0.f;
+                        if constexpr (ACT != HD_ACT_IDENTITY) b[u].v[e] = n + e < N ? zp[e] : (T)0.f;
+                    }
                 }
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (m + u * slots >= m1) break;
+                Pack<T, 8> o;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    float d = (float)a[u].v[e];
+                    if constexpr (ACT != HD_ACT_IDENTITY) d *= act_slope<ACT>((float)b[u].v[e]);
+                    s[e] += d;
+                    o.v[e] = (T)d;
+                }
+                if (dz) store_pack<T, 8>(dz + (long long)(m + u * slots) * lddz + n, o);   // columns behind N: 0 * slope(0) = 0
             }
         }
     }
@@ -388,6 +428,28 @@ __global__ __launch_bounds__(256) void act_bwd_k(const T* __restrict__ g, long l
             if (n + e < N) part[(long long)rb * N + n + e] = t;
         }
     }
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void act_bwd_k(const T* __restrict__ g, long long ldg, const T* __restrict__ z, int M, int N, int act,
+                                                 int log2_lanes, int rows_wg, int col_tiles, int dz_wgs, T* __restrict__ dz, long long lddz,
+                                                 float* __restrict__ part, const T* __restrict__ w, long long ldw, int K, T* __restrict__ wt) {
+    __shared__ float red[256 * 8];
+    if ((int)blockIdx.x < dz_wgs) {
+        if (act == HD_ACT_GELU) dz_block<T, HD_ACT_GELU>(g, ldg, z, M, N, log2_lanes, rows_wg, col_tiles, dz, lddz, part, red);
+        else if (act == HD_ACT_RELU) dz_block<T, HD_ACT_RELU>(g, ldg, z, M, N, log2_lanes, rows_wg, col_tiles, dz, lddz, part, red);
+        else dz_block<T, HD_ACT_IDENTITY>(g, ldg, z, M, N, log2_lanes, rows_wg, col_tiles, dz, lddz, part, red);
+        return;
+    }
+    T* tile = (T*)red;                                                        // 32 x 33
+    const int tk = (K + 31) / 32, b = (int)blockIdx.x - dz_wgs, n0 = b / tk * 32, k0 = b % tk * 32;
+    const int c = threadIdx.x & 31, r0 = threadIdx.x >> 5;
+#pragma unroll
+    for (int r = r0; r < 32; r += 8) tile[r * 33 + c] = n0 + r < N && k0 + c < K ? w[(long long)(n0 + r) * ldw + k0 + c] : (T)0.f;
+    __syncthreads();
+#pragma unroll
+    for (int r = r0; r < 32; r += 8)
+        if (k0 + r < K && n0 + c < (N + 7) / 8 * 8) wt[(long long)(k0 + r) * lddz + n0 + c] = tile[c * 33 + r];
 }
 
 // ---- partial sums in order: dW from its slices, db from its row blocks -----------------------------------------------------------
@@ -440,58 +502,72 @@ inline bool direct_ok(const void* p, int64_t ld, int64_t inner, int64_t outer) {
     return (uintptr_t)p % 16 == 0 && inner % 8 == 0 && (ld % 8 == 0 || outer == 1);
 }
 
-constexpr int kBM = 128, kBN = 128, kBK = 64;
-
-template <typename T, bool TA, bool TB, bool PARTIAL>
-void launch_product(Prod g, int slices, bool direct, hipStream_t st) {
-    g.tiles_n = (g.N + kBN - 1) / kBN;
-    g.tiles = (g.M + kBM - 1) / kBM * g.tiles_n;
+template <typename T, bool TR, int BM, int BN, int BK>
+void launch_tiles(Prod g, int slices, bool direct, hipStream_t st) {
+    g.tiles_n = (g.N + BN - 1) / BN;
+    g.tiles = (g.M + BM - 1) / BM * g.tiles_n;
     g.total = g.tiles * slices;
-    const int slabs = (g.K + kBK - 1) / kBK;
+    const int slabs = (g.K + BK - 1) / BK;
     g.slabs = slabs / slices;
     g.slabs_rem = slabs % slices;
     const unsigned grid = (unsigned)((g.total + 7) / 8 * 8);
-    if (direct) half_gemm<T, TA, TB, true, kBM, kBN, kBK, PARTIAL><<<grid, 256, 0, st>>>(g);
-    else half_gemm<T, TA, TB, false, kBM, kBN, kBK, PARTIAL><<<grid, 256, 0, st>>>(g);
+    if (direct) half_gemm<T, TR, true, BM, BN, BK><<<grid, 256, 0, st>>>(g);
+    else half_gemm<T, TR, false, BM, BN, BK><<<grid, 256, 0, st>>>(g);
 }
 
-inline int dw_slices(int64_t R, int64_t P, int64_t Q) {
-    // one resident round of two workgroups per CU; slices of at least two slabs
-    const int64_t tiles = ((P + kBM - 1) / kBM) * ((Q + kBN - 1) / kBN);
-    int64_t s = 512 / tiles;
-    const int64_t most = (R + 2 * kBK - 1) / (2 * kBK);
+inline int64_t tiles_of(int64_t M, int64_t N, int64_t bm, int64_t bn) { return ((M + bm - 1) / bm) * ((N + bn - 1) / bn); }
+// fewer than this many large tiles leave CUs idle: the 64 x 64 tiles fill them
+constexpr int64_t kFewTiles = 256;
+
+template <typename T>
+void launch_product(const Prod& g, bool direct, hipStream_t st) {
+    if (tiles_of(g.M, g.N, 128, 192) >= kFewTiles) launch_tiles<T, false, 128, 192, 32>(g, 1, direct, st);
+    else launch_tiles<T, false, 64, 64, 32>(g, 1, direct, st);
+}
+
+// slices of dW's contraction over R rows: one resident round of workgroups, slices of at least four slabs
+struct DwPlan { bool large; int slices; };
+inline DwPlan dw_plan(int64_t R, int64_t P, int64_t Q) {
+    DwPlan p;
+    p.large = R >= 2048 && tiles_of(P, Q, 128, 192) >= 8;
+    const int64_t tiles = p.large ? tiles_of(P, Q, 128, 192) : tiles_of(P, Q, 64, 64);
+    int64_t s = (p.large ? 512 : 1024) / tiles;
+    const int64_t most = (R + 127) / 128;
     s = s > most ? most : s;
-    return (int)(s < 1 ? 1 : (s > 64 ? 64 : s));
+    p.slices = (int)(s < 1 ? 1 : (s > 64 ? 64 : s));
+    return p;
 }
 
 struct BwdPlan {
-    int log2_lanes, col_tiles, rows_wg, row_wgs, slices;
-    bool need_dz;
-    int64_t off_part, off_ws, bytes;
+    int log2_lanes, col_tiles, rows_wg, row_wgs;
+    DwPlan dw;
+    int64_t lddz;
+    int64_t off_wt, off_part, off_ws, bytes;
 };
 
-BwdPlan bwd_plan(int64_t M, int64_t N, int64_t K, int act) {
+BwdPlan bwd_plan(int64_t M, int64_t N, int64_t K) {
     BwdPlan p;
     const int64_t groups = (N + 7) / 8;
     p.log2_lanes = 0;
     while (p.log2_lanes < 8 && (int64_t(1) << p.log2_lanes) < groups) ++p.log2_lanes;
     p.col_tiles = (int)((groups + (1 << p.log2_lanes) - 1) >> p.log2_lanes);
     const int slots = 256 >> p.log2_lanes;
-    // about 1024 workgroups, at least 8 rows for a thread to sum
+    // about 1024 workgroups, at least 4 rows for a thread
     int64_t rows = (M * p.col_tiles + 1023) / 1024;
-    rows = rows < 8 * slots ? 8 * slots : rows;
-    rows = (rows + slots - 1) / slots * slots;
+    rows = (rows + 4 * slots - 1) / (4 * slots) * (4 * slots);
     p.rows_wg = (int)rows;
     p.row_wgs = (int)((M + rows - 1) / rows);
-    p.slices = dw_slices(M, N, K);
-    p.need_dz = act != HD_ACT_IDENTITY;
+    p.dw = dw_plan(M, N, K);
+    p.lddz = (N + 63) / 64 * 64;
     auto up = [](int64_t b) { return (b + 255) / 256 * 256; };
-    int64_t at = p.need_dz ? up(M * N * 2) : 0;
+    int64_t at = up(M * p.lddz * 2);
+    p.off_wt = at;
+    at += up(K * p.lddz * 2);
     p.off_part = at;
     at += up((int64_t)p.row_wgs * N * 4);
     p.off_ws = at;
-    at += up((int64_t)p.slices * N * K * 4);
-    p.bytes = at > 256 ? at : 256;
+    at += up((int64_t)p.dw.slices * N * K * 4);
+    p.bytes = at;
     return p;
 }
 
@@ -500,12 +576,12 @@ bool known_act(int a) { return a == HD_ACT_IDENTITY || a == HD_ACT_RELU || a == 
 #define HD_LINEAR_SHAPE(fn)                                                                                                     \
     HD_REQUIRE(dtype == HD_DT_BF16 || dtype == HD_DT_F16, fn ": element type bf16 or fp16, not %d", dtype);                      \
     HD_REQUIRE(known_act(act), fn ": activation identity, relu or gelu, not %d", act);                                          \
-    HD_REQUIRE(M >= 0 && M < (1LL << 30) && N >= 1 && N < (1LL << 24) && K >= 1 && K < (1LL << 24), fn ": bad shape");             \
+    HD_REQUIRE(M >= 0 && M < (1LL << 30) && N >= 1 && N < (1LL << 22) && K >= 1 && K < (1LL << 22), fn ": bad shape");             \
     HD_REQUIRE(ldx >= K && ldw >= K, fn ": row pitch below the width")
 
 template <typename T>
 int linear_fwd(const Prod& g, bool direct, hipStream_t s) {
-    launch_product<T, false, false, false>(g, 1, direct, s);
+    launch_product<T>(g, direct, s);
     return check_launch("hd_linear_act_fwd");
 }
 
@@ -514,28 +590,34 @@ int linear_bwd(const T* g, int64_t ldg, const T* z, const T* x, int64_t ldx, con
                int act, T* dx, T* dw, T* db, const BwdPlan& p, unsigned char* ws, hipStream_t s) {
     const T* dz = g;
     long long lddz = ldg;
+    T* wt = (T*)(ws + p.off_wt);
     float* part = db ? (float*)(ws + p.off_part) : nullptr;
-    if (p.need_dz || db) {
-        T* o = p.need_dz && (dx || dw) ? (T*)ws : nullptr;
-        act_bwd_k<T><<<(unsigned)(p.row_wgs * p.col_tiles), 256, 0, s>>>(g, ldg, z, (int)M, (int)N, act, p.log2_lanes, p.rows_wg, p.col_tiles,
-                                                                        o, part);
-        if (o) { dz = o; lddz = N; }
-    }
+    // dz itself is written unless it is g and g's rows can be staged as they are
+    const bool copy = (dx || dw) && (act != HD_ACT_IDENTITY || !direct_ok(g, ldg, N, M));
+    const int dz_wgs = copy || db ? p.row_wgs * p.col_tiles : 0;
+    const int64_t wt_wgs = dx ? ((N + 31) / 32) * ((K + 31) / 32) : 0;
+    if (dz_wgs + wt_wgs)
+        act_bwd_k<T><<<(unsigned)(dz_wgs + wt_wgs), 256, 0, s>>>(g, ldg, z, (int)M, (int)N, act, p.log2_lanes, p.rows_wg, p.col_tiles, dz_wgs,
+                                                                copy ? (T*)ws : nullptr, p.lddz, part, w, ldw, (int)K, wt);
+    if (copy) { dz = (const T*)ws; lddz = p.lddz; }
     Prod q = {};
     q.act = HD_ACT_IDENTITY;
-    if (dx) {                                                                 // (M, K) = dz (M, N) . W (N, K)
-        q.A = dz; q.lda = lddz; q.B = w; q.ldb = ldw; q.M = (int)M; q.N = (int)K; q.K = (int)N; q.C = dx; q.ldc = K;
-        launch_product<T, false, true, false>(q, 1, direct_ok(dz, lddz, N, M) && direct_ok(w, ldw, K, N), s);
+    q.A = dz; q.lda = lddz;
+    if (dx) {                                                                 // (M, K) = dz (M, N) . W^T (K, N), zeros up to whole chunks
+        q.B = wt; q.ldb = p.lddz; q.M = (int)M; q.N = (int)K; q.K = (int)((N + 7) / 8 * 8); q.C = dx;
+        launch_product<T>(q, true, s);
     }
     if (dw) {                                                                 // (N, K) = dz^T (N, M) . x (M, K)
-        q.A = dz; q.lda = lddz; q.B = x; q.ldb = ldx; q.M = (int)N; q.N = (int)K; q.K = (int)M; q.C = ws + p.off_ws; q.ldc = K;
-        launch_product<T, true, true, true>(q, p.slices, direct_ok(dz, lddz, N, M) && direct_ok(x, ldx, K, M), s);
+        q.B = x; q.ldb = ldx; q.M = (int)N; q.N = (int)K; q.K = (int)M; q.C = ws + p.off_ws;
+        const bool direct = direct_ok(x, ldx, K, M);
+        if (p.dw.large) launch_tiles<T, true, 128, 192, 32>(q, p.dw.slices, direct, s);
+        else launch_tiles<T, true, 64, 64, 32>(q, p.dw.slices, direct, s);
     }
     if (dw || db) {
         const int64_t count = dw ? N * K : 0;
         const int w_wgs = (int)((count + 1023) / 1024), b_wgs = db ? (int)((N + 15) / 16) : 0;
-        half_reduce_k<T><<<(unsigned)(w_wgs + b_wgs), 256, 0, s>>>((const float*)(ws + p.off_ws), p.slices, count, dw, w_wgs, part, p.row_wgs,
-                                                                   (int)N, db);
+        half_reduce_k<T><<<(unsigned)(w_wgs + b_wgs), 256, 0, s>>>((const float*)(ws + p.off_ws), p.dw.slices, count, dw, w_wgs, part,
+                                                                   p.row_wgs, (int)N, db);
     }
     return check_launch("hd_linear_act_bwd");
 }
@@ -550,17 +632,17 @@ extern "C" int hd_linear_act_fwd(const void* x, int64_t ldx, const void* w, int6
     HD_REQUIRE(!resid || ldr >= 0, "hd_linear_act_fwd: negative pitch");
     HD_REQUIRE((((uintptr_t)x | (uintptr_t)w | (uintptr_t)y | (uintptr_t)z | (uintptr_t)bias | (uintptr_t)resid) & 1) == 0,
                "hd_linear_act_fwd: pointer not aligned to the element");
-    HD_REQUIRE(((M + kBM - 1) / kBM) * ((N + kBN - 1) / kBN) < (1LL << 31) - 8, "hd_linear_act_fwd: too many tiles");
+    HD_REQUIRE(tiles_of(M, N, 64, 64) < (1LL << 31) - 8, "hd_linear_act_fwd: too many tiles");
     Prod g = {};
     g.A = x; g.lda = ldx; g.B = w; g.ldb = ldw; g.M = (int)M; g.N = (int)N; g.K = (int)K;
-    g.C = y; g.ldc = N; g.bias = bias; g.resid = resid; g.ldr = ldr; g.z = z; g.act = act;
+    g.C = y; g.bias = bias; g.resid = resid; g.ldr = ldr; g.z = z; g.act = act;
     const bool direct = direct_ok(x, ldx, K, M) && direct_ok(w, ldw, K, N);
     return dtype == HD_DT_BF16 ? linear_fwd<bf16>(g, direct, (hipStream_t)st) : linear_fwd<f16>(g, direct, (hipStream_t)st);
 }
 
 extern "C" int64_t hd_linear_act_bwd_workspace_bytes(int64_t M, int64_t N, int64_t K, int act) {
-    if (M < 0 || N < 1 || K < 1 || M >= (1LL << 30) || N >= (1LL << 24) || K >= (1LL << 24) || !known_act(act)) return 0;
-    return bwd_plan(M, N, K, act).bytes;
+    if (M < 0 || N < 1 || K < 1 || M >= (1LL << 30) || N >= (1LL << 22) || K >= (1LL << 22) || !known_act(act)) return 0;
+    return bwd_plan(M, N, K).bytes;
 }
 
 extern "C" int hd_linear_act_bwd(const void* g, int64_t ldg, const void* z, const void* x, int64_t ldx, const void* w, int64_t ldw,
@@ -575,11 +657,10 @@ extern "C" int hd_linear_act_bwd(const void* g, int64_t ldg, const void* z, cons
     HD_REQUIRE((((uintptr_t)g | (uintptr_t)z | (uintptr_t)x | (uintptr_t)w | (uintptr_t)dx | (uintptr_t)dw | (uintptr_t)db) & 1) == 0,
                "hd_linear_act_bwd: pointer not aligned to the element");
     HD_REQUIRE(M > 0, "hd_linear_act_bwd: no rows (the gradients are zeros; fill them)");
-    const BwdPlan p = bwd_plan(M, N, K, act);
+    const BwdPlan p = bwd_plan(M, N, K);
     HD_REQUIRE(workspace_bytes >= p.bytes, "hd_linear_act_bwd: workspace of %lld bytes required, got %lld", (long long)p.bytes,
                (long long)workspace_bytes);
-    HD_REQUIRE(((M + kBM - 1) / kBM) * ((K + kBN - 1) / kBN) < (1LL << 31) - 8 &&
-                   ((N + kBM - 1) / kBM) * ((K + kBN - 1) / kBN) * p.slices < (1LL << 31) - 8,
+    HD_REQUIRE(tiles_of(M, K, 64, 64) < (1LL << 31) - 8 && tiles_of(N, K, 32, 32) < (1LL << 30) && N * K < (1LL << 38),
                "hd_linear_act_bwd: too many tiles");
     unsigned char* ws = (unsigned char*)workspace;
     hipStream_t s = (hipStream_t)st;
