@@ -370,6 +370,51 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void h
 // A thread owns 8 columns and every (256 / lanes)-th row of the workgroup's rows, four rows in flight; part[row block][N] gets
 // the sums.  dz has the row pitch lddz, a multiple of 64, and zeros up to the next multiple of 8 columns, so that the products
 // take whole chunks.  The workgroups behind transpose W (N, K) into wt (K, N) with the same pitch and padding.
+// n: the thread's first column.  WIDE (N >= 8): the thread of the last, short group takes the last 8 columns, of which
+// some belong to its neighbour: those come out twice, equal, and are summed once; it also writes the zeros behind column N.
+template <typename T, int ACT, bool WIDE>
+__device__ __forceinline__ void dz_rows(const T* __restrict__ g, long long ldg, const T* __restrict__ z, int N, int n, int m, int m1, int slots,
+                                        T* __restrict__ dz, long long lddz, float (&s)[8]) {
+    constexpr int U = 4;
+    auto fetch = [&](const T* p) {
+        Pack<T, 8> v;
+        if constexpr (WIDE) {
+            v = load_pack<T, 8>(p);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v.v[e] = n + e < N ? p[e] : (T)0.f;
+        }
+        return v;
+    };
+    const int pads = WIDE && dz && n + 8 == N ? (8 - N % 8) % 8 : 0;
+    for (; m < m1; m += U * slots) {
+        Pack<T, 8> a[U], b[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int r = m + u * slots < m1 ? m + u * slots : m;              // a row that is not there: read another, count none
+            a[u] = fetch(g + (long long)r * ldg + n);
+            if constexpr (ACT != HD_ACT_IDENTITY) b[u] = fetch(z + (long long)r * N + n);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (m + u * slots >= m1) break;
+            Pack<T, 8> o;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                float d = (float)a[u].v[e];
+                if constexpr (ACT != HD_ACT_IDENTITY) d *= act_slope<ACT>((float)b[u].v[e]);
+                s[e] += d;
+                o.v[e] = (T)d;
+            }
+            if (dz) {
+                T* out = dz + (long long)(m + u * slots) * lddz + n;
+                store_pack<T, 8>(out, o);                                     // not WIDE: 0 * slope(0) = 0 behind N
+                for (int e = 0; e < pads; ++e) out[8 + e] = (T)0.f;
+            }
+        }
+    }
+}
+
 template <typename T, int ACT>
 __device__ __forceinline__ void dz_block(const T* __restrict__ g, long long ldg, const T* __restrict__ z, int M, int N, int log2_lanes,
                                          int rows_wg, int col_tiles, T* __restrict__ dz, long long lddz, float* __restrict__ part,
@@ -380,40 +425,13 @@ __device__ __forceinline__ void dz_block(const T* __restrict__ g, long long ldg,
     const int slot = threadIdx.x >> log2_lanes;
     const int m0 = rb * rows_wg, m1 = M - m0 < rows_wg ? M : m0 + rows_wg;
     float s[8] = {};
+    int skip = 0;                                                             // columns before the thread's own
     if (n < N) {
-        const bool whole = n + 8 <= N;
-        constexpr int U = 4;
-        for (int m = m0 + slot; m < m1; m += U * slots) {
-            Pack<T, 8> a[U], b[U];
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int r = m + u * slots < m1 ? m + u * slots : m;          // a row that is not there: read another, count none
-                const T* gp = g + (long long)r * ldg + n;
-                const T* zp = z + (long long)r * N + n;
-                if (whole) {
-                    a[u] = load_pack<T, 8>(gp);
-                    if constexpr (ACT != HD_ACT_IDENTITY) b[u] = load_pack<T, 8>(zp);
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        a[u].v[e] = n + e < N ? gp[e] : (T)0.f;
-                        if constexpr (ACT != HD_ACT_IDENTITY) b[u].v[e] = n + e < N ? zp[e] : (T)0.f;
-                    }
-                }
-            }
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                if (m + u * slots >= m1) break;
-                Pack<T, 8> o;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    float d = (float)a[u].v[e];
-                    if constexpr (ACT != HD_ACT_IDENTITY) d *= act_slope<ACT>((float)b[u].v[e]);
-                    s[e] += d;
-                    o.v[e] = (T)d;
-                }
-                if (dz) store_pack<T, 8>(dz + (long long)(m + u * slots) * lddz + n, o);   // columns behind N: 0 * slope(0) = 0
-            }
+        if (N >= 8) {
+            skip = n + 8 <= N ? 0 : n + 8 - N;
+            dz_rows<T, ACT, true>(g, ldg, z, N, n - skip, m0 + slot, m1, slots, dz, lddz, s);
+        } else {
+            dz_rows<T, ACT, false>(g, ldg, z, N, n, m0 + slot, m1, slots, dz, lddz, s);
         }
     }
     if (!part) return;                                                        // uniform
@@ -425,7 +443,7 @@ __device__ __forceinline__ void dz_block(const T* __restrict__ g, long long ldg,
         for (int e = 0; e < 8; ++e) {
             float t = 0.f;
             for (int q = 0; q < slots; ++q) t += red[e * 256 + q * lanes + threadIdx.x];
-            if (n + e < N) part[(long long)rb * N + n + e] = t;
+            if (e >= skip && n - skip + e < N) part[(long long)rb * N + n - skip + e] = t;
         }
     }
 }
