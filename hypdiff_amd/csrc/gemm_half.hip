@@ -208,12 +208,13 @@ struct Prod {
     void* z;                        // (M, N) contiguous, or null
     long long ldr;
     int act;
+    int z_past;                     // store z past the caches
     int tiles_n, tiles, total;      // total = tiles * slices
     int slabs, slabs_rem;           // slice s covers slabs + (s < slabs_rem) slabs of BK
 };
 
 // V neighbouring n of row m leave: bias, z, activation, residual, one rounding.  yb / zb: the tile's first element, off: this lane's
-// byte offset in the tile.  z is not read before the backward pass: stored past the caches (8 % of the training forward).
+// byte offset in the tile.
 template <typename T, int V, int ACT>
 __device__ __forceinline__ void write_row(const Prod& g, char* yb, char* zb, unsigned off, int m, int n, const float (&acc)[V],
                                           const float (&bias)[V]) {
@@ -230,7 +231,8 @@ __device__ __forceinline__ void write_row(const Prod& g, char* yb, char* zb, uns
                 typedef unsigned words __attribute__((ext_vector_type(V / 2), aligned(2)));
                 words w;
                 __builtin_memcpy(&w, &zz, sizeof(zz));
-                __builtin_nontemporal_store(w, (words*)(zb + off));
+                if (g.z_past) __builtin_nontemporal_store(w, (words*)(zb + off));
+                else __builtin_memcpy(zb + off, &w, sizeof(w));
             } else {
                 store_pack<T, V>((T*)(zb + off), zz);
             }
@@ -364,6 +366,98 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void h
         else if (g.act == HD_ACT_RELU) write_tile<T, FI, FJ, HD_ACT_RELU>(g, acc, m0 + wm, n0 + wn, lane);
         else write_tile<T, FI, FJ, HD_ACT_IDENTITY>(g, acc, m0 + wm, n0 + wn, lane);
     }
+}
+
+// ---- few rows: 32 x 32 tiles, the contraction dealt over the 4 wavefronts -----------------------------------------------------------
+// With so few tiles a slab-by-slab loop is a chain of load latencies (200 x 512 x 512: 8 workgroups of 16 slabs).  Here a
+// wavefront loads the fragments of 4 slabs straight into registers, all in flight together, and multiplies; the four partial
+// tiles meet in LDS, in wavefront order.  Any alignment: a fragment is 8 consecutive k of a row.
+template <typename T>
+__device__ __forceinline__ uint4 load_frag_tail(const T* row, int k, int K) {   // the slab that holds the row's end: zeros behind it
+    Pack<T, 8> v;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const T x = row[k + e < K ? k + e : K - 1];                           // no branch: the loads stay in flight together
+        v.v[e] = k + e < K ? x : (T)0.f;
+    }
+    return __builtin_bit_cast(uint4, v);
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void small_gemm(const Prod g) {
+    __shared__ float red[4][32][36];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int r16 = lane & 15, kq = lane >> 4;
+    const int tm = blockIdx.x / g.tiles_n, tn = blockIdx.x - tm * g.tiles_n;
+    const int m0 = tm * 32, n0 = tn * 32;
+    const T *pa[2], *pb[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {                                             // beyond the matrix: any row
+        const int m = m0 + 16 * i + r16 < g.M ? m0 + 16 * i + r16 : g.M - 1, n = n0 + 16 * i + r16 < g.N ? n0 + 16 * i + r16 : g.N - 1;
+        pa[i] = (const T*)g.A + (long long)m * g.lda;
+        pb[i] = (const T*)g.B + (long long)n * g.ldb;
+    }
+    f32x4 acc[2][2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const int slabs = (g.K + 31) / 32;
+    const int inside = g.K / 32;                                              // slabs without the row's end
+    int t = wave;
+    for (; t + 12 < inside; t += 16) {                                        // slabs t, t + 4, t + 8, t + 12
+        uint4 fa[4][2], fb[4][2];
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int k = (t + 4 * u) * 32 + 8 * kq;
+                fa[u][i] = __builtin_bit_cast(uint4, load_pack<T, 8>(pa[i] + k));
+                fb[u][i] = __builtin_bit_cast(uint4, load_pack<T, 8>(pb[i] + k));
+            }
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) acc[i][j] = mfma<T>(fa[u][i], fb[u][j], acc[i][j]);
+    }
+    for (; t < slabs; t += 4) {                                               // the last few, one at a time
+        uint4 fa[2], fb[2];
+        const int k = t * 32 + 8 * kq;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            if (t < inside) {                                                 // uniform
+                fa[i] = __builtin_bit_cast(uint4, load_pack<T, 8>(pa[i] + k));
+                fb[i] = __builtin_bit_cast(uint4, load_pack<T, 8>(pb[i] + k));
+            } else {
+                fa[i] = load_frag_tail<T>(pa[i], k, g.K);
+                fb[i] = load_frag_tail<T>(pb[i], k, g.K);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) acc[i][j] = mfma<T>(fa[i], fb[j], acc[i][j]);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) red[wave][16 * i + 4 * kq + e][16 * j + r16] = acc[i][j][e];
+    __syncthreads();
+    const int r = tid >> 3, c = (tid & 7) * 4, m = m0 + r, n = n0 + c;
+    if (m >= g.M || n >= g.N) return;
+    float v[4], bias[4];
+    load_bias<T, 4>(g, n, bias);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = ((red[0][r][c + e] + red[1][r][c + e]) + red[2][r][c + e]) + red[3][r][c + e];
+    char* yb = (char*)g.C + ((long long)m * g.N + n) * 2;
+    char* zb = g.z ? (char*)g.z + ((long long)m * g.N + n) * 2 : nullptr;
+    if (g.act == HD_ACT_GELU) write_row<T, 4, HD_ACT_GELU>(g, yb, zb, 0, m, n, v, bias);
+    else if (g.act == HD_ACT_RELU) write_row<T, 4, HD_ACT_RELU>(g, yb, zb, 0, m, n, v, bias);
+    else write_row<T, 4, HD_ACT_IDENTITY>(g, yb, zb, 0, m, n, v, bias);
 }
 
 // ---- dz = g * act'(z), the column sums of the unrounded products, and W^T ---------------------------------------------------------
@@ -534,13 +628,30 @@ void launch_tiles(Prod g, int slices, bool direct, hipStream_t st) {
 }
 
 inline int64_t tiles_of(int64_t M, int64_t N, int64_t bm, int64_t bn) { return ((M + bm - 1) / bm) * ((N + bn - 1) / bn); }
-// fewer than this many large tiles leave CUs idle: the 64 x 64 tiles fill them
-constexpr int64_t kFewTiles = 256;
+
+// Which kernel a product of M x N results takes: 0 small_gemm, 1 64 x 64, 2 128 x 128, 3 128 x 192 (bf16, GELU, us, the kernels
+// side by side):
+//   up to 512 tiles of 32 x 32 small_gemm: 512 x 512 x 512 5.0 against 7.9; above, 64 x 64: 2048 x 512 x 512 8.6 against 12.1
+//   (up to 64 tiles where rows start off 16-byte borders, whose fragments cost more loads: 512 x 800 x 513 16.8 against 9.7)
+//   up to 1280 tiles of 64 x 64 those: 8192 x 512 x 512 13.0 against 15.8; above, the large ones: 16384 x 512 x 512 20.3 against 23.5
+//   of the large ones the one with less time in its rounds over the chip: three 128 x 192 workgroups fit a CU, a round takes 37
+//   (K = 800), four of 128 x 128 take 34: 74750 x 900 151 against 170, 74750 x 512 77 against 66, 74750 x 700 144 against 136
+inline int choose_tiles(int64_t M, int64_t N, bool direct) {
+    if (tiles_of(M, N, 32, 32) <= (direct ? 512 : 64)) return 0;
+    if (tiles_of(M, N, 64, 64) <= 1280) return 1;
+    const int64_t wide = (tiles_of(M, N, 128, 192) + 767) / 768 * 37, square = (tiles_of(M, N, 128, 128) + 1023) / 1024 * 34;
+    return wide <= square ? 3 : 2;
+}
 
 template <typename T>
-void launch_product(const Prod& g, bool direct, hipStream_t st) {
-    if (tiles_of(g.M, g.N, 128, 192) >= kFewTiles) launch_tiles<T, false, 128, 192, 32>(g, 1, direct, st);
-    else launch_tiles<T, false, 64, 64, 32>(g, 1, direct, st);
+void launch_product(Prod g, bool direct, hipStream_t st) {
+    const int v = choose_tiles(g.M, g.N, direct);
+    if (v == 0) {
+        g.tiles_n = (g.N + 31) / 32;
+        small_gemm<T><<<(unsigned)tiles_of(g.M, g.N, 32, 32), 256, 0, st>>>(g);
+    } else if (v == 1) launch_tiles<T, false, 64, 64, 32>(g, 1, direct, st);
+    else if (v == 2) launch_tiles<T, false, 128, 128, 32>(g, 1, direct, st);
+    else launch_tiles<T, false, 128, 192, 32>(g, 1, direct, st);
 }
 
 // slices of dW's contraction over R rows: one resident round of workgroups, slices of at least four slabs
@@ -628,7 +739,7 @@ int linear_bwd(const T* g, int64_t ldg, const T* z, const T* x, int64_t ldx, con
     if (dw) {                                                                 // (N, K) = dz^T (N, M) . x (M, K)
         q.B = x; q.ldb = ldx; q.M = (int)N; q.N = (int)K; q.K = (int)M; q.C = ws + p.off_ws;
         const bool direct = direct_ok(x, ldx, K, M);
-        if (p.dw.large) launch_tiles<T, true, 128, 192, 32>(q, p.dw.slices, direct, s);
+        if (p.dw.large) launch_tiles<T, true, 128, 192, 64>(q, p.dw.slices, direct, s);
         else launch_tiles<T, true, 64, 64, 32>(q, p.dw.slices, direct, s);
     }
     if (dw || db) {
@@ -650,10 +761,12 @@ extern "C" int hd_linear_act_fwd(const void* x, int64_t ldx, const void* w, int6
     HD_REQUIRE(!resid || ldr >= 0, "hd_linear_act_fwd: negative pitch");
     HD_REQUIRE((((uintptr_t)x | (uintptr_t)w | (uintptr_t)y | (uintptr_t)z | (uintptr_t)bias | (uintptr_t)resid) & 1) == 0,
                "hd_linear_act_fwd: pointer not aligned to the element");
-    HD_REQUIRE(tiles_of(M, N, 64, 64) < (1LL << 31) - 8, "hd_linear_act_fwd: too many tiles");
+    HD_REQUIRE(tiles_of(M, N, 32, 32) < (1LL << 31) - 8, "hd_linear_act_fwd: too many tiles");
     Prod g = {};
     g.A = x; g.lda = ldx; g.B = w; g.ldb = ldw; g.M = (int)M; g.N = (int)N; g.K = (int)K;
     g.C = y; g.bias = bias; g.resid = resid; g.ldr = ldr; g.z = z; g.act = act;
+    // a z beside which nothing stays in the 256 MB behind the L2s until the backward pass reads it: 74750 x 900 183 against 200 us
+    g.z_past = M * N >= (1LL << 25);
     const bool direct = direct_ok(x, ldx, K, M) && direct_ok(w, ldw, K, N);
     return dtype == HD_DT_BF16 ? linear_fwd<bf16>(g, direct, (hipStream_t)st) : linear_fwd<f16>(g, direct, (hipStream_t)st);
 }
@@ -678,7 +791,7 @@ extern "C" int hd_linear_act_bwd(const void* g, int64_t ldg, const void* z, cons
     const BwdPlan p = bwd_plan(M, N, K);
     HD_REQUIRE(workspace_bytes >= p.bytes, "hd_linear_act_bwd: workspace of %lld bytes required, got %lld", (long long)p.bytes,
                (long long)workspace_bytes);
-    HD_REQUIRE(tiles_of(M, K, 64, 64) < (1LL << 31) - 8 && tiles_of(N, K, 32, 32) < (1LL << 30) && N * K < (1LL << 38),
+    HD_REQUIRE(tiles_of(M, K, 32, 32) < (1LL << 31) - 8 && tiles_of(N, K, 32, 32) < (1LL << 30) && N * K < (1LL << 38),
                "hd_linear_act_bwd: too many tiles");
     unsigned char* ws = (unsigned char*)workspace;
     hipStream_t s = (hipStream_t)st;
