@@ -18,7 +18,6 @@ PyTorch owns memory, the autograd graph and RNG (and the optimizer unless dist.B
 import os
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib, ops
 
@@ -499,25 +498,31 @@ class EmbeddingAdd(torch.autograd.Function):
         return g, gt, None
 
 
+def _first_order(what):
+    # backward runs with gradients enabled under create_graph=True only.  (torch's once_differentiable decorator refuses the same
+    # at the second backward pass, for 15 us a call: a tenth of a small layer's whole step)
+    if torch.is_grad_enabled():
+        raise NotImplementedError(f"{what}: gradients of gradients (create_graph=True) are not offered")
+
+
 class LinearAct(torch.autograd.Function):
     """resid + act(x W^T + b) on 16-bit operands (ops.linear_act).  The pre-activation is kept in 16 bits (nothing for the
     identity); backward: hd_linear_act_bwd, and the incoming gradient itself for resid."""
 
     @staticmethod
     def forward(ctx, x, w, b, resid, act):
-        y, z = ops._linear_act_fwd(x, w, b, resid, act, want_z=act != 0)
-        ctx.save_for_backward(x, w, z)
-        ctx.act = act
+        y, z, x2, ldx, w2, ldw = ops._linear_act_fwd(x, w, b, resid, act, act != 0)
+        ctx.save_for_backward(x2, w2, z)
+        ctx.args = (ldx, ldw, act, x.shape)
         return y
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, g):
-        x, w, z = ctx.saved_tensors
+        _first_order("linear_act")
         need = ctx.needs_input_grad
-        dx, dw, db = (None, None, None)
-        if any(need[:3]):
-            dx, dw, db = ops._linear_act_bwd(g, z, x, w, ctx.act, *need[:3])
+        x2, w2, z = ctx.saved_tensors
+        dx, dw, db = ops._linear_act_bwd(g, z, x2, w2, *ctx.args, need[0], need[1], need[2]) \
+            if need[0] or need[1] or need[2] else (None, None, None)
         return dx, dw, db, g if need[3] else None, None
 
 
@@ -528,14 +533,13 @@ class Embedding(torch.autograd.Function):
     @staticmethod
     def forward(ctx, table, add, idx, scale, padding):
         ctx.save_for_backward(idx)
-        ctx.scale, ctx.padding, ctx.T = scale, padding, table.shape[0]
+        ctx.args = (table.shape[0], scale, padding)
         return ops._embedding_lookup(table, idx, scale, add)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, g):
-        (idx,) = ctx.saved_tensors
-        gt = ops._embedding_sum(g, idx, ctx.T, ctx.scale, ctx.padding) if ctx.needs_input_grad[0] else None
+        _first_order("embedding")
+        gt = ops._embedding_sum(g, ctx.saved_tensors[0], *ctx.args) if ctx.needs_input_grad[0] else None
         return gt, g if ctx.needs_input_grad[1] else None, None, None, None
 
 

@@ -789,7 +789,7 @@ def linear_act(x, weight, bias=None, act="identity", resid=None):
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, resid)):
         from . import autograd as hag
         return hag.LinearAct.apply(x, weight, bias, resid, code)
-    return _linear_act_fwd(x, weight, bias, resid, code)[0]
+    return _linear_act_fwd(x, weight, bias, resid, code, False)[0]
 
 
 def _matrix(t):
@@ -798,41 +798,42 @@ def _matrix(t):
     if t.dim() != 2:
         t = t.reshape(-1, t.shape[-1])
     rows, cols = t.shape
-    if (cols > 1 and t.stride(1) != 1) or (rows > 1 and t.stride(0) < cols):
-        t = t.contiguous()
-    return t, (t.stride(0) if rows > 1 else cols)
+    pitch, step = t.stride()
+    if (step != 1 and cols > 1) or (pitch < cols and rows > 1):
+        t, pitch = t.contiguous(), cols
+    return t, (pitch if rows > 1 else cols)
 
 
-def _linear_act_fwd(x, w, b, resid, act, want_z=False):
+def _linear_act_fwd(x, w, b, resid, act, want_z):
+    """(y, z or None, x as a matrix, its pitch, w as a matrix, its pitch)"""
     x2, ldx = _matrix(x)
     w2, ldw = _matrix(w)
     M, (N, K) = x2.shape[0], w2.shape
-    y = torch.empty(x.shape[:-1] + (N,), dtype=x.dtype, device=x.device)
-    z = torch.empty(M, N, dtype=x.dtype, device=x.device) if want_z else None
-    if M == 0:
-        return y, z
-    r2, ldr = (None, 0) if resid is None else _pitched(resid.detach().reshape(M, N))
-    b = None if b is None else b.detach().contiguous()
-    _lib.call("hd_linear_act_fwd", _p(x2), ldx, _p(w2), ldw, _p(b), _p(r2), ldr, DT_CODES[x.dtype], M, N, K, act, _p(y), _p(z),
-              _stream())
-    return y, z
+    dt, dev = x.dtype, x.device
+    y = torch.empty(x.shape[:-1] + (N,), dtype=dt, device=dev)
+    z = torch.empty((M, N), dtype=dt, device=dev) if want_z else None
+    if M:
+        r2, ldr = (None, 0) if resid is None else _pitched(resid.detach().reshape(M, N))
+        b = None if b is None else b.detach().contiguous()
+        _lib.call("hd_linear_act_fwd", x2.data_ptr(), ldx, w2.data_ptr(), ldw, _p(b), _p(r2), ldr, DT_CODES[dt], M, N, K, act,
+                  y.data_ptr(), _p(z), raw_stream())
+    return y, z, x2, ldx, w2, ldw
 
 
-def _linear_act_bwd(g, z, x, w, act, need_x, need_w, need_b):
-    _dev(g, x, w)
+def _linear_act_bwd(g, z, x2, w2, ldx, ldw, act, x_shape, need_x, need_w, need_b):
+    _dev(g, x2, w2)
     g2, ldg = _matrix(g)
-    x2, ldx = _matrix(x)
-    w2, ldw = _matrix(w)
     M, (N, K) = x2.shape[0], w2.shape
-    new = torch.zeros if M == 0 else torch.empty
-    dx = new(x.shape, dtype=x.dtype, device=x.device) if need_x else None
-    dw = new(N, K, dtype=x.dtype, device=x.device) if need_w else None
-    db = new(N, dtype=x.dtype, device=x.device) if need_b else None
-    if M > 0:
+    dt, dev = x2.dtype, x2.device
+    new = torch.empty if M else torch.zeros
+    dx = new(x_shape, dtype=dt, device=dev) if need_x else None
+    dw = new((N, K), dtype=dt, device=dev) if need_w else None
+    db = new((N,), dtype=dt, device=dev) if need_b else None
+    if M:
         nbytes = _lib.load().hd_linear_act_bwd_workspace_bytes(M, N, K, act)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
-        _lib.call("hd_linear_act_bwd", _p(g2), ldg, _p(z), _p(x2), ldx, _p(w2), ldw, DT_CODES[x.dtype], M, N, K, act, _p(dx), _p(dw),
-                  _p(db), _p(ws), nbytes, _stream())
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        _lib.call("hd_linear_act_bwd", g2.data_ptr(), ldg, _p(z), x2.data_ptr(), ldx, w2.data_ptr(), ldw, DT_CODES[dt], M, N, K, act,
+                  _p(dx), _p(dw), _p(db), ws.data_ptr(), nbytes, raw_stream())
     return dx, dw, db
 
 

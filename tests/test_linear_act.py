@@ -228,8 +228,9 @@ def test_captured_and_replayed(M, N, K):
     x, w, b, g = new(M, K), new(N, K), new(N), new(M, N)
 
     def both():
-        y, z = ops._linear_act_fwd(x, w, b, None, 6, want_z=True)
-        return (y,) + ops._linear_act_bwd(g, z, x, w, 6, True, True, True)
+        ls = [t.detach().requires_grad_(True) for t in (x, w, b)]
+        y = ops.linear_act(*ls, act="gelu")
+        return (y.detach(),) + torch.autograd.grad(y, ls, g)
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(side):
@@ -256,8 +257,9 @@ def test_two_streams_at_once():
     sets = [(new(3000, 512), new(512, 512), new(512), new(3000, 512)) for _ in range(2)]
 
     def step(x, w, b, g):
-        y, z = ops._linear_act_fwd(x, w, b, None, 6, want_z=True)
-        return (y,) + ops._linear_act_bwd(g, z, x, w, 6, True, True, True)
+        ls = [t.detach().requires_grad_(True) for t in (x, w, b)]
+        y = ops.linear_act(*ls, act="gelu")
+        return (y.detach(),) + torch.autograd.grad(y, ls, g)
     want = [step(*s) for s in sets]
     torch.cuda.synchronize()
     streams = [torch.cuda.Stream() for _ in sets]
@@ -269,6 +271,16 @@ def test_two_streams_at_once():
     for outs, w in zip(got, want):
         for o in outs:
             assert all(torch.equal(a, c) for a, c in zip(o, w))
+
+
+@gpu
+def test_second_derivatives_are_refused():
+    from hypdiff_amd import ops
+    x, w = (torch.randn(8, 8, device="cuda", dtype=torch.bfloat16, requires_grad=True) for _ in range(2))
+    with pytest.raises(NotImplementedError, match="create_graph"):
+        torch.autograd.grad(ops.linear_act(x, w, act="gelu").sum(), [x], create_graph=True)
+    with pytest.raises(NotImplementedError, match="create_graph"):
+        torch.autograd.grad(ops.embedding(torch.zeros(1, dtype=torch.int64, device="cuda"), w).sum(), [w], create_graph=True)
 
 
 def test_refusals_on_the_host():
