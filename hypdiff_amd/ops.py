@@ -106,6 +106,10 @@ _raw_stream_fn = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 _cur_device_fn = getattr(torch._C, "_cuda_getDevice", None)
 
 
+def _cur_device():
+    return _cur_device_fn() if _cur_device_fn is not None else torch.cuda.current_device()
+
+
 def raw_stream():
     if _raw_stream_fn is not None and _cur_device_fn is not None:
         return _raw_stream_fn(_cur_device_fn())
@@ -768,25 +772,36 @@ def linear_act(x, weight, bias=None, act="identity", resid=None):
     kept in the operands' type, dL/dz is rounded to it for the products, sums are in fp32 and in a fixed order (the same
     bits on every run).  The 16-bit form of the layers that linear_chain / autograd.linear_stack run in fp32
     (models/direction_diffusion.py:47-69, ddpm.py:9-27)."""
-    if x.dtype not in (torch.bfloat16, torch.float16):
-        raise TypeError(f"linear_act: operands in bfloat16 or float16, not {x.dtype}")
-    if act not in LINEAR_ACTS:
+    dt, ws, xs = x.dtype, weight.shape, x.shape
+    if dt is not torch.bfloat16 and dt is not torch.float16:
+        raise TypeError(f"linear_act: operands in bfloat16 or float16, not {dt}")
+    code = LINEAR_ACTS.get(act)
+    if code is None:
         raise ValueError(f"linear_act: act is one of {sorted(LINEAR_ACTS)}, not {act!r}")
-    if weight.dim() != 2 or weight.shape[0] < 1 or weight.shape[1] < 1:
-        raise ValueError(f"linear_act: a weight of shape (N, K), not {tuple(weight.shape)}")
-    if x.dim() < 1 or x.shape[-1] != weight.shape[1]:
-        raise ValueError(f"linear_act: x has shape {tuple(x.shape)}, the weight {tuple(weight.shape)}")
-    N = weight.shape[0]
-    if bias is not None and tuple(bias.shape) != (N,):
-        raise ValueError(f"linear_act: bias has shape {tuple(bias.shape)}, not ({N},)")
-    if resid is not None and tuple(resid.shape) != tuple(x.shape[:-1]) + (N,):
-        raise ValueError(f"linear_act: resid has shape {tuple(resid.shape)}, not {tuple(x.shape[:-1]) + (N,)}")
-    for name, t in (("weight", weight), ("bias", bias), ("resid", resid)):
-        if t is not None and t.dtype != x.dtype:
-            raise TypeError(f"linear_act: {name} is {t.dtype}, x {x.dtype}")
-    _dev(x, weight, bias, resid)
-    code = LINEAR_ACTS[act]
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, resid)):
+    if len(ws) != 2 or ws[0] < 1 or ws[1] < 1:
+        raise ValueError(f"linear_act: a weight of shape (N, K), not {tuple(ws)}")
+    if len(xs) < 1 or xs[-1] != ws[1]:
+        raise ValueError(f"linear_act: x has shape {tuple(xs)}, the weight {tuple(ws)}")
+    dev = x.get_device()
+    same = dev >= 0 and weight.get_device() == dev and dev == _cur_device()
+    grad = x.requires_grad or weight.requires_grad
+    if weight.dtype is not dt:
+        raise TypeError(f"linear_act: weight is {weight.dtype}, x {dt}")
+    if bias is not None:
+        if bias.dim() != 1 or bias.shape[0] != ws[0]:
+            raise ValueError(f"linear_act: bias has shape {tuple(bias.shape)}, not ({ws[0]},)")
+        if bias.dtype is not dt:
+            raise TypeError(f"linear_act: bias is {bias.dtype}, x {dt}")
+        same, grad = same and bias.get_device() == dev, grad or bias.requires_grad
+    if resid is not None:
+        if resid.dim() != len(xs) or resid.shape[-1] != ws[0] or resid.shape[:-1] != xs[:-1]:
+            raise ValueError(f"linear_act: resid has shape {tuple(resid.shape)}, not {tuple(xs[:-1]) + (ws[0],)}")
+        if resid.dtype is not dt:
+            raise TypeError(f"linear_act: resid is {resid.dtype}, x {dt}")
+        same, grad = same and resid.get_device() == dev, grad or resid.requires_grad
+    if not same:
+        _dev(x, weight, bias, resid)                      # says which one is elsewhere
+    if grad and torch.is_grad_enabled():
         from . import autograd as hag
         return hag.LinearAct.apply(x, weight, bias, resid, code)
     return _linear_act_fwd(x, weight, bias, resid, code, False)[0]
