@@ -8,11 +8,14 @@
 //   sort    key = token (the padding token and tokens outside the table become T, behind all others), value = row.  Up to
 //           4096 rows: one workgroup, bitonic on (key, row) in LDS.  More: least-significant-digit radix passes of at most
 //           8 bits; a workgroup counts its own digits' places from the counts of all workgroups (at most 256 of them, one
-//           read of 256 KB) and the scatter of a pass counts the next pass's digits, so p passes are p + 1 launches.
+//           read of 256 KB): two launches a pass.  (Counting the next pass's digits in the scatter, by atomics on the counts of the
+//           workgroup a row moves to, saved a launch of 3 us and cost 11: the rows of a hot token meet on one counter.)
 //   sum     the sorted rows are cut into chunks of P; a lane owns VEC columns, walks a chunk and writes a table row
 //           whenever a run ends.  A run that crosses a chunk's border leaves a partial sum there, which the next launch
 //           adds up in chunk order: a hot token (18 000 of 75 000 rows) is spread over hundreds of wavefronts.  Further
 //           workgroups of the same launch write the zeros of the table rows that no row names.
+// A width that is no multiple of VEC: the last lane takes the last VEC columns, some of them a second time, with equal results
+// (branches for its short group cost half of the time: loads that wait for each other).
 // Bound by HBM: one read of g and one write of the table's gradient (the lookup: one read of the named rows, one write).
 #include <type_traits>
 #include "hd_common.cuh"
@@ -33,31 +36,37 @@ template <typename T, int VEC, typename I>
 __global__ __launch_bounds__(256) void lookup_k(const T* __restrict__ table, long long ldt, const I* __restrict__ idx,
                                                 const T* __restrict__ add, long long lda, float scale, long long n_table,
                                                 long long rows, int dim, int log2_lanes, T* __restrict__ out) {
-    const int lanes = 1 << log2_lanes;                                        // lanes of a row (a power of two up to 256)
+    const int lanes = 1 << log2_lanes;                                        // lanes of a row (a power of two up to 64)
     const long long r = (long long)blockIdx.x * (256 >> log2_lanes) + (threadIdx.x >> log2_lanes);
     if (r >= rows) return;
     const long long t = (long long)idx[r];
     const bool inside = t >= 0 && t < n_table;                                // outside the table: a row of NaN
     const T* src = table + (inside ? t : 0) * ldt;
-    for (int c = (threadIdx.x & (lanes - 1)) * VEC; c < dim; c += lanes * VEC) {
-        if (c + VEC <= dim) {
-            const Pack<T, VEC> a = load_pack<T, VEC>(src + c);
+    const T* plus = add ? add + r * lda : nullptr;
+    T* dst = out + r * dim;
+    constexpr int U = 4;                                                      // chunks in flight
+    for (int c0 = (threadIdx.x & (lanes - 1)) * VEC; c0 < dim; c0 += U * lanes * VEC) {
+        Pack<T, VEC> a[U], b[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            int c = c0 + u * lanes * VEC;
+            c = c + VEC <= dim ? c : dim - VEC;
+            a[u] = load_pack<T, VEC>(src + c);
+            if (plus) b[u] = load_pack<T, VEC>(plus + c);                     // uniform
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            int c = c0 + u * lanes * VEC;
+            if (c >= dim) break;
+            c = c + VEC <= dim ? c : dim - VEC;
             Pack<T, VEC> o;
-            if (add) {
-                const Pack<T, VEC> b = load_pack<T, VEC>(add + r * lda + c);
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) o.v[e] = (T)(inside ? (float)b.v[e] + scale * (float)a.v[e] : __builtin_nanf(""));
-            } else {
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) o.v[e] = (T)(inside ? scale * (float)a.v[e] : __builtin_nanf(""));
+            for (int e = 0; e < VEC; ++e) {
+                float v = scale * (float)a[u].v[e];
+                if (plus) v = (float)b[u].v[e] + v;
+                o.v[e] = (T)(inside ? v : __builtin_nanf(""));
             }
-            store_pack<T, VEC>(out + r * dim + c, o);
-        } else {
-            for (int k = c; k < dim; ++k) {
-                float v = scale * (float)src[k];
-                if (add) v = (float)add[r * lda + k] + v;
-                out[r * dim + k] = (T)(inside ? v : __builtin_nanf(""));
-            }
+            store_pack<T, VEC>(dst + c, o);
         }
     }
 }
@@ -91,30 +100,31 @@ __global__ __launch_bounds__(kSortWg) void sort_small_k(const I* __restrict__ id
     }
 }
 
-// digit counts of the first pass, [workgroup][256]; clears the counts of the further passes
-template <typename I>
-__global__ __launch_bounds__(kSortWg) void radix_count_k(const I* __restrict__ idx, long long padding, unsigned n_table, unsigned n,
-                                                         unsigned per_wg, unsigned mask, unsigned* __restrict__ hist,
-                                                         unsigned more_words) {
-    __shared__ unsigned h[256];
-    if (threadIdx.x < 256) h[threadIdx.x] = 0;
+// digit counts of a pass, [workgroup][256].  FIRST: keys come from idx
+template <typename I, bool FIRST>
+__global__ __launch_bounds__(kSortWg) void radix_count_k(const I* __restrict__ idx, long long padding, unsigned n_table,
+                                                         const unsigned* __restrict__ keys, unsigned n, unsigned per_wg, int shift,
+                                                         unsigned mask, unsigned* __restrict__ hist) {
+    __shared__ unsigned h[4][256];                                            // four copies: fewer meet on a hot token's counter
+    (&h[0][0])[threadIdx.x] = 0;
     __syncthreads();
     const unsigned i0 = blockIdx.x * per_wg, i1 = n - i0 < per_wg ? n : i0 + per_wg;
-    for (unsigned i = i0 + threadIdx.x; i < i1; i += kSortWg) atomicAdd(&h[key_of(idx[i], padding, n_table) & mask], 1u);
+    for (unsigned i = i0 + threadIdx.x; i < i1; i += kSortWg) {
+        unsigned key;
+        if constexpr (FIRST) key = key_of(idx[i], padding, n_table);
+        else key = keys[i];
+        atomicAdd(&h[threadIdx.x & 3][(key >> shift) & mask], 1u);
+    }
     __syncthreads();
-    if (threadIdx.x < 256) hist[blockIdx.x * 256 + threadIdx.x] = h[threadIdx.x];
-    unsigned* more = hist + gridDim.x * 256;
-    for (unsigned i = blockIdx.x * kSortWg + threadIdx.x; i < more_words; i += gridDim.x * kSortWg) more[i] = 0;
+    if (threadIdx.x < 256) hist[blockIdx.x * 256 + threadIdx.x] = h[0][threadIdx.x] + h[1][threadIdx.x] + h[2][threadIdx.x] + h[3][threadIdx.x];
 }
 
-// One stable scatter by the digit (key >> shift) & mask.  FIRST: keys come from idx.  next: the counts of the next pass
-// ([workgroup][256], integers: the order of the additions does not matter), or NULL after the last.
+// One stable scatter by the digit (key >> shift) & mask
 template <typename I, bool FIRST>
 __global__ __launch_bounds__(kSortWg) void radix_scatter_k(const I* __restrict__ idx, long long padding, unsigned n_table,
                                                            const unsigned* __restrict__ keys_in, const unsigned* __restrict__ pos_in,
-                                                           unsigned n, unsigned per_wg, int shift, unsigned mask, int next_shift,
-                                                           unsigned next_mask, const unsigned* __restrict__ hist,
-                                                           unsigned* __restrict__ next, unsigned* __restrict__ keys_out,
+                                                           unsigned n, unsigned per_wg, int shift, unsigned mask,
+                                                           const unsigned* __restrict__ hist, unsigned* __restrict__ keys_out,
                                                            unsigned* __restrict__ pos_out) {
     __shared__ unsigned part_all[4][256], part_before[4][256], place[256], wave_count[16][256];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, digit = tid & 255, quarter = tid >> 8;
@@ -187,7 +197,6 @@ __global__ __launch_bounds__(kSortWg) void radix_scatter_k(const I* __restrict__
             const unsigned to = wave_count[wave][d] + rank;
             keys_out[to] = key;
             pos_out[to] = row;
-            if (next) atomicAdd(&next[to / per_wg * 256 + ((key >> next_shift) & next_mask)], 1u);
         }
         __syncthreads();
     }
@@ -204,28 +213,24 @@ __device__ __forceinline__ unsigned lower_bound(const unsigned* keys, unsigned n
 }
 
 template <int VEC>
-__device__ __forceinline__ void store_part(float* p, const float (&acc)[VEC], int c, int dim) {
+__device__ __forceinline__ void store_part(float* p, const float (&acc)[VEC]) {
+    Pack<float, VEC> o;
 #pragma unroll
-    for (int e = 0; e < VEC; ++e)
-        if (c + e < dim) p[c + e] = acc[e];
+    for (int e = 0; e < VEC; ++e) o.v[e] = acc[e];
+    store_pack<float, VEC>(p, o);
 }
 template <typename T, int VEC>
-__device__ __forceinline__ void store_row(T* p, const float (&acc)[VEC], float scale, int c, int dim) {
-    if (c + VEC <= dim) {
-        Pack<T, VEC> o;
+__device__ __forceinline__ void store_row(T* p, const float (&acc)[VEC], float scale) {
+    Pack<T, VEC> o;
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) o.v[e] = (T)(acc[e] * scale);
-        store_pack<T, VEC>(p + c, o);
-    } else {
-#pragma unroll
-        for (int e = 0; e < VEC; ++e)
-            if (c + e < dim) p[c + e] = (T)(acc[e] * scale);
-    }
+    for (int e = 0; e < VEC; ++e) o.v[e] = (T)(acc[e] * scale);
+    store_pack<T, VEC>(p, o);
 }
 
 // head[chunk]: the sum of the chunk's rows that continue the run of the chunk before; tail[chunk]: of the run that begins in
-// the chunk and goes on in the next.  A lane owns the columns c .. c + VEC - 1 of one chunk.
-template <typename T, int VEC>
+// the chunk and goes on in the next.  A lane owns the columns c .. c + VEC - 1 of one chunk.  ONE: a wavefront is in one chunk, so
+// that its keys and rows are scalar loads and the ends of runs scalar branches.
+template <typename T, int VEC, bool ONE>
 __global__ __launch_bounds__(256) void segment_sum_k(const T* __restrict__ g, long long ldg, const unsigned* __restrict__ keys,
                                                      const unsigned* __restrict__ pos, unsigned n, int dim, unsigned n_table,
                                                      float scale, int chunk, int log2_lanes, int tiles, unsigned sum_wgs,
@@ -245,88 +250,104 @@ __global__ __launch_bounds__(256) void segment_sum_k(const T* __restrict__ g, lo
         const float zero[VEC] = {};
         for (unsigned t = t0 + wave; t < t1; t += 4)
             if (!present[t - t0])
-                for (int c = lane * VEC; c < dim; c += 64 * VEC) store_row<T, VEC>(out + (long long)t * dim, zero, 1.f, c, dim);
+                for (int c = lane * VEC; c < dim; c += 64 * VEC)
+                    store_row<T, VEC>(out + (long long)t * dim + (c + VEC <= dim ? c : dim - VEC), zero, 1.f);
         return;
     }
-    const unsigned item = blockIdx.x * (256u >> log2_lanes) + (threadIdx.x >> log2_lanes);
+    unsigned item = blockIdx.x * (256u >> log2_lanes) + (threadIdx.x >> log2_lanes);
+    if constexpr (ONE) item = (unsigned)__builtin_amdgcn_readfirstlane((int)item);
     const unsigned ch = item / (unsigned)tiles;
-    const int c = ((int)(item - ch * tiles) * (1 << log2_lanes) + (int)(threadIdx.x & ((1 << log2_lanes) - 1))) * VEC;
+    int c = ((int)(item - ch * tiles) * (1 << log2_lanes) + (int)(threadIdx.x & ((1 << log2_lanes) - 1))) * VEC;
     const unsigned i0 = ch * chunk;
     if (i0 >= n || c >= dim) return;
+    c = c + VEC <= dim ? c : dim - VEC;
     const unsigned i1 = n - i0 < (unsigned)chunk ? n : i0 + chunk;
-    const bool whole = c + VEC <= dim;
     const unsigned after = i1 < n ? keys[i1] : ~0u;
     unsigned cur = keys[i0];
     bool cont = i0 > 0 && keys[i0 - 1] == cur;                                // the run began in an earlier chunk
     float acc[VEC] = {};
     constexpr int U = 8;                                                      // rows in flight
-    for (unsigned i = i0; i < i1; i += U) {
-        unsigned k[U], p[U];
-        Pack<T, VEC> x[U];
+    unsigned k[U], p[U];
+    auto names = [&](unsigned i) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const unsigned j = i + u < i1 ? i + u : i1 - 1;
             k[u] = i + u < i1 ? keys[j] : ~0u;
             p[u] = pos[j];
         }
+    };
+    names(i0);
+    for (unsigned i = i0; i < i1; i += U) {
+        Pack<T, VEC> x[U];
+        unsigned kk[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const T* src = g + (long long)p[u] * ldg + c;
-            if (whole) {
-                x[u] = load_pack<T, VEC>(src);
-            } else {
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) x[u].v[e] = c + e < dim ? src[e] : (T)0.f;
-            }
+            kk[u] = k[u];
+            x[u] = load_pack<T, VEC>(g + (long long)p[u] * ldg + c);
         }
+        if (i + U < i1) names(i + U);                                         // on their way while the rows are
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            if (k[u] == ~0u) break;
-            if (k[u] != cur) {                                                // the run of cur is over
-                if (cont) store_part<VEC>(head + (long long)ch * dim, acc, c, dim);
-                else if (cur < n_table) store_row<T, VEC>(out + (long long)cur * dim, acc, scale, c, dim);
+            if (kk[u] == ~0u) break;
+            if (kk[u] != cur) {                                               // the run of cur is over
+                if (cont) store_part<VEC>(head + (long long)ch * dim + c, acc);
+                else if (cur < n_table) store_row<T, VEC>(out + (long long)cur * dim + c, acc, scale);
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) acc[e] = 0.f;
-                cur = k[u];
+                cur = kk[u];
                 cont = false;
             }
 #pragma unroll
             for (int e = 0; e < VEC; ++e) acc[e] += (float)x[u].v[e];
         }
     }
-    if (cont) store_part<VEC>(head + (long long)ch * dim, acc, c, dim);
-    else if (after == cur) store_part<VEC>(tail + (long long)ch * dim, acc, c, dim);
-    else if (cur < n_table) store_row<T, VEC>(out + (long long)cur * dim, acc, scale, c, dim);
+    if (cont) store_part<VEC>(head + (long long)ch * dim + c, acc);
+    else if (after == cur) store_part<VEC>(tail + (long long)ch * dim + c, acc);
+    else if (cur < n_table) store_row<T, VEC>(out + (long long)cur * dim + c, acc, scale);
 }
 
 // Runs that cross chunks: tail of the chunk where the run begins, then the heads up to the chunk where it ends, in order;
-// four wavefronts take a quarter of the heads each.  One workgroup per (chunk, 64 columns); chunks without a tail leave at once.
-template <typename T>
+// four wavefronts take a quarter of the heads each.  One workgroup per (chunk, 64 VEC columns); chunks without a tail leave at once.
+template <typename T, int VEC>
 __global__ __launch_bounds__(256) void segment_join_k(const unsigned* __restrict__ keys, unsigned n, int dim, unsigned n_table,
                                                       float scale, int chunk, int tiles, const float* __restrict__ head,
                                                       const float* __restrict__ tail, T* __restrict__ out) {
-    __shared__ float red[4][64];
+    __shared__ float red[4][64][VEC];
     __shared__ unsigned last;
     const unsigned ch = blockIdx.x / (unsigned)tiles;
     const unsigned i0 = ch * chunk, i1 = i0 + chunk;                          // the last chunk has no tail: not launched for it
     const unsigned cur = keys[i1 - 1];
     if (cur >= n_table || keys[i1] != cur || (keys[i0] == cur && i0 > 0 && keys[i0 - 1] == cur)) return;
-    if (threadIdx.x == 0) last = (lower_bound(keys, n, cur + 1) - 1) / (unsigned)chunk;
-    __syncthreads();
+    if (i1 + chunk < n && keys[i1 + chunk] == cur) {                          // it goes on behind the next chunk: where does it end?
+        if (threadIdx.x == 0) last = (lower_bound(keys, n, cur + 1) - 1) / (unsigned)chunk;
+        __syncthreads();
+    } else {
+        if (threadIdx.x == 0) last = ch + 1;
+        __syncthreads();
+    }
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const int c = (int)(blockIdx.x - ch * tiles) * 64 + lane;
+    int c = ((int)(blockIdx.x - ch * tiles) * 64 + lane) * VEC;
+    const bool live = c < dim;
+    c = c + VEC <= dim ? c : dim - VEC;
     const unsigned heads = last - ch, per = (heads + 3) / 4;
     const unsigned a = ch + 1 + wave * per, b = a + per < last + 1 ? a + per : last + 1;
-    float acc = 0.f;
-    if (c < dim) {
-        if (wave == 0) acc = tail[(long long)ch * dim + c];
+    float acc[VEC] = {};
+    auto add = [&](const float* row) {
+        const Pack<float, VEC> x = load_pack<float, VEC>(row + c);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) acc[e] += x.v[e];
+    };
+    if (wave == 0) add(tail + (long long)ch * dim);
 #pragma unroll 8
-        for (unsigned k = a; k < b; ++k) acc += head[(long long)k * dim + c];
-    }
-    red[wave][lane] = acc;
+    for (unsigned k = a; k < b; ++k) add(head + (long long)k * dim);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) red[wave][lane][e] = acc[e];
     __syncthreads();
-    if (wave == 0 && c < dim)
-        out[(long long)cur * dim + c] = (T)((((red[0][lane] + red[1][lane]) + red[2][lane]) + red[3][lane]) * scale);
+    if (wave == 0 && live) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) acc[e] = ((red[0][lane][e] + red[1][lane][e]) + red[2][lane][e]) + red[3][lane][e];
+        store_row<T, VEC>(out + (long long)cur * dim + c, acc, scale);
+    }
 }
 
 // ---- host side ------------------------------------------------------------------------------------------------------------
@@ -382,7 +403,7 @@ Plan make_plan(int64_t rows, int64_t dim, int64_t n_table, int dt) {
     p.off_pos2 = at;
     at += small ? 0 : up(rows * 4);
     p.off_hist = at;
-    at += small ? 0 : up((int64_t)p.passes * p.sort_wgs * 256 * 4);
+    at += small ? 0 : up((int64_t)p.sort_wgs * 256 * 4);
     p.off_head = at;
     at += up(p.chunks * dim * 4);
     p.off_tail = at;
@@ -403,21 +424,19 @@ void sort_rows(const I* idx, long long padding, unsigned n_table, int64_t rows, 
     unsigned* buf_k[2] = {keys, (unsigned*)(ws + p.off_keys2)};
     unsigned* buf_p[2] = {pos, (unsigned*)(ws + p.off_pos2)};
     unsigned* hist = (unsigned*)(ws + p.off_hist);
-    const unsigned mask = (1u << p.width) - 1, words = (unsigned)p.sort_wgs * 256;
-    radix_count_k<I><<<p.sort_wgs, kSortWg, 0, st>>>(idx, padding, n_table, (unsigned)rows, (unsigned)p.per_wg, mask, hist,
-                                                     words * (p.passes - 1));
+    const unsigned mask = (1u << p.width) - 1, n = (unsigned)rows, per = (unsigned)p.per_wg;
     int to = (p.passes - 1) & 1;                                                 // so that the last pass writes buffer 0
     for (int k = 0; k < p.passes; ++k, to ^= 1) {
-        unsigned* next = k + 1 < p.passes ? hist + (size_t)(k + 1) * words : nullptr;
-        if (k == 0)
-            radix_scatter_k<I, true><<<p.sort_wgs, kSortWg, 0, st>>>(idx, padding, n_table, nullptr, nullptr, (unsigned)rows,
-                                                                     (unsigned)p.per_wg, 0, mask, p.width, mask, hist, next, buf_k[to],
-                                                                     buf_p[to]);
-        else
-            radix_scatter_k<I, false><<<p.sort_wgs, kSortWg, 0, st>>>(idx, padding, n_table, buf_k[to ^ 1], buf_p[to ^ 1],
-                                                                      (unsigned)rows, (unsigned)p.per_wg, k * p.width, mask,
-                                                                      (k + 1) * p.width, mask, hist + (size_t)k * words, next,
-                                                                      buf_k[to], buf_p[to]);
+        const int shift = k * p.width;
+        if (k == 0) {
+            radix_count_k<I, true><<<p.sort_wgs, kSortWg, 0, st>>>(idx, padding, n_table, nullptr, n, per, shift, mask, hist);
+            radix_scatter_k<I, true><<<p.sort_wgs, kSortWg, 0, st>>>(idx, padding, n_table, nullptr, nullptr, n, per, shift, mask, hist,
+                                                                     buf_k[to], buf_p[to]);
+        } else {
+            radix_count_k<I, false><<<p.sort_wgs, kSortWg, 0, st>>>(idx, padding, n_table, buf_k[to ^ 1], n, per, shift, mask, hist);
+            radix_scatter_k<I, false><<<p.sort_wgs, kSortWg, 0, st>>>(idx, padding, n_table, buf_k[to ^ 1], buf_p[to ^ 1], n, per, shift,
+                                                                      mask, hist, buf_k[to], buf_p[to]);
+        }
     }
 }
 
@@ -429,12 +448,22 @@ void sum_rows(const T* g, int64_t ldg, int64_t rows, int64_t dim, int64_t n_tabl
     const int64_t per_wg = 256 >> p.log2_lanes;
     const unsigned sum_wgs = (unsigned)((p.chunks * p.tiles + per_wg - 1) / per_wg);
     const unsigned zero_wgs = (unsigned)((n_table + kZeroRows - 1) / kZeroRows);
-    segment_sum_k<T, VEC><<<sum_wgs + zero_wgs, 256, 0, st>>>(g, ldg, keys, pos, (unsigned)rows, (int)dim, (unsigned)n_table, scale, p.chunk,
-                                                              p.log2_lanes, p.tiles, sum_wgs, out, head, tail);
+    auto go = [&](auto one) {
+        segment_sum_k<T, VEC, decltype(one)::value><<<sum_wgs + zero_wgs, 256, 0, st>>>(g, ldg, keys, pos, (unsigned)rows, (int)dim,
+                                                                                       (unsigned)n_table, scale, p.chunk, p.log2_lanes,
+                                                                                       p.tiles, sum_wgs, out, head, tail);
+    };
+    if (p.log2_lanes == 6) go(std::true_type{});
+    else go(std::false_type{});
     if (p.chunks > 1) {
-        const int tiles = (int)((dim + 63) / 64);
-        segment_join_k<T><<<(unsigned)((p.chunks - 1) * tiles), 256, 0, st>>>(keys, (unsigned)rows, (int)dim, (unsigned)n_table, scale,
-                                                                              p.chunk, tiles, head, tail, out);
+        auto join = [&](auto vec) {
+            constexpr int V = decltype(vec)::value;
+            const int tiles = (int)((dim + 64 * V - 1) / (64 * V));
+            segment_join_k<T, V><<<(unsigned)((p.chunks - 1) * tiles), 256, 0, st>>>(keys, (unsigned)rows, (int)dim, (unsigned)n_table, scale,
+                                                                                     p.chunk, tiles, head, tail, out);
+        };
+        if (dim >= 4) join(std::integral_constant<int, 4>{});
+        else join(std::integral_constant<int, 1>{});
     }
 }
 
@@ -455,7 +484,7 @@ void lookup_any(const T* table, int64_t ldt, const I* idx, const T* add, int64_t
     constexpr int MOST = 16 / sizeof(T);
     const int vec = pick_vec(dim, MOST);
     const int64_t used = (dim + vec - 1) / vec;
-    const int l2 = used >= 256 ? 8 : ceil_log2(used);
+    const int l2 = used >= 64 ? 6 : ceil_log2(used);
     const unsigned wgs = (unsigned)((rows + (256 >> l2) - 1) / (256 >> l2));
     auto go = [&](auto tag) {
         constexpr int VEC = decltype(tag)::value;
@@ -514,7 +543,7 @@ extern "C" int hd_embedding_sum(const void* g, int64_t ldg, const void* idx, int
     const Plan p = make_plan(rows, dim, T, dtype);
     HD_REQUIRE(workspace_bytes >= p.bytes, "hd_embedding_sum: workspace of %lld bytes required, got %lld", (long long)p.bytes,
                (long long)workspace_bytes);
-    HD_REQUIRE(p.chunks * ((dim + 63) / 64) < (1LL << 31) && p.chunks * p.tiles + T / kZeroRows < (1LL << 31) - 256,
+    HD_REQUIRE(p.chunks * ((dim + 255) / 256) < (1LL << 31) && p.chunks * p.tiles + T / kZeroRows < (1LL << 31) - 256,
                "hd_embedding_sum: too many workgroups");
     hipStream_t s = (hipStream_t)st;
     unsigned char* ws = (unsigned char*)workspace;
