@@ -384,7 +384,7 @@ Plan make_plan(int64_t rows, int64_t dim, int64_t n_table, int dt) {
     // short enough that a small batch still fills the chip
     const int64_t lanes_per_row = (int64_t)p.tiles << p.log2_lanes;
     p.chunk = 8;
-    while (p.chunk < 64 && rows * lanes_per_row / (2 * p.chunk) >= 4096 * 64) p.chunk *= 2;
+    while (p.chunk < 64 && rows * lanes_per_row / (2 * p.chunk) >= 2048 * 64) p.chunk *= 2;
     p.chunks = (rows + p.chunk - 1) / p.chunk;
     const int bits = ceil_log2(n_table + 1) > 0 ? ceil_log2(n_table + 1) : 1;     // keys are 0 .. n_table
     p.passes = (bits + 7) / 8;
