@@ -155,7 +155,7 @@ SIGNATURES = {
     "hd_transpose_multi_f32": [POINTER(HdTransposeJob), c_int, P],
     "hd_adam_step_f32": [POINTER(HdAdamJob), c_int, P, P, P, c_double, c_double, c_double, c_double, I64, P, P],
     "hd_linear_act_fwd": [P, I64, P, I64, P, P, I64, c_int, I64, I64, I64, c_int, P, P, P],
-    "hd_linear_act_bwd": [P, I64, P, P, I64, P, I64, c_int, I64, I64, I64, c_int, P, P, P, P, I64, P],
+    "hd_linear_act_bwd": [P, I64, P, P, I64, P, I64, c_int, I64, I64, I64, c_int, P, I64, P, P, P, P, I64, P],
     "hd_adamw_step": [P, c_int, c_int, c_int, P, P, P, P, P, I64, c_double, c_double, c_double, c_double, c_double, I64, P,
                       I64, P],
     "hd_colsum_f32": [P, P, I64, I64, I64, P, P],

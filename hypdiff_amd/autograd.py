@@ -507,13 +507,14 @@ def _first_order(what):
 
 class LinearAct(torch.autograd.Function):
     """resid + act(x W^T + b) on 16-bit operands (ops.linear_act).  The pre-activation is kept in 16 bits (nothing for the
-    identity); backward: hd_linear_act_bwd, and the incoming gradient itself for resid."""
+    identity); backward: hd_linear_act_bwd, and the incoming gradient itself for resid.  skip: resid is x (given as None here);
+    the incoming gradient is added to dx where dx is written."""
 
     @staticmethod
-    def forward(ctx, x, w, b, resid, act):
-        y, z, x2, ldx, w2, ldw = ops._linear_act_fwd(x, w, b, resid, act, act != 0)
+    def forward(ctx, x, w, b, resid, act, skip):
+        y, z, x2, ldx, w2, ldw = ops._linear_act_fwd(x, w, b, x if skip else resid, act, act != 0)
         ctx.save_for_backward(x2, w2, z)
-        ctx.args = (ldx, ldw, act, x.shape)
+        ctx.args = (ldx, ldw, act, x.shape, skip)
         return y
 
     @staticmethod
@@ -523,7 +524,7 @@ class LinearAct(torch.autograd.Function):
         x2, w2, z = ctx.saved_tensors
         dx, dw, db = ops._linear_act_bwd(g, z, x2, w2, *ctx.args, need[0], need[1], need[2]) \
             if need[0] or need[1] or need[2] else (None, None, None)
-        return dx, dw, db, g if need[3] else None, None
+        return dx, dw, db, g if need[3] else None, None, None
 
 
 class Embedding(torch.autograd.Function):

@@ -716,7 +716,7 @@ int linear_fwd(const Prod& g, bool direct, hipStream_t s) {
 
 template <typename T>
 int linear_bwd(const T* g, int64_t ldg, const T* z, const T* x, int64_t ldx, const T* w, int64_t ldw, int64_t M, int64_t N, int64_t K,
-               int act, T* dx, T* dw, T* db, const BwdPlan& p, unsigned char* ws, hipStream_t s) {
+               int act, const T* dx_add, int64_t ld_add, T* dx, T* dw, T* db, const BwdPlan& p, unsigned char* ws, hipStream_t s) {
     const T* dz = g;
     long long lddz = ldg;
     T* wt = (T*)(ws + p.off_wt);
@@ -734,7 +734,9 @@ int linear_bwd(const T* g, int64_t ldg, const T* z, const T* x, int64_t ldx, con
     q.A = dz; q.lda = lddz;
     if (dx) {                                                                 // (M, K) = dz (M, N) . W^T (K, N), zeros up to whole chunks
         q.B = wt; q.ldb = p.lddz; q.M = (int)M; q.N = (int)K; q.K = (int)((N + 7) / 8 * 8); q.C = dx;
+        q.resid = dx_add; q.ldr = ld_add;
         launch_product<T>(q, true, s);
+        q.resid = nullptr;
     }
     if (dw) {                                                                 // (N, K) = dz^T (N, M) . x (M, K)
         q.B = x; q.ldb = ldx; q.M = (int)N; q.N = (int)K; q.K = (int)M; q.C = ws + p.off_ws;
@@ -777,15 +779,16 @@ extern "C" int64_t hd_linear_act_bwd_workspace_bytes(int64_t M, int64_t N, int64
 }
 
 extern "C" int hd_linear_act_bwd(const void* g, int64_t ldg, const void* z, const void* x, int64_t ldx, const void* w, int64_t ldw,
-                                 int dtype, int64_t M, int64_t N, int64_t K, int act, void* dx, void* dw, void* db, void* workspace,
-                                 int64_t workspace_bytes, void* st) {
+                                 int dtype, int64_t M, int64_t N, int64_t K, int act, const void* dx_add, int64_t ld_add, void* dx,
+                                 void* dw, void* db, void* workspace, int64_t workspace_bytes, void* st) {
     HD_LINEAR_SHAPE("hd_linear_act_bwd");
     HD_REQUIRE(ldg >= N, "hd_linear_act_bwd: row pitch below the width");
     HD_REQUIRE(workspace && (uintptr_t)workspace % 16 == 0, "hd_linear_act_bwd: null or misaligned workspace");
+    HD_REQUIRE(!dx_add || (dx && ld_add >= 0), "hd_linear_act_bwd: dx_add without dx, or a negative pitch");
     HD_REQUIRE(M == 0 || (g && (z || act == HD_ACT_IDENTITY)), "hd_linear_act_bwd: null pointer");
     HD_REQUIRE(!(dx && M > 0) || w, "hd_linear_act_bwd: dx needs w");
     HD_REQUIRE(!(dw && M > 0) || x, "hd_linear_act_bwd: dw needs x");
-    HD_REQUIRE((((uintptr_t)g | (uintptr_t)z | (uintptr_t)x | (uintptr_t)w | (uintptr_t)dx | (uintptr_t)dw | (uintptr_t)db) & 1) == 0,
+    HD_REQUIRE((((uintptr_t)g | (uintptr_t)z | (uintptr_t)x | (uintptr_t)w | (uintptr_t)dx | (uintptr_t)dw | (uintptr_t)db | (uintptr_t)dx_add) & 1) == 0,
                "hd_linear_act_bwd: pointer not aligned to the element");
     HD_REQUIRE(M > 0, "hd_linear_act_bwd: no rows (the gradients are zeros; fill them)");
     const BwdPlan p = bwd_plan(M, N, K);
@@ -796,8 +799,8 @@ extern "C" int hd_linear_act_bwd(const void* g, int64_t ldg, const void* z, cons
     unsigned char* ws = (unsigned char*)workspace;
     hipStream_t s = (hipStream_t)st;
     if (dtype == HD_DT_BF16)
-        return linear_bwd<bf16>((const bf16*)g, ldg, (const bf16*)z, (const bf16*)x, ldx, (const bf16*)w, ldw, M, N, K, act, (bf16*)dx,
+        return linear_bwd<bf16>((const bf16*)g, ldg, (const bf16*)z, (const bf16*)x, ldx, (const bf16*)w, ldw, M, N, K, act, (const bf16*)dx_add, ld_add, (bf16*)dx,
                                 (bf16*)dw, (bf16*)db, p, ws, s);
-    return linear_bwd<f16>((const f16*)g, ldg, (const f16*)z, (const f16*)x, ldx, (const f16*)w, ldw, M, N, K, act, (f16*)dx, (f16*)dw,
-                           (f16*)db, p, ws, s);
+    return linear_bwd<f16>((const f16*)g, ldg, (const f16*)z, (const f16*)x, ldx, (const f16*)w, ldw, M, N, K, act, (const f16*)dx_add,
+                           ld_add, (f16*)dx, (f16*)dw, (f16*)db, p, ws, s);
 }

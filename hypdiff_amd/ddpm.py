@@ -4,7 +4,9 @@
 Same constructors and state_dict keys (`backbone.linear_model1.layers.N.*`,
 `backbone.embedding_layer.weight`, `backbone.linear_model2.layers.N.*`).  Every Linear
 is one MFMA GEMM launch with its bias, exact-erf GELU and residual add fused into the
-accumulator write-out (ddpm.py:17-27); the time embedding is added in place.
+accumulator write-out (ddpm.py:17-27); the time embedding is added in place.  With weights in
+bf16 or fp16 (`model.bfloat16()`) the denoiser runs and trains on the 16-bit operators
+(ops.linear_act, ops.embedding; optim.AdamW keeps fp32 masters).
 """
 import numpy as np
 import torch
@@ -26,6 +28,8 @@ class MLP(nn.Module):
 
     def forward(self, x):
         ops._dev(x)
+        if self.layers[0].weight.dtype in ops.HALF_TYPES:
+            return self._forward_half(x)
         x = x.to(torch.float32).contiguous()
         last = len(self.layers) - 1
         if hag.chain_wants_grad(self.chain(), x):
@@ -38,6 +42,15 @@ class MLP(nn.Module):
         if ops.chain_small_ok(x, chain):                 # small batch: the whole stack in one launch
             return ops.linear_chain_small(x, chain)
         return ops.linear_chain(x, chain)
+
+    def _forward_half(self, x):
+        """the stack on bf16 / fp16 weights (module.bfloat16() / module.half()), inference and training: one fused launch a
+        layer, activations in the weights' type"""
+        first, last = self.layers[0], self.layers[-1]
+        h = ops.linear_act(x.to(first.weight.dtype), first.weight, first.bias, act="gelu")
+        for layer in self.layers[1:-1]:
+            h = ops.linear_act(h, layer.weight, layer.bias, act="gelu", resid=h)
+        return ops.linear_act(h, last.weight, last.bias)
 
     def chain(self):
         """gelu(layer(x)) first, x0 + gelu(layer(x0)) in between, plain layer last (ddpm.py:17-27)"""
@@ -57,6 +70,11 @@ class Backbone(nn.Module):
 
     def forward(self, x, idx):
         ops._dev(x)
+        if self.embedding_layer.weight.dtype in ops.HALF_TYPES:
+            # bf16 / fp16 weights: the result comes back in x's type (the noising and the sampler around it stay in fp32)
+            h = self.linear_model1(x)
+            h = ops.embedding(idx.to(device=x.device, dtype=torch.int64), self.embedding_layer.weight, add=h)
+            return self.linear_model2(h).to(x.dtype)
         c1, c2 = self.linear_model1.chain(), self.linear_model2.chain()
         if not hag.chain_wants_grad(c1 + c2, x, self.embedding_layer.weight):
             xf = x.to(torch.float32)

@@ -74,7 +74,7 @@ def allreduce_moments(m, group=None):
 
 
 class GradBucket:
-    """All gradients of a module as ONE flat fp32 buffer (2.8 M elements for the mlp denoiser at
+    """All gradients of a module as ONE flat buffer in fp32 -- or in bf16 / fp16 where all parameters are -- (2.8 M elements for the mlp denoiser at
     D=512 ~ 11 MB; 6.4 M ~ 25 MB for ddpm.Backbone).
 
     The buffer is reduced in a few large chunks rather than per parameter -- xGMI links are
@@ -87,7 +87,9 @@ class GradBucket:
         self.params = [p for p in params if p.requires_grad]
         n = sum(p.numel() for p in self.params)
         dev = self.params[0].device if self.params else "cpu"
-        self.flat = torch.zeros(n, dtype=torch.float32, device=dev)
+        types = {p.dtype for p in self.params}
+        dtype = types.pop() if types in ({torch.bfloat16}, {torch.float16}) else torch.float32
+        self.flat = torch.zeros(n, dtype=dtype, device=dev)
         self.offsets = {}
         off = 0
         for p in self.params:
@@ -98,7 +100,7 @@ class GradBucket:
         # which backward produces gradients), closed once they hold chunk_bytes
         self.chunks, hi, acc = [], n, 0
         for p in reversed(self.params):
-            acc += p.numel() * 4
+            acc += p.numel() * self.flat.element_size()
             lo = self.offsets[id(p)][0]
             if acc >= chunk_bytes:
                 self.chunks.append((lo, hi))
@@ -245,7 +247,8 @@ class DataParallelTrainer:
     into views of it).  With `overlap` (default) the bucket leaves in >= 4 MB chunks over RCCL while
     backward is still running -- 3 chunks for the mlp at D=512 (11 MB), 6 for ddpm.Backbone (25 MB);
     otherwise as ONE all-reduce after backward.  The optimizer is Adam on every rank (BucketAdam: one launch over the
-    bucket; torch.optim.Adam for host tensors or when passed in) -- identical updates: weights never need a broadcast
+    bucket; optim.AdamW without decay and with fp32 masters for 16-bit parameters; torch.optim.Adam for host tensors; or the
+    one passed in) -- identical updates: weights never need a broadcast
     after the first."""
 
     def __init__(self, module, lr=1e-3, group=None, optimizer=None, broadcast=True, overlap=True):
@@ -254,7 +257,11 @@ class DataParallelTrainer:
         if optimizer is not None:
             self.opt = optimizer
         elif self.bucket.params and all(p.is_cuda for p in self.bucket.params):
-            self.opt = BucketAdam(self.bucket, lr=lr)
+            if self.bucket.flat.dtype == torch.float32:
+                self.opt = BucketAdam(self.bucket, lr=lr)
+            else:                                 # 16-bit parameters: the same update on fp32 masters
+                from . import optim
+                self.opt = optim.AdamW(self.bucket.params, lr=lr, weight_decay=0.0, master_weights=True)
         else:                                     # host tensors (the gloo tests of the trainer's logic)
             self.opt = torch.optim.Adam(self.bucket.params, lr=lr)
         if broadcast and _collective(group):
@@ -292,7 +299,7 @@ class DataParallelTrainer:
         launches of a few microseconds: 2.5 ms issued one by one, 1.3 ms of kernels).  Requirements: loss_fn reads
         the same device tensors on every call, draws its random numbers on the device (torch's CUDA generator is
         graph-safe; ddpm.Model does that while a capture is running), never reads anything back to the host; the
-        optimizer is BucketAdam (its step count lives on the device).  With more than one rank (backend nccl = RCCL) the
+        optimizer is BucketAdam or optim.AdamW (their step counts live on the device).  With more than one rank (backend nccl = RCCL) the
         chunked gradient all-reduces are recorded into the graph as well -- they are stream operations -- so the graphed
         step survives data parallelism (every rank must capture and replay in lockstep).
         `warmup` eager steps run first on a side stream (allocations, caches).  The parameters' versions are bumped
@@ -301,8 +308,9 @@ class DataParallelTrainer:
         if coll and dist.get_backend(self.group) != "nccl":
             raise NotImplementedError("DataParallelTrainer.capture with more than one rank needs the nccl (RCCL) backend: "
                                       "its collectives are stream operations and can be recorded into the graph")
-        if not isinstance(self.opt, BucketAdam):
-            raise TypeError("DataParallelTrainer.capture needs the BucketAdam optimizer (device-side step count)")
+        from . import optim
+        if not isinstance(self.opt, (BucketAdam, optim.AdamW)):
+            raise TypeError("DataParallelTrainer.capture needs the BucketAdam optimizer or optim.AdamW (device-side step count)")
         side = torch.cuda.Stream()
         side.wait_stream(torch.cuda.current_stream())
         with torch.cuda.stream(side):
@@ -319,8 +327,11 @@ class DataParallelTrainer:
 
         def replay():
             graph.replay()
-            self.opt.t += 1
-            torch.autograd.graph.increment_version(params)
+            if isinstance(self.opt, BucketAdam):
+                self.opt.t += 1
+                torch.autograd.graph.increment_version(params)
+            else:
+                self.opt.replayed()
             return loss
         replay.graph = graph
         return replay

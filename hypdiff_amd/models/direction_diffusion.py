@@ -165,7 +165,8 @@ class mlp(nn.Module):
                  (self.fc3.weight, self.fc3.bias, 1), (self.fc4.weight, self.fc4.bias, 1),
                  (self.fc5.weight, self.fc5.bias, 0)]
         fmt = ops.GEMM_MODE if ops.GEMM_MODE in ops.ROW_PACK_MAX_DIM else None
-        if fmt and d + 1 <= ops.ROW_PACK_MAX_DIM[fmt] and n > 0 and not hag.chain_wants_grad(chain):
+        half = self.fc1.weight.dtype in ops.HALF_TYPES
+        if fmt and not half and d + 1 <= ops.ROW_PACK_MAX_DIM[fmt] and n > 0 and not hag.chain_wants_grad(chain):
             # inference: the concat goes straight into the limb image of the first GEMM's operand
             img = ops.limb_empty(n, d + 1, x.device, fmt, zero_amax=False)
             if fmt == "f16x2":
@@ -183,6 +184,13 @@ class mlp(nn.Module):
     def forward_packed(self, h, d):
         """the stack on an already packed input: h = [x.float(), t, 0 ...] rows of pitch (d + 1) rounded up to 4"""
         ld = h.shape[1]
+        if self.fc1.weight.dtype in ops.HALF_TYPES:
+            # bf16 / fp16 weights, inference and training: one fused launch a layer; the result in fp32 like the other paths
+            # (t enters in the weights' type: bf16 holds whole steps up to 256 exactly, fp16 up to 2048)
+            y = h[:, : d + 1].to(self.fc1.weight.dtype)
+            for fc in (self.fc1, self.fc2, self.fc3, self.fc4):
+                y = ops.linear_act(y, fc.weight, fc.bias, act="gelu")
+            return ops.linear_act(y, self.fc5.weight, self.fc5.bias).to(torch.float32)
         chain = [(self.fc1.weight, self.fc1.bias, 1), (self.fc2.weight, self.fc2.bias, 1),
                  (self.fc3.weight, self.fc3.bias, 1), (self.fc4.weight, self.fc4.bias, 1),
                  (self.fc5.weight, self.fc5.bias, 0)]

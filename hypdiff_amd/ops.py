@@ -760,6 +760,7 @@ def linear_chain_small(x, layers, emb_after=None, emb=None, emb_idx=None):
 
 
 # ---- Linear layers on 16-bit operands (csrc/gemm_half.hip) ---------------------------------------------------
+HALF_TYPES = (torch.bfloat16, torch.float16)
 LINEAR_ACTS = {"identity": 0, "relu": 1, "gelu": 6}
 
 
@@ -803,7 +804,8 @@ def linear_act(x, weight, bias=None, act="identity", resid=None):
         _dev(x, weight, bias, resid)                      # says which one is elsewhere
     if grad and torch.is_grad_enabled():
         from . import autograd as hag
-        return hag.LinearAct.apply(x, weight, bias, resid, code)
+        skip = resid is x                                 # x's two gradients leave as one
+        return hag.LinearAct.apply(x, weight, bias, None if skip else resid, code, skip)
     return _linear_act_fwd(x, weight, bias, resid, code, False)[0]
 
 
@@ -835,7 +837,7 @@ def _linear_act_fwd(x, w, b, resid, act, want_z):
     return y, z, x2, ldx, w2, ldw
 
 
-def _linear_act_bwd(g, z, x2, w2, ldx, ldw, act, x_shape, need_x, need_w, need_b):
+def _linear_act_bwd(g, z, x2, w2, ldx, ldw, act, x_shape, skip, need_x, need_w, need_b):
     _dev(g, x2, w2)
     g2, ldg = _matrix(g)
     M, (N, K) = x2.shape[0], w2.shape
@@ -848,7 +850,7 @@ def _linear_act_bwd(g, z, x2, w2, ldx, ldw, act, x_shape, need_x, need_w, need_b
         nbytes = _lib.load().hd_linear_act_bwd_workspace_bytes(M, N, K, act)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
         _lib.call("hd_linear_act_bwd", g2.data_ptr(), ldg, _p(z), x2.data_ptr(), ldx, w2.data_ptr(), ldw, DT_CODES[dt], M, N, K, act,
-                  _p(dx), _p(dw), _p(db), ws.data_ptr(), nbytes, raw_stream())
+                  g2.data_ptr() if skip and need_x else None, ldg, _p(dx), _p(dw), _p(db), ws.data_ptr(), nbytes, raw_stream())
     return dx, dw, db
 
 

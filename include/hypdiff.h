@@ -455,13 +455,15 @@ int hd_adam_step_f32(const hd_adam_job* jobs, int n_jobs, const void* grad_flat,
 int hd_linear_act_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, const void* resid, int64_t ldr,
                       int dtype, int64_t M, int64_t N, int64_t K, int act, void* y, void* z, void* stream);
 /* Its gradients from g = dL/dy (M, N) with row pitch ldg:  dz = g * act'(z);  dx (M, K) = dz W,  dw (N, K) = dz^T x,
- * db (N) = colsum(dz); each contiguous, of the operands' type, or NULL.  z may be NULL for HD_ACT_IDENTITY.  M >= 1.
+ * db (N) = colsum(dz); each contiguous, of the operands' type, or NULL.  dx_add (M, K) with
+ * row pitch ld_add, or NULL, is added to dx before its rounding (the gradient that reaches x past the layer, as a skip
+ * connection's does).  z may be NULL for HD_ACT_IDENTITY.  M >= 1.
  * workspace: hd_linear_act_bwd_workspace_bytes bytes, 16-byte aligned, contents arbitrary, not shared between calls in
  * flight.  No atomics: the same bits on every call. */
 int64_t hd_linear_act_bwd_workspace_bytes(int64_t M, int64_t N, int64_t K, int act);
 int hd_linear_act_bwd(const void* g, int64_t ldg, const void* z, const void* x, int64_t ldx, const void* w, int64_t ldw, int dtype,
-                      int64_t M, int64_t N, int64_t K, int act, void* dx, void* dw, void* db, void* workspace,
-                      int64_t workspace_bytes, void* stream);
+                      int64_t M, int64_t N, int64_t K, int act, const void* dx_add, int64_t ld_add, void* dx, void* dw, void* db,
+                      void* workspace, int64_t workspace_bytes, void* stream);
 /* One step of AdamW (decoupled weight decay) over up to hd_adamw_max_jobs() parameter tensors in ONE launch:
  *   m = b1 m + (1-b1) g;  v = b2 v + (1-b2) g^2;  p = p (1 - lr wd) - lr/(1-b1^t) * m / (sqrt(v)/sqrt(1-b2^t) + eps)   (fp32)
  * Job i: `count` elements of type `dtype` (HD_DT_*) at param / grad, contiguous, aligned to the element; its state is the

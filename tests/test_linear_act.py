@@ -163,6 +163,30 @@ def test_transposed_and_strided_operands():
 
 
 @gpu
+@pytest.mark.parametrize("M,N", [(40, 72), (300, 136), (5000, 264), (20000, 520), (130, 33)])
+def test_skip_connection(M, N):
+    """resid is x: the skip's gradient is added to dx in fp32, before its one rounding"""
+    from hypdiff_amd import ops
+    gen = _gen(M)
+    x = torch.randn(M, N, device="cuda", generator=gen).bfloat16().requires_grad_(True)
+    w = (torch.randn(N, N, device="cuda", generator=gen) / math.sqrt(N)).bfloat16().requires_grad_(True)
+    g = torch.randn(M, N, device="cuda", generator=gen).bfloat16()
+    y = ops.linear_act(x, w, act="gelu", resid=x)
+    dx, dw = torch.autograd.grad(y, [x, w], g)
+    xd, wd, gd = x.detach().double(), w.detach().double(), g.double()
+    want = _reference(xd, wd, None, xd, gd, "gelu", torch.bfloat16)
+    _check(y, *want["y"], "y")
+    _check(dw, *want["dw"], "dw")
+    v, e = want["dx"]
+    h = HALF[torch.bfloat16]
+    _check(dx, v + gd, e - h * v.abs() + (h + 2 * U) * (v + gd).abs(), "dx")
+    only = torch.autograd.grad(ops.linear_act(x, w.detach(), act="relu", resid=x), [x], g)[0]
+    apart = x.detach().requires_grad_(True)
+    other = torch.autograd.grad(ops.linear_act(apart, w.detach(), act="relu", resid=x.detach()), [apart], g)[0]
+    assert float((only.double() - other.double() - gd).abs().max()) <= 2 * h * float((other.double().abs() + gd.abs()).max())
+
+
+@gpu
 def test_no_rows():
     from hypdiff_amd import ops
     x = torch.zeros(0, 24, device="cuda", dtype=torch.bfloat16, requires_grad=True)
@@ -303,9 +327,9 @@ def test_refusals_of_the_entry_points():
     def fwd(x=256, ldx=16, w=256, ldw=16, bias=None, resid=None, ldr=0, dt=1, M=4, N=8, K=16, act=0, y=256, z=None):
         _lib.call("hd_linear_act_fwd", x, ldx, w, ldw, bias, resid, ldr, dt, M, N, K, act, y, z, None)
 
-    def bwd(g=256, ldg=8, z=256, x=256, ldx=16, w=256, ldw=16, dt=1, M=4, N=8, K=16, act=6, dx=256, dw=256, db=256, ws=256,
-            nbytes=1 << 30):
-        _lib.call("hd_linear_act_bwd", g, ldg, z, x, ldx, w, ldw, dt, M, N, K, act, dx, dw, db, ws, nbytes, None)
+    def bwd(g=256, ldg=8, z=256, x=256, ldx=16, w=256, ldw=16, dt=1, M=4, N=8, K=16, act=6, add=None, dx=256, dw=256, db=256,
+            ws=256, nbytes=1 << 30):
+        _lib.call("hd_linear_act_bwd", g, ldg, z, x, ldx, w, ldw, dt, M, N, K, act, add, 16, dx, dw, db, ws, nbytes, None)
     for fn in (fwd, bwd):
         for bad, what in ((dict(dt=0), "element type"), (dict(act=2), "activation"), (dict(M=-1), "shape"), (dict(N=0), "shape"),
                           (dict(K=0), "shape"), (dict(M=1 << 30), "shape"), (dict(ldx=15), "pitch"), (dict(ldw=15), "pitch"),
@@ -313,7 +337,7 @@ def test_refusals_of_the_entry_points():
             with pytest.raises(RuntimeError, match=what):
                 fn(**bad)
     for bad, what in ((dict(ws=None), "workspace"), (dict(nbytes=16), "workspace of"), (dict(M=0), "no rows"), (dict(z=None), "null"),
-                      (dict(ldg=7), "pitch"), (dict(w=None), "needs")):
+                      (dict(ldg=7), "pitch"), (dict(w=None), "needs"), (dict(add=256, dx=None), "dx_add"), (dict(add=257), "aligned")):
         with pytest.raises(RuntimeError, match=what):
             bwd(**bad)
     assert _lib.load().hd_linear_act_bwd_workspace_bytes(1 << 30, 8, 8, 6) == 0
