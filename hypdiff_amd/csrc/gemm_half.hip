@@ -55,6 +55,11 @@ template <> __device__ __forceinline__ f32x4 mfma<f16>(uint4 a, uint4 b, f32x4 c
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
+// Loads through a pointer that may be the zero page: named as global memory, or the compiler takes them for flat loads, which
+// the waits for LDS reads then wait for too
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef u32x4 u32x4_any __attribute__((aligned(2)));
+__device__ __forceinline__ u32x4 global16(const void* p) { return *(const __attribute__((address_space(1))) u32x4_any*)p; }
 __device__ __forceinline__ void dma16(const void* g, char* l) {              // the hardware adds 16 * lane to the wavefront's l
     __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)g, (__attribute__((address_space(3))) void*)l, 16, 0, 0);
 }
@@ -94,19 +99,36 @@ struct Slab {
     }
 };
 
+__device__ __forceinline__ u32x4 shift_out(u32x4 v, int n) {                  // drops the first n of 8 elements, zeros behind; 0 <= n < 8
+    unsigned long long lo = ((unsigned long long)v[1] << 32) | v[0], hi = ((unsigned long long)v[3] << 32) | v[2];
+    if (n >= 4) { lo = hi; hi = 0; }
+    const int b = 16 * (n & 3);
+    lo = (lo >> b) | (b ? hi << (64 - b) : 0ull);
+    hi >>= b;
+    return u32x4{(unsigned)lo, (unsigned)(lo >> 32), (unsigned)hi, (unsigned)(hi >> 32)};
+}
+
 // What a workgroup stages of one operand: chunk q (0 .. kChunks - 1) of every slab.  DEAL > 0: the rows of a wavefront's DEAL rows
 // lie in LDS in the order in which the fragments take them (fragment f, row r16 = row r16 * DEAL / 16 + f).
+//
+// Without DIRECT a chunk may start anywhere and the last one of a row (of 8 elements at least) may be short: then the row's last 8
+// elements are loaded and shifted into place on the way to LDS.  No lane branches around a load (a branch per chunk kept the
+// loads from being in flight together: dW of 7850 x 800 x 513 28 us against 21).
 template <typename T, int MN, int BK, bool TR, bool DIRECT, int DEAL>
 struct Stager {
     using L = Slab<MN, BK, TR>;
     static constexpr int kPer = L::kChunks / 256;                             // chunks of a thread
     static_assert(L::kChunks % 256 == 0, "whole rounds");
+    // k fast: a thread's chunks lie in rows 256 / kRowChunks apart, at one position and, as swz() repeats by then, of one k
+    static_assert(TR || (256 % L::kRowChunks == 0 && 256 / L::kRowChunks % 16 == 0), "one k for all chunks of a thread");
+    static constexpr int kKs = TR ? kPer : 1;
     const T* p[kPer];                                                         // the chunk of the slab at hand
-    int k[kPer];                                                              // its first k (k fast) or its k (k slow)
-    int ok[kPer];                                                             // registers path, k slow: elements inside the matrix
-    uint4 reg[DIRECT ? 1 : kPer];
+    int k[kKs];                                                               // its first k (k fast) or its k (k slow)
+    int off[!DIRECT && TR ? kPer : 1];                                        // elements that its load starts early
+    u32x4 reg[DIRECT ? 1 : kPer];
     long long step;
     int k_end;
+    bool edge;                                                                // uniform: some chunk of the slab at hand is short
 
     static __device__ __forceinline__ int row_of(int r) {
         if constexpr (DEAL == 0) return r;
@@ -115,52 +137,63 @@ struct Stager {
     __device__ __forceinline__ void init(const T* base, long long ld, int mn0, int mn_end, int k0, int k_end_, int tid) {
         k_end = k_end_;
         step = TR ? (long long)BK * ld : BK;
+        edge = TR && mn0 + MN > mn_end;
 #pragma unroll
         for (int q = 0; q < kPer; ++q) {
             const int at = q * 256 + tid, r = at / L::kRowChunks, c = (at % L::kRowChunks) ^ L::swz(r);
             if constexpr (TR) {
                 k[q] = k0 + r;
                 int col = mn0 + c * 8;
-                ok[q] = mn_end - col;
-                if (ok[q] <= 0) { col = 0; ok[q] = 0; }                       // beyond the matrix: any column
+                if (col >= mn_end) col = 0;                                   // beyond the matrix: any column
+                if constexpr (!DIRECT) {
+                    off[q] = col + 8 > mn_end ? col + 8 - mn_end : 0;
+                    col -= off[q];
+                }
                 p[q] = base + (long long)k[q] * ld + col;
             } else {
-                k[q] = k0 + c * 8;
+                if (q == 0) k[0] = k0 + c * 8;
                 int row = mn0 + row_of(r);
                 if (row >= mn_end) row = mn_end - 1;                          // beyond the matrix: any row
-                ok[q] = 0;
-                p[q] = base + (long long)row * ld + k[q];
+                p[q] = base + (long long)row * ld + k[0];
             }
         }
     }
     __device__ __forceinline__ void advance() {
 #pragma unroll
-        for (int q = 0; q < kPer; ++q) { p[q] += step; k[q] += BK; }
+        for (int q = 0; q < kPer; ++q) p[q] += step;
+#pragma unroll
+        for (int q = 0; q < kKs; ++q) k[q] += BK;
     }
-    // DIRECT: the slab at hand goes to LDS (in flight); otherwise into registers, and store() brings it to LDS
-    __device__ __forceinline__ void load(char* lds, int wave) {
+    // DIRECT: the slab at hand (from k_slab on) goes to LDS, in flight; otherwise into registers, and store() brings it to LDS
+    __device__ __forceinline__ void load(char* lds, int wave, int k_slab) {
+        if constexpr (DIRECT) {
 #pragma unroll
-        for (int q = 0; q < kPer; ++q) {
-            if constexpr (DIRECT) {
-                const void* src = k[q] < k_end ? (const void*)p[q] : (const void*)zero_page;   // whole chunks (k_end % 8 == 0, or a k row)
+            for (int q = 0; q < kPer; ++q) {
+                const void* src = k[TR ? q : 0] < k_end ? (const void*)p[q] : (const void*)zero_page;   // whole chunks, or a k row
                 dma16(src, lds + (q * 256 + wave * 64) * 16);
-            } else {
-                Pack<T, 8> v;
-                const int n = TR ? (k[q] < k_end ? ok[q] : 0) : k_end - k[q];
-                if (n >= 8) {
-                    v = load_pack<T, 8>(p[q]);
-                } else {
+            }
+        } else {
+            int early = 0;
+            if constexpr (!TR) {
+                edge = k_slab + BK > k_end;
+                early = edge && k[0] + 8 > k_end ? k[0] + 8 - k_end : 0;
+                off[0] = early & 7;
+            }
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) v.v[e] = e < n ? p[q][e] : (T)0.f;
-                }
-                reg[q] = __builtin_bit_cast(uint4, v);
+            for (int q = 0; q < kPer; ++q) {
+                const T* src = k[TR ? q : 0] < k_end ? p[q] - early : (const T*)zero_page;
+                reg[q] = global16(src);
             }
         }
     }
     __device__ __forceinline__ void store(char* lds, int tid) {
         if constexpr (!DIRECT) {
+            if (edge) {
 #pragma unroll
-            for (int q = 0; q < kPer; ++q) *reinterpret_cast<uint4*>(lds + (q * 256 + tid) * 16) = reg[q];
+                for (int q = 0; q < kPer; ++q) reg[q] = shift_out(reg[q], off[TR ? q : 0]);
+            }
+#pragma unroll
+            for (int q = 0; q < kPer; ++q) *reinterpret_cast<u32x4*>(lds + (q * 256 + tid) * 16) = reg[q];
         }
     }
 };
@@ -315,8 +348,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void h
     for (int i = 0; i < FI; ++i)
 #pragma unroll
         for (int j = 0; j < FJ; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    sa.load(lds, wave);
-    sb.load(lds + kA, wave);
+    sa.load(lds, wave, k0);
+    sb.load(lds + kA, wave, k0);
     sa.store(lds, tid);
     sb.store(lds + kA, tid);
     for (int t = 0; t < nslab; ++t) {
@@ -327,8 +360,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void h
         if (t + 1 < nslab) {                                                  // in flight during the multiplies
             sa.advance();
             sb.advance();
-            sa.load(nxt, wave);
-            sb.load(nxt + kA, wave);
+            sa.load(nxt, wave, k0 + (t + 1) * BK);
+            sb.load(nxt + kA, wave, k0 + (t + 1) * BK);
         }
 #pragma unroll
         for (int s = 0; s < BK / 32; ++s) {
@@ -463,7 +496,8 @@ __global__ __launch_bounds__(256) void small_gemm(const Prod g) {
 // ---- dz = g * act'(z), the column sums of the unrounded products, and W^T ---------------------------------------------------------
 // A thread owns 8 columns and every (256 / lanes)-th row of the workgroup's rows, four rows in flight; part[row block][N] gets
 // the sums.  dz has the row pitch lddz, a multiple of 64, and zeros up to the next multiple of 8 columns, so that the products
-// take whole chunks.  The workgroups behind transpose W (N, K) into wt (K, N) with the same pitch and padding.
+// take whole chunks.  The workgroups behind transpose W (N, K) into wt (K, N) with the same pitch and padding; the last ones copy
+// an x of fewer than 8 columns into rows of 8.
 // n: the thread's first column.  WIDE (N >= 8): the thread of the last, short group takes the last 8 columns, of which
 // some belong to its neighbour: those come out twice, equal, and are summed once; it also writes the zeros behind column N.
 template <typename T, int ACT, bool WIDE>
@@ -545,7 +579,8 @@ __device__ __forceinline__ void dz_block(const T* __restrict__ g, long long ldg,
 template <typename T>
 __global__ __launch_bounds__(256) void act_bwd_k(const T* __restrict__ g, long long ldg, const T* __restrict__ z, int M, int N, int act,
                                                  int log2_lanes, int rows_wg, int col_tiles, int dz_wgs, T* __restrict__ dz, long long lddz,
-                                                 float* __restrict__ part, const T* __restrict__ w, long long ldw, int K, T* __restrict__ wt) {
+                                                 float* __restrict__ part, const T* __restrict__ w, long long ldw, int K, T* __restrict__ wt, int wt_wgs,
+                                                 const T* __restrict__ x, long long ldx, T* __restrict__ x8) {
     __shared__ float red[256 * 8];
     if ((int)blockIdx.x < dz_wgs) {
         if (act == HD_ACT_GELU) dz_block<T, HD_ACT_GELU>(g, ldg, z, M, N, log2_lanes, rows_wg, col_tiles, dz, lddz, part, red);
@@ -553,8 +588,18 @@ __global__ __launch_bounds__(256) void act_bwd_k(const T* __restrict__ g, long l
         else dz_block<T, HD_ACT_IDENTITY>(g, ldg, z, M, N, log2_lanes, rows_wg, col_tiles, dz, lddz, part, red);
         return;
     }
+    const int b = (int)blockIdx.x - dz_wgs;
+    if (b >= wt_wgs) {                                                        // rows of fewer than 8 elements, zeros behind them
+        const int m = (b - wt_wgs) * 256 + (int)threadIdx.x;
+        if (m >= M) return;
+        Pack<T, 8> v;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v.v[e] = e < K ? x[(long long)m * ldx + e] : (T)0.f;
+        store_pack<T, 8>(x8 + (long long)m * 8, v);
+        return;
+    }
     T* tile = (T*)red;                                                        // 32 x 33
-    const int tk = (K + 31) / 32, b = (int)blockIdx.x - dz_wgs, n0 = b / tk * 32, k0 = b % tk * 32;
+    const int tk = (K + 31) / 32, n0 = b / tk * 32, k0 = b % tk * 32;
     const int c = threadIdx.x & 31, r0 = threadIdx.x >> 5;
 #pragma unroll
     for (int r = r0; r < 32; r += 8) tile[r * 33 + c] = n0 + r < N && k0 + c < K ? w[(long long)(n0 + r) * ldw + k0 + c] : (T)0.f;
@@ -636,7 +681,8 @@ inline int64_t tiles_of(int64_t M, int64_t N, int64_t bm, int64_t bn) { return (
 //   up to 1280 tiles of 64 x 64 those: 8192 x 512 x 512 13.0 against 15.8; above, the large ones: 16384 x 512 x 512 20.3 against 23.5
 //   of the large ones the one with less time in its rounds over the chip: three 128 x 192 workgroups fit a CU, a round takes 37
 //   (K = 800), four of 128 x 128 take 34: 74750 x 900 151 against 170, 74750 x 512 77 against 66, 74750 x 700 144 against 136
-inline int choose_tiles(int64_t M, int64_t N, bool direct) {
+inline int choose_tiles(int64_t M, int64_t N, int64_t K, bool direct) {
+    if (K < 8 && !direct) return 0;                                           // no 8 elements in a row to load at once
     if (tiles_of(M, N, 32, 32) <= (direct ? 512 : 64)) return 0;
     if (tiles_of(M, N, 64, 64) <= 1280) return 1;
     const int64_t wide = (tiles_of(M, N, 128, 192) + 767) / 768 * 37, square = (tiles_of(M, N, 128, 128) + 1023) / 1024 * 34;
@@ -645,7 +691,7 @@ inline int choose_tiles(int64_t M, int64_t N, bool direct) {
 
 template <typename T>
 void launch_product(Prod g, bool direct, hipStream_t st) {
-    const int v = choose_tiles(g.M, g.N, direct);
+    const int v = choose_tiles(g.M, g.N, g.K, direct);
     if (v == 0) {
         g.tiles_n = (g.N + 31) / 32;
         small_gemm<T><<<(unsigned)tiles_of(g.M, g.N, 32, 32), 256, 0, st>>>(g);
@@ -671,7 +717,7 @@ struct BwdPlan {
     int log2_lanes, col_tiles, rows_wg, row_wgs;
     DwPlan dw;
     int64_t lddz;
-    int64_t off_wt, off_part, off_ws, bytes;
+    int64_t off_wt, off_x8, off_part, off_ws, bytes;
 };
 
 BwdPlan bwd_plan(int64_t M, int64_t N, int64_t K) {
@@ -692,6 +738,8 @@ BwdPlan bwd_plan(int64_t M, int64_t N, int64_t K) {
     int64_t at = up(M * p.lddz * 2);
     p.off_wt = at;
     at += up(K * p.lddz * 2);
+    p.off_x8 = at;
+    at += K < 8 ? up(M * 16) : 0;
     p.off_part = at;
     at += up((int64_t)p.row_wgs * N * 4);
     p.off_ws = at;
@@ -725,9 +773,11 @@ int linear_bwd(const T* g, int64_t ldg, const T* z, const T* x, int64_t ldx, con
     const bool copy = (dx || dw) && (act != HD_ACT_IDENTITY || !direct_ok(g, ldg, N, M));
     const int dz_wgs = copy || db ? p.row_wgs * p.col_tiles : 0;
     const int64_t wt_wgs = dx ? ((N + 31) / 32) * ((K + 31) / 32) : 0;
-    if (dz_wgs + wt_wgs)
-        act_bwd_k<T><<<(unsigned)(dz_wgs + wt_wgs), 256, 0, s>>>(g, ldg, z, (int)M, (int)N, act, p.log2_lanes, p.rows_wg, p.col_tiles, dz_wgs,
-                                                                copy ? (T*)ws : nullptr, p.lddz, part, w, ldw, (int)K, wt);
+    T* x8 = dw && K < 8 ? (T*)(ws + p.off_x8) : nullptr;
+    const int64_t x8_wgs = x8 ? (M + 255) / 256 : 0;
+    if (dz_wgs + wt_wgs + x8_wgs)
+        act_bwd_k<T><<<(unsigned)(dz_wgs + wt_wgs + x8_wgs), 256, 0, s>>>(g, ldg, z, (int)M, (int)N, act, p.log2_lanes, p.rows_wg, p.col_tiles, dz_wgs,
+                                                                copy ? (T*)ws : nullptr, p.lddz, part, w, ldw, (int)K, wt, (int)wt_wgs, x, ldx, x8);
     if (copy) { dz = (const T*)ws; lddz = p.lddz; }
     Prod q = {};
     q.act = HD_ACT_IDENTITY;
@@ -739,8 +789,8 @@ int linear_bwd(const T* g, int64_t ldg, const T* z, const T* x, int64_t ldx, con
         q.resid = nullptr;
     }
     if (dw) {                                                                 // (N, K) = dz^T (N, M) . x (M, K)
-        q.B = x; q.ldb = ldx; q.M = (int)N; q.N = (int)K; q.K = (int)M; q.C = ws + p.off_ws;
-        const bool direct = direct_ok(x, ldx, K, M);
+        q.B = x8 ? x8 : x; q.ldb = x8 ? 8 : ldx; q.M = (int)N; q.N = (int)K; q.K = (int)M; q.C = ws + p.off_ws;
+        const bool direct = x8 || direct_ok(x, ldx, K, M);
         if (p.dw.large) launch_tiles<T, true, 128, 192, 64>(q, p.dw.slices, direct, s);
         else launch_tiles<T, true, 64, 64, 32>(q, p.dw.slices, direct, s);
     }

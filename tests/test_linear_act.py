@@ -112,7 +112,7 @@ def _run(M, N, K, dtype, act, bias, resid, seed, pitch=0, lead=None, w_pitch=0, 
         assert torch.equal(t, grads[k]), k               # no order of sums to differ in
 
 
-SIZES = [(1, 1, 1), (1, 512, 512), (2, 7, 5), (15, 16, 17), (16, 8, 8), (33, 40, 24), (64, 64, 64), (127, 129, 72), (128, 128, 128),
+SIZES = [(1, 1, 1), (700, 90, 3), (5000, 5, 7), (3, 9, 8), (1, 512, 512), (2, 7, 5), (15, 16, 17), (16, 8, 8), (33, 40, 24), (64, 64, 64), (127, 129, 72), (128, 128, 128),
          (130, 136, 264), (200, 512, 512), (200, 64, 512), (200, 512, 64), (257, 300, 513), (1000, 14, 15), (300, 900, 800),
          (2049, 72, 88), (4100, 260, 136)]
 
