@@ -11,9 +11,10 @@
 // Three products C[m][n] = sum_k A(m, k) B(n, k): forward (A = x, B = W), dx (A = dz, B = W^T, which the launch that makes dz
 // also writes), dW (A = dz, B = x, both with k -- the rows of the batch -- as the slow index).
 //
-//   tiles     128 x 192 (4 wavefronts of 64 x 96), slabs of 32 k in two LDS buffers of 20 KB, so that three or four workgroups
-//             share a CU and one's epilogue runs beside another's products; 64 x 64 where that gives too few tiles to fill the
-//             chip; 32 x 32 with the contraction split over the wavefronts where even those are few (small_gemm).
+//   tiles     128 x 192, 128 x 128, 64 x 128 or 64 x 64 of 4 wavefronts, by a cost model (choose_tiles); 32 x 32 with the
+//             contraction split over the wavefronts for few rows (small_gemm).  One slab of 64 k in LDS, not two: a workgroup
+//             waits for its loads, and the 3 to 8 that fit a CU because of it multiply meanwhile (74750 x 800 -> 900: 137 us with
+//             three workgroups of one buffer, 165 with two, 173 with two of two buffers).
 //   staging   16-byte chunks go from memory to LDS without passing registers where every row starts on a 16-byte border and
 //             holds whole chunks; otherwise (an odd width, a sliced matrix) through registers, with the tail masked.  Chunks
 //             beyond the contraction's end come from a page of zeros, rows and columns beyond the matrix from a valid one
@@ -26,10 +27,10 @@
 //             consecutive k of its own column, so nothing is transposed in memory.
 //   split     the contraction of dW is cut into slices, one workgroup each; fp32 partial tiles are summed in slice order by
 //             the last launch, which also finishes db: the same bits on every call.
-// What bounds the large forward (74750 x 800 -> 900, bf16): bytes from L2 into the CUs.  A CU takes 64 bytes a clock in whole
-// 128-byte lines (34 TB/s for the chip), 16 TB/s in the 64-byte runs of a 32-k slab; the products alone take 72 us, the loads
-// alone 100, the stores and the GELU 25 more than they hide.
-#include <stdlib.h>
+// What bounds the large forward (74750 x 800 -> 900, bf16): bytes from L2 into the CUs, beside the products.  A CU takes 64 bytes a
+// clock in whole 128-byte lines (34 TB/s for the chip; 21 where the runs of 128 bytes straddle lines, as with rows of 1600 bytes;
+// 16 in runs of 64 bytes).  Timed alone: products 72 us, loads 70 to 100; stores and GELU cost 25 more than they hide.
+#include <type_traits>
 #include "hd_common.cuh"
 #include "hd_half.cuh"
 #include "hd_gelu.cuh"
@@ -320,14 +321,15 @@ __device__ __forceinline__ void write_tile(const Prod& g, const f32x4 (&acc)[FI]
         }
 }
 
-// ---- the tile kernel: 4 wavefronts as 2 x 2, two LDS buffers, one barrier a slab ------------------------------------------------
-template <typename T, bool TR, bool DIRECT, int BM, int BN, int BK>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void half_gemm(const Prod g) {
+// ---- the tile kernel: 4 wavefronts as 2 x 2, one slab in LDS -------------------------------------------------------------------------
+// OCC: wavefronts a SIMD that the registers have to allow, i.e. workgroups a CU
+template <typename T, bool TR, bool DIRECT, int BM, int BN, int BK, int OCC>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC))) void half_gemm(const Prod g) {
     constexpr int WM = BM / 2, WN = BN / 2, FI = WM / 16, FJ = WN / 16;       // a wavefront's part, its fragments
     using SA = Stager<T, BM, BK, TR, DIRECT, 0>;
     using SB = Stager<T, BN, BK, TR, DIRECT, TR ? 0 : WN>;
-    constexpr int kA = SA::L::kBytes, kStage = kA + SB::L::kBytes;
-    __shared__ __attribute__((aligned(1024))) char lds[2 * kStage];
+    constexpr int kA = SA::L::kBytes;
+    __shared__ __attribute__((aligned(1024))) char lds[kA + SB::L::kBytes];
     // workgroup b runs on XCD b % 8: every XCD a contiguous run of (slice, tile) pairs, so that tiles sharing rows meet in one L2
     const int per_xcd = (gridDim.x + 7) >> 3;
     const int vid = (blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3);
@@ -348,36 +350,39 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void h
     for (int i = 0; i < FI; ++i)
 #pragma unroll
         for (int j = 0; j < FJ; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    sa.load(lds, wave, k0);
+    sa.load(lds, wave, k0);                                                   // DIRECT: on its way to LDS; otherwise to registers
     sb.load(lds + kA, wave, k0);
-    sa.store(lds, tid);
-    sb.store(lds + kA, tid);
     for (int t = 0; t < nslab; ++t) {
+        sa.store(lds, tid);
+        sb.store(lds + kA, tid);
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();                                                      // slab t is in LDS; the other buffer is free
-        char* cur = lds + (t & 1) * kStage;
-        char* nxt = lds + ((t + 1) & 1) * kStage;
-        if (t + 1 < nslab) {                                                  // in flight during the multiplies
+        __syncthreads();                                                      // slab t is in LDS
+        if (!DIRECT && t + 1 < nslab) {                                       // to registers during the multiplies
             sa.advance();
             sb.advance();
-            sa.load(nxt, wave, k0 + (t + 1) * BK);
-            sb.load(nxt + kA, wave, k0 + (t + 1) * BK);
+            sa.load(lds, wave, k0 + (t + 1) * BK);
+            sb.load(lds + kA, wave, k0 + (t + 1) * BK);
         }
 #pragma unroll
         for (int s = 0; s < BK / 32; ++s) {
             uint4 fa[FI], fb[FJ];
 #pragma unroll
-            for (int i = 0; i < FI; ++i) fa[i] = SA::L::read(cur, wm, i, s, lane);
+            for (int i = 0; i < FI; ++i) fa[i] = SA::L::read(lds, wm, i, s, lane);
 #pragma unroll
-            for (int j = 0; j < FJ; ++j) fb[j] = SB::L::read(cur + kA, wn, j, s, lane);
+            for (int j = 0; j < FJ; ++j) fb[j] = SB::L::read(lds + kA, wn, j, s, lane);
 #pragma unroll
             for (int i = 0; i < FI; ++i)
 #pragma unroll
                 for (int j = 0; j < FJ; ++j) acc[i][j] = mfma<T>(fa[i], fb[j], acc[i][j]);   // D rows = m, D columns = n
         }
         if (t + 1 < nslab) {
-            sa.store(nxt, tid);
-            sb.store(nxt + kA, tid);
+            __syncthreads();                                                  // every wavefront has read slab t
+            if (DIRECT) {
+                sa.advance();
+                sb.advance();
+                sa.load(lds, wave, k0 + (t + 1) * BK);
+                sb.load(lds + kA, wave, k0 + (t + 1) * BK);
+            }
         }
     }
     if constexpr (TR) {                                                       // fp32 partial tile of this slice
@@ -659,34 +664,49 @@ inline bool direct_ok(const void* p, int64_t ld, int64_t inner, int64_t outer) {
     return (uintptr_t)p % 16 == 0 && inner % 8 == 0 && (ld % 8 == 0 || outer == 1);
 }
 
-template <typename T, bool TR, int BM, int BN, int BK>
+template <typename T, bool TR, int BM, int BN, int OCC>
 void launch_tiles(Prod g, int slices, bool direct, hipStream_t st) {
-    g.tiles_n = (g.N + BN - 1) / BN;
-    g.tiles = (g.M + BM - 1) / BM * g.tiles_n;
-    g.total = g.tiles * slices;
-    const int slabs = (g.K + BK - 1) / BK;
-    g.slabs = slabs / slices;
-    g.slabs_rem = slabs % slices;
-    const unsigned grid = (unsigned)((g.total + 7) / 8 * 8);
-    if (direct) half_gemm<T, TR, true, BM, BN, BK><<<grid, 256, 0, st>>>(g);
-    else half_gemm<T, TR, false, BM, BN, BK><<<grid, 256, 0, st>>>(g);
+    // slabs of 64 k; 32 where a slab passes through registers, which 64 would take from a resident workgroup
+    auto go = [&](auto bk, auto tag) {
+        constexpr int BK = decltype(bk)::value;
+        constexpr bool DIRECT = decltype(tag)::value;
+        g.tiles_n = (g.N + BN - 1) / BN;
+        g.tiles = (g.M + BM - 1) / BM * g.tiles_n;
+        g.total = g.tiles * slices;
+        const int slabs = (g.K + BK - 1) / BK;
+        g.slabs = slabs / slices;
+        g.slabs_rem = slabs % slices;
+        const unsigned grid = (unsigned)((g.total + 7) / 8 * 8);
+        half_gemm<T, TR, DIRECT, BM, BN, BK, DIRECT ? OCC : 2><<<grid, 256, 0, st>>>(g);
+    };
+    if (direct) go(std::integral_constant<int, 64>{}, std::true_type{});
+    else go(std::integral_constant<int, 32>{}, std::false_type{});
 }
 
 inline int64_t tiles_of(int64_t M, int64_t N, int64_t bm, int64_t bn) { return ((M + bm - 1) / bm) * ((N + bn - 1) / bn); }
 
-// Which kernel a product of M x N results takes: 0 small_gemm, 1 64 x 64, 2 128 x 128, 3 128 x 192 (bf16, GELU, us, the kernels
-// side by side):
-//   up to 512 tiles of 32 x 32 small_gemm: 512 x 512 x 512 5.0 against 7.9; above, 64 x 64: 2048 x 512 x 512 8.6 against 12.1
-//   (up to 64 tiles where rows start off 16-byte borders, whose fragments cost more loads: 512 x 800 x 513 16.8 against 9.7)
-//   up to 1280 tiles of 64 x 64 those: 8192 x 512 x 512 13.0 against 15.8; above, the large ones: 16384 x 512 x 512 20.3 against 23.5
-//   of the large ones the one with less time in its rounds over the chip: three 128 x 192 workgroups fit a CU, a round takes 37
-//   (K = 800), four of 128 x 128 take 34: 74750 x 900 151 against 170, 74750 x 512 77 against 66, 74750 x 700 144 against 136
+// Which kernel a product of M x N results takes.  0: small_gemm, up to 512 tiles of 32 x 32 (512 x 512 x 512 5.0 us against 7.9;
+// 2048 x 512 x 512 12.1 against 7.9), up to 64 where rows start off 16-byte borders, whose fragments cost more loads (512 x 800 x
+// 513 16.8 against 9.7).  Above, the least of start + share of the chip per 256 tiles, fitted to K = 800 (bf16, GELU, us; the
+// times at 4096, 8192, 16384 and 74750 rows of 900); the small ones cost 3.6 and 5.4 where slabs pass through registers (7850 x
+// 800 x 513: 29.6 us in 64 x 128 tiles, 25.3 in 128 x 128):
+//   1  64 x 64     6 + 2.85, at least 11      16.7   28.4   48.9   240
+//   2  64 x 128    6 + 4.6,  at least 13      15.1   24.5   42.9   179
+//   3  128 x 128   8 + 8.0,  at least 18      18.6   23.0   37.7   145
+//   4  128 x 192   8 + 12,   at least 20      20.9   26.3   36.9   137
 inline int choose_tiles(int64_t M, int64_t N, int64_t K, bool direct) {
     if (K < 8 && !direct) return 0;                                           // no 8 elements in a row to load at once
     if (tiles_of(M, N, 32, 32) <= (direct ? 512 : 64)) return 0;
-    if (tiles_of(M, N, 64, 64) <= 1280) return 1;
-    const int64_t wide = (tiles_of(M, N, 128, 192) + 767) / 768 * 37, square = (tiles_of(M, N, 128, 128) + 1023) / 1024 * 34;
-    return wide <= square ? 3 : 2;
+    static const struct { int bm, bn; double start, per, odd, least; } kind[4] = {
+        {64, 64, 6, 2.85, 3.6, 11}, {64, 128, 6, 4.6, 5.4, 13}, {128, 128, 8, 8, 8, 18}, {128, 192, 8, 12, 12, 20}};
+    int best = 0;
+    double least = 0;
+    for (int v = 0; v < 4; ++v) {
+        const double t = kind[v].start + (direct ? kind[v].per : kind[v].odd) / 256 * (double)tiles_of(M, N, kind[v].bm, kind[v].bn);
+        const double c = t > kind[v].least ? t : kind[v].least;
+        if (v == 0 || c < least) { best = v; least = c; }
+    }
+    return best + 1;
 }
 
 template <typename T>
@@ -695,17 +715,19 @@ void launch_product(Prod g, bool direct, hipStream_t st) {
     if (v == 0) {
         g.tiles_n = (g.N + 31) / 32;
         small_gemm<T><<<(unsigned)tiles_of(g.M, g.N, 32, 32), 256, 0, st>>>(g);
-    } else if (v == 1) launch_tiles<T, false, 64, 64, 32>(g, 1, direct, st);
-    else if (v == 2) launch_tiles<T, false, 128, 128, 32>(g, 1, direct, st);
-    else launch_tiles<T, false, 128, 192, 32>(g, 1, direct, st);
+    } else if (v == 1) launch_tiles<T, false, 64, 64, 4>(g, 1, direct, st);
+    else if (v == 2) launch_tiles<T, false, 64, 128, 4>(g, 1, direct, st);
+    else if (v == 3) launch_tiles<T, false, 128, 128, 4>(g, 1, direct, st);
+    else launch_tiles<T, false, 128, 192, 3>(g, 1, direct, st);
 }
 
-// slices of dW's contraction over R rows: one resident round of workgroups, slices of at least four slabs
+// dW's tiles and the slices of its contraction over R rows: one resident round of workgroups (two of 192 x 192 a CU, four of
+// 64 x 64), slices of at least 128 rows.  900 x 800 over 74750 rows: 139 us in 20 slices of 192 x 192 tiles, 156 in 12 of 128 x 192.
 struct DwPlan { bool large; int slices; };
 inline DwPlan dw_plan(int64_t R, int64_t P, int64_t Q) {
     DwPlan p;
-    p.large = R >= 2048 && tiles_of(P, Q, 128, 192) >= 8;
-    const int64_t tiles = p.large ? tiles_of(P, Q, 128, 192) : tiles_of(P, Q, 64, 64);
+    p.large = R >= 2048 && tiles_of(P, Q, 192, 192) >= 6;
+    const int64_t tiles = p.large ? tiles_of(P, Q, 192, 192) : tiles_of(P, Q, 64, 64);
     int64_t s = (p.large ? 512 : 1024) / tiles;
     const int64_t most = (R + 127) / 128;
     s = s > most ? most : s;
@@ -791,8 +813,8 @@ int linear_bwd(const T* g, int64_t ldg, const T* z, const T* x, int64_t ldx, con
     if (dw) {                                                                 // (N, K) = dz^T (N, M) . x (M, K)
         q.B = x8 ? x8 : x; q.ldb = x8 ? 8 : ldx; q.M = (int)N; q.N = (int)K; q.K = (int)M; q.C = ws + p.off_ws;
         const bool direct = x8 || direct_ok(x, ldx, K, M);
-        if (p.dw.large) launch_tiles<T, true, 128, 192, 64>(q, p.dw.slices, direct, s);
-        else launch_tiles<T, true, 64, 64, 32>(q, p.dw.slices, direct, s);
+        if (p.dw.large) launch_tiles<T, true, 192, 192, 2>(q, p.dw.slices, direct, s);
+        else launch_tiles<T, true, 64, 64, 4>(q, p.dw.slices, direct, s);
     }
     if (dw || db) {
         const int64_t count = dw ? N * K : 0;
