@@ -1,6 +1,6 @@
 // Linear layers on 16-bit operands (bf16 / fp16), fp32 accumulation on the matrix cores:
 //
-//   forward   z = x W^T + b,  y = resid + act(z)              (z kept in 16 bits for the backward pass)
+//   forward   z = x W^T + b,  y = resid + act(z)              (z kept in fp16 for the backward pass)
 //   backward  dz = g * act'(z),  dx = dz W,  dW = dz^T x,  db = colsum(dz)
 //
 // the mixed-precision form of the denoisers' nn.Linear + F.gelu (+ skip) layers (models/direction_diffusion.py:47-69,
@@ -233,13 +233,22 @@ __device__ __forceinline__ float act_slope(float z) {
     else return 1.f;
 }
 
+// The pre-activation as it is kept for the backward pass: in fp16 for bf16 operands too, whose own 8 bits would add a third of dz's
+// rounding to the gradients (error 1.5 instead of 1.41 roundings).  Only the slope reads it: beyond 30000 that is 0 or 1 (the
+// clamp keeps fp16 finite), and a positive z stays positive for ReLU.  A NaN stays one.
+__device__ __forceinline__ f16 kept_z(float z) {
+    const float c = fminf(fmaxf(z, -30000.f), 30000.f);
+    const float p = z > 0.f ? fmaxf(c, 0x1p-24f) : c;
+    return (f16)(z == z ? p : z);
+}
+
 struct Prod {
     const void *A, *B;
     long long lda, ldb;
     int M, N, K;
     void* C;                        // T (M, N) contiguous, or fp32 partial tiles [slice][M][N]
     const void *bias, *resid;
-    void* z;                        // (M, N) contiguous, or null
+    void* z;                        // fp16 (M, N) contiguous, or null
     long long ldr;
     int act;
     int z_past;                     // store z past the caches
@@ -258,9 +267,9 @@ __device__ __forceinline__ void write_row(const Prod& g, char* yb, char* zb, uns
     for (int e = 0; e < V; ++e) v[e] = acc[e] + bias[e];
     if (n + V <= g.N) {
         if (zb) {
-            Pack<T, V> zz;
+            Pack<f16, V> zz;
 #pragma unroll
-            for (int e = 0; e < V; ++e) zz.v[e] = (T)v[e];
+            for (int e = 0; e < V; ++e) zz.v[e] = kept_z(v[e]);
             if constexpr (V % 2 == 0) {
                 typedef unsigned words __attribute__((ext_vector_type(V / 2), aligned(2)));
                 words w;
@@ -268,7 +277,7 @@ __device__ __forceinline__ void write_row(const Prod& g, char* yb, char* zb, uns
                 if (g.z_past) __builtin_nontemporal_store(w, (words*)(zb + off));
                 else __builtin_memcpy(zb + off, &w, sizeof(w));
             } else {
-                store_pack<T, V>((T*)(zb + off), zz);
+                store_pack<f16, V>((f16*)(zb + off), zz);
             }
         }
 #pragma unroll
@@ -286,7 +295,7 @@ __device__ __forceinline__ void write_row(const Prod& g, char* yb, char* zb, uns
 #pragma unroll
         for (int e = 0; e < V; ++e) {
             if (n + e >= g.N) break;
-            if (zb) ((T*)(zb + off))[e] = (T)v[e];
+            if (zb) ((f16*)(zb + off))[e] = kept_z(v[e]);
             float s = act_value<ACT>(v[e]);
             if (g.resid) s += (float)resid[e];
             ((T*)(yb + off))[e] = (T)s;
@@ -506,22 +515,24 @@ __global__ __launch_bounds__(256) void small_gemm(const Prod g) {
 // n: the thread's first column.  WIDE (N >= 8): the thread of the last, short group takes the last 8 columns, of which
 // some belong to its neighbour: those come out twice, equal, and are summed once; it also writes the zeros behind column N.
 template <typename T, int ACT, bool WIDE>
-__device__ __forceinline__ void dz_rows(const T* __restrict__ g, long long ldg, const T* __restrict__ z, int N, int n, int m, int m1, int slots,
+__device__ __forceinline__ void dz_rows(const T* __restrict__ g, long long ldg, const f16* __restrict__ z, int N, int n, int m, int m1, int slots,
                                         T* __restrict__ dz, long long lddz, float (&s)[8]) {
     constexpr int U = 4;
-    auto fetch = [&](const T* p) {
-        Pack<T, 8> v;
+    auto fetch = [&](auto* p) {
+        using E = std::remove_const_t<std::remove_pointer_t<decltype(p)>>;
+        Pack<E, 8> v;
         if constexpr (WIDE) {
-            v = load_pack<T, 8>(p);
+            v = load_pack<E, 8>(p);
         } else {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v.v[e] = n + e < N ? p[e] : (T)0.f;
+            for (int e = 0; e < 8; ++e) v.v[e] = n + e < N ? p[e] : (E)0.f;
         }
         return v;
     };
     const int pads = WIDE && dz && n + 8 == N ? (8 - N % 8) % 8 : 0;
     for (; m < m1; m += U * slots) {
-        Pack<T, 8> a[U], b[U];
+        Pack<T, 8> a[U];
+        Pack<f16, 8> b[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int r = m + u * slots < m1 ? m + u * slots : m;              // a row that is not there: read another, count none
@@ -549,7 +560,7 @@ __device__ __forceinline__ void dz_rows(const T* __restrict__ g, long long ldg, 
 }
 
 template <typename T, int ACT>
-__device__ __forceinline__ void dz_block(const T* __restrict__ g, long long ldg, const T* __restrict__ z, int M, int N, int log2_lanes,
+__device__ __forceinline__ void dz_block(const T* __restrict__ g, long long ldg, const f16* __restrict__ z, int M, int N, int log2_lanes,
                                          int rows_wg, int col_tiles, T* __restrict__ dz, long long lddz, float* __restrict__ part,
                                          float* red) {
     const int lanes = 1 << log2_lanes, slots = 256 >> log2_lanes;
@@ -582,7 +593,7 @@ __device__ __forceinline__ void dz_block(const T* __restrict__ g, long long ldg,
 }
 
 template <typename T>
-__global__ __launch_bounds__(256) void act_bwd_k(const T* __restrict__ g, long long ldg, const T* __restrict__ z, int M, int N, int act,
+__global__ __launch_bounds__(256) void act_bwd_k(const T* __restrict__ g, long long ldg, const f16* __restrict__ z, int M, int N, int act,
                                                  int log2_lanes, int rows_wg, int col_tiles, int dz_wgs, T* __restrict__ dz, long long lddz,
                                                  float* __restrict__ part, const T* __restrict__ w, long long ldw, int K, T* __restrict__ wt, int wt_wgs,
                                                  const T* __restrict__ x, long long ldx, T* __restrict__ x8) {
@@ -785,7 +796,7 @@ int linear_fwd(const Prod& g, bool direct, hipStream_t s) {
 }
 
 template <typename T>
-int linear_bwd(const T* g, int64_t ldg, const T* z, const T* x, int64_t ldx, const T* w, int64_t ldw, int64_t M, int64_t N, int64_t K,
+int linear_bwd(const T* g, int64_t ldg, const f16* z, const T* x, int64_t ldx, const T* w, int64_t ldw, int64_t M, int64_t N, int64_t K,
                int act, const T* dx_add, int64_t ld_add, T* dx, T* dw, T* db, const BwdPlan& p, unsigned char* ws, hipStream_t s) {
     const T* dz = g;
     long long lddz = ldg;
@@ -871,7 +882,7 @@ extern "C" int hd_linear_act_bwd(const void* g, int64_t ldg, const void* z, cons
     unsigned char* ws = (unsigned char*)workspace;
     hipStream_t s = (hipStream_t)st;
     if (dtype == HD_DT_BF16)
-        return linear_bwd<bf16>((const bf16*)g, ldg, (const bf16*)z, (const bf16*)x, ldx, (const bf16*)w, ldw, M, N, K, act, (const bf16*)dx_add, ld_add, (bf16*)dx,
+        return linear_bwd<bf16>((const bf16*)g, ldg, (const f16*)z, (const bf16*)x, ldx, (const bf16*)w, ldw, M, N, K, act, (const bf16*)dx_add, ld_add, (bf16*)dx,
                                 (bf16*)dw, (bf16*)db, p, ws, s);
     return linear_bwd<f16>((const f16*)g, ldg, (const f16*)z, (const f16*)x, ldx, (const f16*)w, ldw, M, N, K, act, (const f16*)dx_add,
                            ld_add, (f16*)dx, (f16*)dw, (f16*)db, p, ws, s);

@@ -770,7 +770,7 @@ def linear_act(x, weight, bias=None, act="identity", resid=None):
 
     x (..., K), weight (N, K), bias (N) or None, resid (..., N) or None, all of one type; the result has that type.
     Differentiable in all four: one fused pass for dL/dz and the bias gradient, then the two products; the pre-activation is
-    kept in the operands' type, dL/dz is rounded to it for the products, sums are in fp32 and in a fixed order (the same
+    kept in fp16, dL/dz is rounded to it for the products, sums are in fp32 and in a fixed order (the same
     bits on every run).  The 16-bit form of the layers that linear_chain / autograd.linear_stack run in fp32
     (models/direction_diffusion.py:47-69, ddpm.py:9-27)."""
     dt, ws, xs = x.dtype, weight.shape, x.shape
@@ -826,31 +826,33 @@ def _linear_act_fwd(x, w, b, resid, act, want_z):
     x2, ldx = _matrix(x)
     w2, ldw = _matrix(w)
     M, (N, K) = x2.shape[0], w2.shape
-    dt, dev = x.dtype, x.device
-    y = torch.empty(x.shape[:-1] + (N,), dtype=dt, device=dev)
-    z = torch.empty((M, N), dtype=dt, device=dev) if want_z else None
+    y = x2.new_empty(x.shape[:-1] + (N,))
+    z = x2.new_empty((M, N), dtype=torch.float16) if want_z else None
     if M:
         r2, ldr = (None, 0) if resid is None else _pitched(resid.detach().reshape(M, N))
-        b = None if b is None else b.detach().contiguous()
-        _lib.call("hd_linear_act_fwd", x2.data_ptr(), ldx, w2.data_ptr(), ldw, _p(b), _p(r2), ldr, DT_CODES[dt], M, N, K, act,
-                  y.data_ptr(), _p(z), raw_stream())
+        if b is not None and not b.is_contiguous():
+            b = b.detach().contiguous()
+        _lib.call("hd_linear_act_fwd", x2.data_ptr(), ldx, w2.data_ptr(), ldw, None if b is None else b.data_ptr(),
+                  None if r2 is None else r2.data_ptr(), ldr, DT_CODES[x2.dtype], M, N, K, act, y.data_ptr(),
+                  None if z is None else z.data_ptr(), raw_stream())
     return y, z, x2, ldx, w2, ldw
 
 
 def _linear_act_bwd(g, z, x2, w2, ldx, ldw, act, x_shape, skip, need_x, need_w, need_b):
-    _dev(g, x2, w2)
+    if not (g.get_device() == x2.get_device() == w2.get_device() == _cur_device()):
+        _dev(g, x2, w2)                                   # says which one is elsewhere
     g2, ldg = _matrix(g)
     M, (N, K) = x2.shape[0], w2.shape
-    dt, dev = x2.dtype, x2.device
-    new = torch.empty if M else torch.zeros
-    dx = new(x_shape, dtype=dt, device=dev) if need_x else None
-    dw = new((N, K), dtype=dt, device=dev) if need_w else None
-    db = new((N,), dtype=dt, device=dev) if need_b else None
+    new = x2.new_empty if M else x2.new_zeros
+    dx = new(x_shape) if need_x else None
+    dw = new((N, K)) if need_w else None
+    db = new((N,)) if need_b else None
     if M:
         nbytes = _lib.load().hd_linear_act_bwd_workspace_bytes(M, N, K, act)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-        _lib.call("hd_linear_act_bwd", g2.data_ptr(), ldg, _p(z), x2.data_ptr(), ldx, w2.data_ptr(), ldw, DT_CODES[dt], M, N, K, act,
-                  g2.data_ptr() if skip and need_x else None, ldg, _p(dx), _p(dw), _p(db), ws.data_ptr(), nbytes, raw_stream())
+        ws = x2.new_empty((nbytes,), dtype=torch.uint8)
+        _lib.call("hd_linear_act_bwd", g2.data_ptr(), ldg, None if z is None else z.data_ptr(), x2.data_ptr(), ldx, w2.data_ptr(), ldw,
+                  DT_CODES[x2.dtype], M, N, K, act, g2.data_ptr() if skip and need_x else None, ldg, None if dx is None else dx.data_ptr(),
+                  None if dw is None else dw.data_ptr(), None if db is None else db.data_ptr(), ws.data_ptr(), nbytes, raw_stream())
     return dx, dw, db
 
 

@@ -450,7 +450,7 @@ int hd_adam_step_f32(const hd_adam_job* jobs, int n_jobs, const void* grad_flat,
  *   z = x W^T + bias,  y = resid + act(z)
  * x (M, K) with row pitch ldx, W (N, K) with row pitch ldw, bias (N) or NULL, resid (M, N) with row pitch ldr (0: one row for
  * all) or NULL, y (M, N) contiguous; act HD_ACT_IDENTITY, HD_ACT_RELU or HD_ACT_GELU.  z (M, N) contiguous or NULL: the
- * pre-activation, rounded, for the backward pass.  y is rounded once, from fp32.  Any sizes, pitches and element-aligned
+ * pre-activation for the backward pass, in fp16 for both types (clamped to +-30000; the slope there is 0 or 1).  y is rounded once, from fp32.  Any sizes, pitches and element-aligned
  * pointers; rows that start on 16-byte borders and hold a multiple of 8 elements are fastest.  y and z overlap nothing. */
 int hd_linear_act_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, const void* resid, int64_t ldr,
                       int dtype, int64_t M, int64_t N, int64_t K, int act, void* y, void* z, void* stream);

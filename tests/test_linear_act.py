@@ -32,7 +32,7 @@ def _reference(x, w, b, r, g, act, dtype):
           more rounding: ez.
     y     act is 1.13-Lipschitz (GELU) and evaluated to 2e-6 |z| (the kernel's fit of erfc) + 4 u |z|, the residual one
           rounding, storage half a step.
-    dz    z was stored with a relative half step h (and fp16's smallest step), g times a slope that moves by at most 0.8 per
+    dz    z was stored in fp16 (its relative half step and smallest step), g times a slope that moves by at most 0.8 per
           unit of z, except at ReLU's border, where an element within the error of 0 may count or not; the product and the
           slope's evaluation (2e-6 for erfc, 8 u for the rest): 2.5e-6 |g|; storage of dz another h.
     dx dw db   sums of those errors against |W|, |x|, 1, and the sum's own roundings."""
@@ -49,7 +49,7 @@ def _reference(x, w, b, r, g, act, dtype):
     out = {"y": (y, ey * (1 + h) + h * y.abs() + tiny)}
     if g is None:
         return out
-    moved = ez * (1 + h) + (0.0 if act == "identity" else h) * z.abs() + tiny
+    moved = ez * (1 + h) + (0.0 if act == "identity" else HALF[torch.float16]) * z.abs() + TINY[torch.float16]
     if act == "relu":
         ds = (z.abs() <= moved).double()
     else:
@@ -196,6 +196,20 @@ def test_no_rows():
     assert y.shape == (0, 16)
     dx, dw, db = torch.autograd.grad(y, [x, w, b], torch.zeros(0, 16, device="cuda", dtype=torch.bfloat16))
     assert dx.shape == (0, 24) and not dw.any() and not db.any()
+
+
+@gpu
+@pytest.mark.parametrize("act", ["gelu", "relu"])
+def test_large_and_tiny_preactivations_keep_their_slope(act):
+    """z far outside fp16 (it is kept clamped) has slope 0 or 1; a tiny positive z counts for ReLU; an infinite y is passed on"""
+    from hypdiff_amd import ops
+    x = torch.tensor([[3e38], [1e30], [7e4], [1e-30], [-1e-30], [-7e4], [-1e30]], device="cuda").bfloat16().requires_grad_(True)
+    w = torch.ones(8, 1, device="cuda", dtype=torch.bfloat16)
+    y = ops.linear_act(x, w, act=act)
+    dx = torch.autograd.grad(y, [x], torch.ones(7, 8, device="cuda", dtype=torch.bfloat16))[0].flatten().tolist()
+    small = (0.5, 0.5) if act == "gelu" else (1.0, 0.0)
+    assert dx == [8.0, 8.0, 8.0, 8 * small[0], 8 * small[1], 0.0, 0.0]
+    assert torch.equal(y[:3, 0], x.detach()[:3, 0]) and float(y[5:].abs().max()) == 0.0
 
 
 @gpu
