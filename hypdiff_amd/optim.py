@@ -157,7 +157,7 @@ class AdamW(torch.optim.Optimizer):
         return loss
 
     def _step_group(self, group, fl):
-        # the host's part is most of a small model's step: about 0.9 us a tensor and 15 us besides
+        # the host's part is most of a small model's step
         options = (group["lr"], group["betas"], group["eps"], group["weight_decay"], group["state_bits"], group["master_weights"])
         if fl.checked != options:
             self._check_options(group)
@@ -169,31 +169,9 @@ class AdamW(torch.optim.Optimizer):
             raise RuntimeError("AdamW: the parameters of a group changed after its first step")
         if torch.cuda.is_current_stream_capturing():
             fl.device_count = True
-        counted = fl.device_count
         cur = torch.cuda.current_device()
-        steps, states, numels = fl.steps, fl.states, fl.numels
-        batches, keep, touched = {}, [], []
-        for i, p in enumerate(params):
-            g = p.grad
-            if g is None:
-                continue
-            dt, n = p.dtype, numels[i]
-            if g.dtype is not dt or g.get_device() != cur or p.get_device() != cur or g.layout is not torch.strided \
-                    or p.numel() != n or g.numel() != n or not p.is_contiguous():
-                self._refuse(i, p, g, fl, cur)
-            if not g.is_contiguous():
-                g = g.contiguous()
-                keep.append(g)                            # lives until the launch is enqueued; its memory is stream-ordered
-            t = steps[i] + 1
-            touched.append((i, p, t))
-            if n:
-                # one launch has one element type and one step count
-                b = batches.get((dt, 0 if counted else t))
-                if b is None:
-                    b = batches[(dt, 0 if counted else t)] = ([], [], [])
-                b[0].append(i)
-                b[1].append(p.data_ptr())
-                b[2].append(g.data_ptr())
+        keep = []
+        batches, touched = self._all_present(params, fl, cur) or self._one_by_one(params, fl, cur, keep)
         b = fl.buffers
         second = b["exp_avg_sq"] if fl.bits == 32 else b["exp_avg_sq_root"]
         most = _lib.load().hd_adamw_max_jobs()
@@ -207,10 +185,55 @@ class AdamW(torch.optim.Optimizer):
                           ops._p(b["exp_avg"]), ops._p(second), ops._p(b.get("exp_avg_scale")),
                           ops._p(b.get("exp_avg_sq_root_scale")), ops._p(master), fl.total, lr, float(b1), float(b2), eps, wd, t,
                           ops._p(fl.table), len(params), ops._stream())
-        for i, _, t in touched:                           # counted once the launches are under way
-            steps[i] = states[i]["step"] = t
+        steps, states = fl.steps, fl.states
+        for i in touched:                                 # counted once the launches are under way
+            steps[i] = states[i]["step"] = steps[i] + 1
         # the kernel wrote behind autograd's back: the versions key the caches of weight copies, and a saved tensor must notice
-        torch.autograd.graph.increment_version([p for _, p, _ in touched])
+        torch.autograd.graph.increment_version(params if len(touched) == len(params) else [params[i] for i in touched])
+
+    @staticmethod
+    def _all_present(params, fl, cur):
+        """the usual step: every gradient there, of its parameter's type and size, contiguous, one type and one count in the
+        group: the launch's lists and the indices, or None (then _one_by_one looks at every tensor and says what is wrong)"""
+        t = fl.steps[0]
+        dt = params[0].dtype
+        if fl.steps.count(t) != len(params) or 0 in fl.numels:
+            return None
+        grads = [p.grad for p in params]
+        T = torch.Tensor
+        try:
+            if not (list(map(T.numel, grads)) == fl.numels == list(map(T.numel, params))
+                    and {g.dtype for g in grads} == {p.dtype for p in params} == {dt}
+                    and set(map(T.get_device, grads)) == set(map(T.get_device, params)) == {cur}
+                    and all(map(T.is_contiguous, grads)) and all(map(T.is_contiguous, params))):
+                return None
+            pointers = list(map(T.data_ptr, params)), list(map(T.data_ptr, grads))
+        except (TypeError, RuntimeError):                 # no gradient, or one without strides
+            return None
+        rows = range(len(params))
+        return {(dt, 0 if fl.device_count else t + 1): (rows,) + pointers}, rows
+
+    def _one_by_one(self, params, fl, cur, keep):
+        batches, touched = {}, []
+        for i, p in enumerate(params):
+            g = p.grad
+            if g is None:
+                continue
+            dt, n = p.dtype, fl.numels[i]
+            if g.dtype is not dt or g.get_device() != cur or p.get_device() != cur or g.layout is not torch.strided \
+                    or p.numel() != n or g.numel() != n or not p.is_contiguous():
+                self._refuse(i, p, g, fl, cur)
+            if not g.is_contiguous():
+                g = g.contiguous()
+                keep.append(g)                            # lives until the launch is enqueued; its memory is stream-ordered
+            touched.append(i)
+            if n:
+                # one launch has one element type and one step count
+                rows, ptrs, grads = batches.setdefault((dt, 0 if fl.device_count else fl.steps[i] + 1), ([], [], []))
+                rows.append(i)
+                ptrs.append(p.data_ptr())
+                grads.append(g.data_ptr())
+        return batches, touched
 
     @staticmethod
     def _refuse(i, p, g, fl, cur):
