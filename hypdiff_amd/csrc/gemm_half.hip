@@ -331,18 +331,15 @@ __device__ __forceinline__ void write_tile(const Prod& g, const f32x4 (&acc)[FI]
 }
 
 // ---- the tile kernel: 4 wavefronts as 2 x 2, one slab in LDS -------------------------------------------------------------------------
-// OCC: wavefronts a SIMD that the registers have to allow, i.e. workgroups a CU
-template <typename T, bool TR, bool DIRECT, int BM, int BN, int BK, int OCC>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC))) void half_gemm(const Prod g) {
+template <bool TR, bool DIRECT, int BM, int BN, int BK>
+constexpr int kTileLds = (Slab<BM, BK, TR>::kBytes + Slab<BN, BK, TR>::kBytes);
+
+template <typename T, bool TR, bool DIRECT, int BM, int BN, int BK>
+__device__ __forceinline__ void tile_item(const Prod& g, int vid, char* lds) {
     constexpr int WM = BM / 2, WN = BN / 2, FI = WM / 16, FJ = WN / 16;       // a wavefront's part, its fragments
     using SA = Stager<T, BM, BK, TR, DIRECT, 0>;
     using SB = Stager<T, BN, BK, TR, DIRECT, TR ? 0 : WN>;
     constexpr int kA = SA::L::kBytes;
-    __shared__ __attribute__((aligned(1024))) char lds[kA + SB::L::kBytes];
-    // workgroup b runs on XCD b % 8: every XCD a contiguous run of (slice, tile) pairs, so that tiles sharing rows meet in one L2
-    const int per_xcd = (gridDim.x + 7) >> 3;
-    const int vid = (blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3);
-    if (vid >= g.total) return;                                               // uniform: the grid is rounded up to a multiple of 8
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int tile = vid % g.tiles, slice = vid / g.tiles;
     const int tm = tile / g.tiles_n, tn = tile - tm * g.tiles_n;
@@ -415,6 +412,17 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC))) void
     }
 }
 
+// OCC: wavefronts a SIMD that the registers have to allow, i.e. workgroups a CU
+template <typename T, bool TR, bool DIRECT, int BM, int BN, int BK, int OCC>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC))) void half_gemm(const Prod g) {
+    __shared__ __attribute__((aligned(1024))) char lds[kTileLds<TR, DIRECT, BM, BN, BK>];
+    // workgroup b runs on XCD b % 8: every XCD a contiguous run of (slice, tile) pairs, so that tiles sharing rows meet in one L2
+    const int per_xcd = (gridDim.x + 7) >> 3;
+    const int vid = (blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3);
+    if (vid >= g.total) return;                                               // uniform: the grid is rounded up to a multiple of 8
+    tile_item<T, TR, DIRECT, BM, BN, BK>(g, vid, lds);
+}
+
 // ---- few rows: 32 x 32 tiles, the contraction dealt over the 4 wavefronts -----------------------------------------------------------
 // With so few tiles a slab-by-slab loop is a chain of load latencies (200 x 512 x 512: 8 workgroups of 16 slabs).  Here a
 // wavefront loads the fragments of 4 slabs straight into registers, all in flight together, and multiplies; the four partial
@@ -430,12 +438,14 @@ __device__ __forceinline__ uint4 load_frag_tail(const T* row, int k, int K) {   
     return __builtin_bit_cast(uint4, v);
 }
 
+constexpr int kSmallLds = 4 * 32 * 36 * 4;
+
 template <typename T>
-__global__ __launch_bounds__(256) void small_gemm(const Prod g) {
-    __shared__ float red[4][32][36];
+__device__ __forceinline__ void small_item(const Prod& g, int vid, char* lds) {
+    float (*red)[32][36] = reinterpret_cast<float (*)[32][36]>(lds);
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int r16 = lane & 15, kq = lane >> 4;
-    const int tm = blockIdx.x / g.tiles_n, tn = blockIdx.x - tm * g.tiles_n;
+    const int tm = vid / g.tiles_n, tn = vid - tm * g.tiles_n;
     const int m0 = tm * 32, n0 = tn * 32;
     const T *pa[2], *pb[2];
 #pragma unroll
@@ -505,6 +515,21 @@ __global__ __launch_bounds__(256) void small_gemm(const Prod g) {
     if (g.act == HD_ACT_GELU) write_row<T, 4, HD_ACT_GELU>(g, yb, zb, 0, m, n, v, bias);
     else if (g.act == HD_ACT_RELU) write_row<T, 4, HD_ACT_RELU>(g, yb, zb, 0, m, n, v, bias);
     else write_row<T, 4, HD_ACT_IDENTITY>(g, yb, zb, 0, m, n, v, bias);
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void small_gemm(const Prod g) {
+    __shared__ __attribute__((aligned(16))) char lds[kSmallLds];
+    small_item<T>(g, (int)blockIdx.x, lds);
+}
+
+// dx by small_gemm and dW's slices by 64 x 64 tiles in one launch: with few rows neither fills the chip nor waits for the other
+template <typename T, bool DIRECT, int BK>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4))) void small_pair(const Prod dx, const Prod dw, int dx_wgs) {
+    constexpr int kTile = kTileLds<true, DIRECT, 64, 64, BK>;
+    __shared__ __attribute__((aligned(1024))) char lds[kTile > kSmallLds ? kTile : kSmallLds];
+    if ((int)blockIdx.x < dx_wgs) small_item<T>(dx, (int)blockIdx.x, lds);
+    else tile_item<T, true, DIRECT, 64, 64, BK>(dw, (int)blockIdx.x - dx_wgs, lds);
 }
 
 // ---- dz = g * act'(z), the column sums of the unrounded products, and W^T ---------------------------------------------------------
@@ -675,18 +700,22 @@ inline bool direct_ok(const void* p, int64_t ld, int64_t inner, int64_t outer) {
     return (uintptr_t)p % 16 == 0 && inner % 8 == 0 && (ld % 8 == 0 || outer == 1);
 }
 
+inline void cut(Prod& g, int bm, int bn, int bk, int slices) {
+    g.tiles_n = (g.N + bn - 1) / bn;
+    g.tiles = (g.M + bm - 1) / bm * g.tiles_n;
+    g.total = g.tiles * slices;
+    const int slabs = (g.K + bk - 1) / bk;
+    g.slabs = slabs / slices;
+    g.slabs_rem = slabs % slices;
+}
+
 template <typename T, bool TR, int BM, int BN, int OCC>
 void launch_tiles(Prod g, int slices, bool direct, hipStream_t st) {
     // slabs of 64 k; 32 where a slab passes through registers, which 64 would take from a resident workgroup
     auto go = [&](auto bk, auto tag) {
         constexpr int BK = decltype(bk)::value;
         constexpr bool DIRECT = decltype(tag)::value;
-        g.tiles_n = (g.N + BN - 1) / BN;
-        g.tiles = (g.M + BM - 1) / BM * g.tiles_n;
-        g.total = g.tiles * slices;
-        const int slabs = (g.K + BK - 1) / BK;
-        g.slabs = slabs / slices;
-        g.slabs_rem = slabs % slices;
+        cut(g, BM, BN, BK, slices);
         const unsigned grid = (unsigned)((g.total + 7) / 8 * 8);
         half_gemm<T, TR, DIRECT, BM, BN, BK, DIRECT ? OCC : 2><<<grid, 256, 0, st>>>(g);
     };
@@ -812,20 +841,24 @@ int linear_bwd(const T* g, int64_t ldg, const f16* z, const T* x, int64_t ldx, c
         act_bwd_k<T><<<(unsigned)(dz_wgs + wt_wgs + x8_wgs), 256, 0, s>>>(g, ldg, z, (int)M, (int)N, act, p.log2_lanes, p.rows_wg, p.col_tiles, dz_wgs,
                                                                 copy ? (T*)ws : nullptr, p.lddz, part, w, ldw, (int)K, wt, (int)wt_wgs, x, ldx, x8);
     if (copy) { dz = (const T*)ws; lddz = p.lddz; }
-    Prod q = {};
+    Prod q = {}, v = {};
     q.act = HD_ACT_IDENTITY;
     q.A = dz; q.lda = lddz;
-    if (dx) {                                                                 // (M, K) = dz (M, N) . W^T (K, N), zeros up to whole chunks
-        q.B = wt; q.ldb = p.lddz; q.M = (int)M; q.N = (int)K; q.K = (int)((N + 7) / 8 * 8); q.C = dx;
-        q.resid = dx_add; q.ldr = ld_add;
-        launch_product<T>(q, true, s);
-        q.resid = nullptr;
-    }
-    if (dw) {                                                                 // (N, K) = dz^T (N, M) . x (M, K)
-        q.B = x8 ? x8 : x; q.ldb = x8 ? 8 : ldx; q.M = (int)N; q.N = (int)K; q.K = (int)M; q.C = ws + p.off_ws;
-        const bool direct = x8 || direct_ok(x, ldx, K, M);
-        if (p.dw.large) launch_tiles<T, true, 192, 192, 2>(q, p.dw.slices, direct, s);
-        else launch_tiles<T, true, 64, 64, 4>(q, p.dw.slices, direct, s);
+    v = q;
+    // dx: (M, K) = dz (M, N) . W^T (K, N), zeros up to whole chunks;  dW: (N, K) = dz^T (N, M) . x (M, K)
+    q.B = wt; q.ldb = p.lddz; q.M = (int)M; q.N = (int)K; q.K = (int)((N + 7) / 8 * 8); q.C = dx; q.resid = dx_add; q.ldr = ld_add;
+    v.B = x8 ? x8 : x; v.ldb = x8 ? 8 : ldx; v.M = (int)N; v.N = (int)K; v.K = (int)M; v.C = ws + p.off_ws;
+    const bool direct = x8 || direct_ok(x, ldx, K, M);
+    if (dx && dw && !p.dw.large && choose_tiles(q.M, q.N, q.K, true) == 0) {
+        const int dx_wgs = (int)tiles_of(M, K, 32, 32);
+        q.tiles_n = (q.N + 31) / 32;
+        cut(v, 64, 64, direct ? 64 : 32, p.dw.slices);
+        if (direct) small_pair<T, true, 64><<<(unsigned)(dx_wgs + v.total), 256, 0, s>>>(q, v, dx_wgs);
+        else small_pair<T, false, 32><<<(unsigned)(dx_wgs + v.total), 256, 0, s>>>(q, v, dx_wgs);
+    } else {
+        if (dx) launch_product<T>(q, true, s);
+        if (dw && p.dw.large) launch_tiles<T, true, 192, 192, 2>(v, p.dw.slices, direct, s);
+        else if (dw) launch_tiles<T, true, 64, 64, 4>(v, p.dw.slices, direct, s);
     }
     if (dw || db) {
         const int64_t count = dw ? N * K : 0;
