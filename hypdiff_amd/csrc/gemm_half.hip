@@ -30,6 +30,7 @@
 // What bounds the large forward (74750 x 800 -> 900, bf16): bytes from L2 into the CUs, beside the products.  A CU takes 64 bytes a
 // clock in whole 128-byte lines (34 TB/s for the chip; 21 where the runs of 128 bytes straddle lines, as with rows of 1600 bytes;
 // 16 in runs of 64 bytes).  Timed alone: products 72 us, loads 70 to 100; stores and GELU cost 25 more than they hide.
+#include <math.h>
 #include <type_traits>
 #include "hd_common.cuh"
 #include "hd_half.cuh"
@@ -761,16 +762,19 @@ void launch_product(Prod g, bool direct, hipStream_t st) {
     else launch_tiles<T, false, 128, 192, 3>(g, 1, direct, st);
 }
 
-// dW's tiles and the slices of its contraction over R rows: one resident round of workgroups (two of 192 x 192 a CU, four of
-// 64 x 64), slices of at least 128 rows.  900 x 800 over 74750 rows: 139 us in 20 slices of 192 x 192 tiles, 156 in 12 of 128 x 192.
+// dW's tiles and the slices of its contraction over R rows (bf16, us, with the launch that adds the slices up).
+//   from 8e9 products on, 192 x 192 tiles in one resident round of two workgroups a CU: 900 x 800 over 74750 rows 133 (64 x 64:
+//   237), over 16384 rows 44 (53), 512 x 512 over 74750 rows 56 (60)
+//   below, 64 x 64 tiles in s slices: a slice's slabs cost about 0.5 each, and s partial tiles are written and read at 4 TB/s, so
+//   s = sqrt(slabs * 250000 / (P Q)): 512 x 512 over 16384 rows 21 in 16 slices (192 x 192: 28), over 2048 rows 10 in 6 (16.6),
+//   900 x 800 over 4096 rows 21 in 4 (25)
 struct DwPlan { bool large; int slices; };
 inline DwPlan dw_plan(int64_t R, int64_t P, int64_t Q) {
     DwPlan p;
-    p.large = R >= 2048 && tiles_of(P, Q, 192, 192) >= 6;
-    const int64_t tiles = p.large ? tiles_of(P, Q, 192, 192) : tiles_of(P, Q, 64, 64);
-    int64_t s = (p.large ? 512 : 1024) / tiles;
-    const int64_t most = (R + 127) / 128;
-    s = s > most ? most : s;
+    p.large = (double)R * (double)P * (double)Q >= 8e9 && tiles_of(P, Q, 192, 192) >= 6;
+    const int64_t slabs = (R + 63) / 64;
+    int64_t s = p.large ? 512 / tiles_of(P, Q, 192, 192) : (int64_t)(sqrt((double)slabs * 250000.0 / ((double)P * (double)Q)) + 0.5);
+    s = s > slabs ? slabs : s;
     p.slices = (int)(s < 1 ? 1 : (s > 64 ? 64 : s));
     return p;
 }
