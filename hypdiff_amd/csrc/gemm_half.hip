@@ -12,14 +12,14 @@
 // also writes), dW (A = dz, B = x, both with k -- the rows of the batch -- as the slow index).
 //
 //   tiles     128 x 192, 128 x 128, 64 x 128 or 64 x 64 of 4 wavefronts, by a cost model (choose_tiles); 32 x 32 with the
-//             contraction split over the wavefronts for few rows (small_gemm).  One slab of 64 k in LDS, not two: a workgroup
+//             contraction split over the wavefronts for few rows (small_gemm); dW 192 x 192 or 64 x 64 (dw_plan).  One slab of 64 k in LDS, not two: a workgroup
 //             waits for its loads, and the 3 to 8 that fit a CU because of it multiply meanwhile (74750 x 800 -> 900: 137 us with
 //             three workgroups of one buffer, 165 with two, 173 with two of two buffers).
 //   staging   16-byte chunks go from memory to LDS without passing registers where every row starts on a 16-byte border and
 //             holds whole chunks; otherwise (an odd width, a sliced matrix) through registers, with the tail masked.  Chunks
 //             beyond the contraction's end come from a page of zeros, rows and columns beyond the matrix from a valid one
 //             (their results are not stored).
-//   LDS       a slab with k fast has rows of 64 bytes whose chunks are permuted by row (c ^ f(row)): a fragment's 16-byte reads
+//   LDS       a slab with k fast has rows of 128 or 64 bytes whose chunks are permuted by row (c ^ f(row)): a fragment's 16-byte reads
 //             then meet distinct banks (measured 8 clocks per 1 KB, the port's width).  B's rows are dealt to the fragments
 //             so that a lane ends with 6 neighbouring n and 16 neighbouring lanes with one row's 96: whole runs of 192 bytes
 //             leave with one store (per-lane 16-byte pieces of 16 rows cost 60 us more at 74750 x 800 -> 900).  A slab with
@@ -227,11 +227,12 @@ __device__ __forceinline__ float act_value(float z) {
     else if constexpr (ACT == HD_ACT_RELU) return z > 0.f ? z : (z == z ? 0.f : z);
     else return z;
 }
+// g * act'(z).  ReLU selects: an infinite g under a closed unit leaves 0, and a NaN z passes g on
 template <int ACT>
-__device__ __forceinline__ float act_slope(float z) {
-    if constexpr (ACT == HD_ACT_GELU) return gelu16_slope(z);
-    else if constexpr (ACT == HD_ACT_RELU) return z > 0.f ? 1.f : 0.f;
-    else return 1.f;
+__device__ __forceinline__ float through_act(float g, float z) {
+    if constexpr (ACT == HD_ACT_GELU) return g * gelu16_slope(z);
+    else if constexpr (ACT == HD_ACT_RELU) return z <= 0.f ? 0.f : g;
+    else return g;
 }
 
 // The pre-activation as it is kept for the backward pass: in fp16 for bf16 operands too, whose own 8 bits would add a third of dz's
@@ -349,7 +350,7 @@ __device__ __forceinline__ void tile_item(const Prod& g, int vid, char* lds) {
     const int k0 = (slice * g.slabs + (slice < g.slabs_rem ? slice : g.slabs_rem)) * BK;
     SA sa;
     SB sb;
-    sa.init((const T*)g.A, g.lda, m0, g.M, k0, g.K, tid);
+    sa.init((const T*)g.A, g.lda, m0, TR ? (g.M + 7) / 8 * 8 : g.M, k0, g.K, tid);   // TR: dz, whose rows are whole chunks
     sb.init((const T*)g.B, g.ldb, n0, g.N, k0, g.K, tid);
     const int wm = (wave >> 1) * WM, wn = (wave & 1) * WN;
     f32x4 acc[FI][FJ];
@@ -572,13 +573,13 @@ __device__ __forceinline__ void dz_rows(const T* __restrict__ g, long long ldg, 
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 float d = (float)a[u].v[e];
-                if constexpr (ACT != HD_ACT_IDENTITY) d *= act_slope<ACT>((float)b[u].v[e]);
+                if constexpr (ACT != HD_ACT_IDENTITY) d = through_act<ACT>(d, (float)b[u].v[e]);
                 s[e] += d;
                 o.v[e] = (T)d;
             }
             if (dz) {
                 T* out = dz + (long long)(m + u * slots) * lddz + n;
-                store_pack<T, 8>(out, o);                                     // not WIDE: 0 * slope(0) = 0 behind N
+                store_pack<T, 8>(out, o);                                     // not WIDE: g = z = 0 behind N, so dz = 0
                 for (int e = 0; e < pads; ++e) out[8 + e] = (T)0.f;
             }
         }
@@ -819,7 +820,7 @@ bool known_act(int a) { return a == HD_ACT_IDENTITY || a == HD_ACT_RELU || a == 
 #define HD_LINEAR_SHAPE(fn)                                                                                                     \
     HD_REQUIRE(dtype == HD_DT_BF16 || dtype == HD_DT_F16, fn ": element type bf16 or fp16, not %d", dtype);                      \
     HD_REQUIRE(known_act(act), fn ": activation identity, relu or gelu, not %d", act);                                          \
-    HD_REQUIRE(M >= 0 && M < (1LL << 30) && N >= 1 && N < (1LL << 22) && K >= 1 && K < (1LL << 22), fn ": bad shape");             \
+    HD_REQUIRE(M >= 0 && M < (1LL << 29) && N >= 1 && N < (1LL << 22) && K >= 1 && K < (1LL << 22), fn ": bad shape");             \
     HD_REQUIRE(ldx >= K && ldw >= K, fn ": row pitch below the width")
 
 template <typename T>
@@ -883,7 +884,7 @@ extern "C" int hd_linear_act_fwd(const void* x, int64_t ldx, const void* w, int6
     HD_REQUIRE(!resid || ldr >= 0, "hd_linear_act_fwd: negative pitch");
     HD_REQUIRE((((uintptr_t)x | (uintptr_t)w | (uintptr_t)y | (uintptr_t)z | (uintptr_t)bias | (uintptr_t)resid) & 1) == 0,
                "hd_linear_act_fwd: pointer not aligned to the element");
-    HD_REQUIRE(tiles_of(M, N, 32, 32) < (1LL << 31) - 8, "hd_linear_act_fwd: too many tiles");
+    HD_REQUIRE(tiles_of(M, N, 64, 64) < (1LL << 24) - 8, "hd_linear_act_fwd: too many tiles");   // a grid holds 2^32 threads
     Prod g = {};
     g.A = x; g.lda = ldx; g.B = w; g.ldb = ldw; g.M = (int)M; g.N = (int)N; g.K = (int)K;
     g.C = y; g.bias = bias; g.resid = resid; g.ldr = ldr; g.z = z; g.act = act;
@@ -894,7 +895,7 @@ extern "C" int hd_linear_act_fwd(const void* x, int64_t ldx, const void* w, int6
 }
 
 extern "C" int64_t hd_linear_act_bwd_workspace_bytes(int64_t M, int64_t N, int64_t K, int act) {
-    if (M < 0 || N < 1 || K < 1 || M >= (1LL << 30) || N >= (1LL << 22) || K >= (1LL << 22) || !known_act(act)) return 0;
+    if (M < 0 || N < 1 || K < 1 || M >= (1LL << 29) || N >= (1LL << 22) || K >= (1LL << 22) || !known_act(act)) return 0;
     return bwd_plan(M, N, K).bytes;
 }
 
@@ -914,7 +915,7 @@ extern "C" int hd_linear_act_bwd(const void* g, int64_t ldg, const void* z, cons
     const BwdPlan p = bwd_plan(M, N, K);
     HD_REQUIRE(workspace_bytes >= p.bytes, "hd_linear_act_bwd: workspace of %lld bytes required, got %lld", (long long)p.bytes,
                (long long)workspace_bytes);
-    HD_REQUIRE(tiles_of(M, K, 32, 32) < (1LL << 31) - 8 && tiles_of(N, K, 32, 32) < (1LL << 30) && N * K < (1LL << 38),
+    HD_REQUIRE(tiles_of(M, K, 64, 64) < (1LL << 24) - 8 && tiles_of(N, K, 32, 32) < (1LL << 23),
                "hd_linear_act_bwd: too many tiles");
     unsigned char* ws = (unsigned char*)workspace;
     hipStream_t s = (hipStream_t)st;

@@ -144,7 +144,7 @@ def test_captured_training_step(dtype, state_bits):
         half = HALF.get(dtype, 2.0 ** -24)
         for p, q in zip(a.parameters(), b.parameters()):
             d = (p.double() - q.double()).norm() / q.double().norm()
-            assert float(d) <= 4 * (k + 1) * half + 1e-3 * 0.05 * (k + 1), float(d)
+            assert float(d.detach()) <= 4 * (k + 1) * half + 1e-3 * 0.05 * (k + 1), float(d.detach())
 
 
 @gpu

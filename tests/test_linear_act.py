@@ -125,6 +125,15 @@ def test_sizes(M, N, K, dtype):
     _run(M, N, K, dtype, ("gelu", "relu", "identity")[k % 3], k % 4 != 3, k % 2 == 0, k)
 
 
+# outputs narrower than a chunk beside inputs that have to be staged through registers; few and many rows
+@gpu
+@pytest.mark.parametrize("M,N,K", [(50, 5, 13), (3000, 1, 41), (9000, 7, 129), (700, 3, 515), (1, 6, 9)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_narrow_outputs_of_odd_inputs(M, N, K, dtype):
+    _run(M, N, K, dtype, "relu", True, False, 21)
+    _run(M, N, K, dtype, "identity", True, True, 22)
+
+
 @gpu
 @pytest.mark.parametrize("act", ["gelu", "relu", "identity"])
 @pytest.mark.parametrize("bias,resid", [(False, False), (True, True)])
@@ -209,7 +218,7 @@ def test_large_and_tiny_preactivations_keep_their_slope(act):
     dx = torch.autograd.grad(y, [x], torch.ones(7, 8, device="cuda", dtype=torch.bfloat16))[0].flatten().tolist()
     small = (0.5, 0.5) if act == "gelu" else (1.0, 0.0)
     assert dx == [8.0, 8.0, 8.0, 8 * small[0], 8 * small[1], 0.0, 0.0]
-    assert torch.equal(y[:3, 0], x.detach()[:3, 0]) and float(y[5:].abs().max()) == 0.0
+    assert torch.equal(y[:3, 0], x.detach()[:3, 0]) and float(y.detach()[5:].abs().max()) == 0.0
 
 
 @gpu
@@ -229,6 +238,39 @@ def test_nonfinite_values_stay_in_their_row_and_column(K):
     hit[:, 139] = True
     assert bool(torch.isnan(got[149]).all()) and bool(torch.isnan(got[:, 139]).all())
     assert torch.equal(got[~hit], clean[~hit])
+
+
+@gpu
+@pytest.mark.parametrize("act", ["relu", "identity"])
+def test_nonfinite_gradients(act):
+    """an infinite gradient stays in its row; behind a closed ReLU it is gone; a NaN pre-activation passes the gradient on"""
+    from hypdiff_amd import ops
+    x = torch.tensor([[-1.0], [1.0], [1.0], [float("nan")]], device="cuda", dtype=torch.bfloat16, requires_grad=True)
+    w = torch.ones(9, 1, device="cuda", dtype=torch.bfloat16)
+    g = torch.ones(4, 9, device="cuda", dtype=torch.bfloat16)
+    g[0, 2] = g[1, 3] = float("inf")
+    dx = torch.autograd.grad(ops.linear_act(x, w, act=act), [x], g)[0].flatten().tolist()
+    assert dx == [0.0 if act == "relu" else float("inf"), float("inf"), 9.0, 9.0]
+
+
+@gpu
+def test_offsets_beyond_32_bits():
+    """x and dx of 4.4 GB: the last rows come out like the formula's, and dW sees them (all others are zeros)"""
+    from hypdiff_amd import ops
+    gen = _gen(15)
+    M, N, K, last = (1 << 22) + 3, 8, 520, 5
+    x = torch.zeros(M, K, device="cuda", dtype=torch.bfloat16)
+    x[-last:] = torch.randn(last, K, device="cuda", generator=gen).bfloat16()
+    w = (torch.randn(N, K, device="cuda", generator=gen) / math.sqrt(K)).bfloat16().requires_grad_(True)
+    g = torch.randn(M, N, device="cuda", generator=gen).bfloat16()
+    x.requires_grad_(True)
+    y = ops.linear_act(x, w, act="gelu")
+    dx, dw = torch.autograd.grad(y, [x, w], g)
+    d = lambda t: t.detach()[-last:].double()  # noqa: E731
+    want = _reference(d(x), w.detach().double(), None, None, d(g), "gelu", torch.bfloat16)
+    _check(y[-last:], *want["y"], "y")
+    _check(dx[-last:], *want["dx"], "dx")
+    _check(dw, *want["dw"], "dw")
 
 
 @gpu
