@@ -30,6 +30,7 @@ constexpr int kSmallRows = 4096;                    // rows that one workgroup s
 constexpr int kSortWg = 1024;
 constexpr int kMaxSortWgs = 256;
 constexpr int kZeroRows = 64;                       // table rows of one zero-writing workgroup
+constexpr int64_t kLookupRows = 1 << 25;            // rows of one lookup launch: a grid holds 2^32 threads
 
 // ---- lookup ---------------------------------------------------------------------------------------------------------------
 template <typename T, int VEC, typename I>
@@ -485,10 +486,13 @@ void lookup_any(const T* table, int64_t ldt, const I* idx, const T* add, int64_t
     const int vec = pick_vec(dim, MOST);
     const int64_t used = (dim + vec - 1) / vec;
     const int l2 = used >= 64 ? 6 : ceil_log2(used);
-    const unsigned wgs = (unsigned)((rows + (256 >> l2) - 1) / (256 >> l2));
     auto go = [&](auto tag) {
         constexpr int VEC = decltype(tag)::value;
-        lookup_k<T, VEC, I><<<wgs, 256, 0, st>>>(table, ldt, idx, add, lda, scale, n_table, rows, (int)dim, l2, out);
+        for (int64_t r = 0; r < rows; r += kLookupRows) {
+            const int64_t n = rows - r < kLookupRows ? rows - r : kLookupRows;
+            lookup_k<T, VEC, I><<<(unsigned)((n + (256 >> l2) - 1) / (256 >> l2)), 256, 0, st>>>(
+                table, ldt, idx + r, add ? add + r * lda : nullptr, lda, scale, n_table, n, (int)dim, l2, out + r * dim);
+        }
     };
     if constexpr (MOST == 8) {
         if (vec == 8) return go(std::integral_constant<int, 8>{});
@@ -543,7 +547,8 @@ extern "C" int hd_embedding_sum(const void* g, int64_t ldg, const void* idx, int
     const Plan p = make_plan(rows, dim, T, dtype);
     HD_REQUIRE(workspace_bytes >= p.bytes, "hd_embedding_sum: workspace of %lld bytes required, got %lld", (long long)p.bytes,
                (long long)workspace_bytes);
-    HD_REQUIRE(p.chunks * ((dim + 255) / 256) < (1LL << 31) && p.chunks * p.tiles + T / kZeroRows < (1LL << 31) - 256,
+    HD_REQUIRE(p.chunks * (dim < 4 ? 1 : (dim + 255) / 256) < (1LL << 24) &&
+                   ((p.chunks * p.tiles) >> (8 - p.log2_lanes)) + T / kZeroRows < (1LL << 24) - 2,                // a grid holds 2^32 threads
                "hd_embedding_sum: too many workgroups");
     hipStream_t s = (hipStream_t)st;
     unsigned char* ws = (unsigned char*)workspace;

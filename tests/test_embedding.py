@@ -167,6 +167,53 @@ def test_captured_and_replayed_with_new_indices():
 
 
 @gpu
+def test_two_streams_at_once():
+    from hypdiff_amd import ops
+    sets = [(torch.randint(0, 300, (20000,), device="cuda", generator=_gen(k)), torch.randn(300, 96, device="cuda", generator=_gen(k + 2)),
+             torch.randn(20000, 96, device="cuda", generator=_gen(k + 4))) for k in range(2)]
+
+    def step(idx, table, g):
+        t = table.detach().requires_grad_(True)
+        y = ops.embedding(idx, t)
+        return y.detach(), torch.autograd.grad(y, [t], g)[0]
+    want = [step(*s) for s in sets]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in sets], []
+    for st, s in zip(streams, sets):
+        with torch.cuda.stream(st):
+            got.append([step(*s) for _ in range(5)])
+    torch.cuda.synchronize()
+    for outs, w in zip(got, want):
+        for o in outs:
+            assert all(torch.equal(a, c) for a, c in zip(o, w))
+
+
+@gpu
+def test_offsets_beyond_32_bits():
+    """a result and a gradient of 4.4 GB (many rows), then a table of that size (many tokens)"""
+    from hypdiff_amd import ops
+    rows, T, D = (1 << 22) + 7, 5, 520
+    table = torch.randn(T, D, device="cuda", generator=_gen(40)).bfloat16().requires_grad_(True)
+    idx = torch.arange(rows, device="cuda") % T
+    g = torch.zeros(rows, D, device="cuda", dtype=torch.bfloat16)
+    g[-3:] = torch.randn(3, D, device="cuda", generator=_gen(41)).bfloat16()
+    y = ops.embedding(idx, table)
+    assert torch.equal(y[-300:], table.detach()[idx[-300:]])
+    gt = torch.autograd.grad(y, [table], g)[0]
+    want = torch.zeros(T, D, device="cuda", dtype=torch.bfloat16)
+    want[idx[-3:]] = g[-3:]                              # one row a token, zeros besides: no rounding
+    assert torch.equal(gt, want)
+    del y, g
+    table = torch.randn(rows, D, device="cuda", dtype=torch.bfloat16).requires_grad_(True)
+    idx = torch.arange(rows - 300, rows, device="cuda", dtype=torch.int32)
+    g = torch.randn(300, D, device="cuda", generator=_gen(42)).bfloat16()
+    y = ops.embedding(idx, table)
+    assert torch.equal(y, table.detach()[-300:])
+    gt = torch.autograd.grad(y, [table], g)[0]
+    assert torch.equal(gt[-300:], g) and not bool(gt[:-300].any())
+
+
+@gpu
 def test_agrees_with_the_fp32_embedding_of_the_backbone():
     from hypdiff_amd import autograd as hag, ops
     g = _gen(8)
