@@ -295,7 +295,7 @@ extern "C" int hd_adamw_step(const hd_adamw_job* jobs, int n_jobs, int dtype, in
         j.row[k] = (int)jobs[i].row;
         j.wg0[k] = (unsigned)wgs;
         wgs += (uint64_t)(jobs[i].count + kWgElems - 1) / kWgElems;
-        HD_REQUIRE(wgs < (1ULL << 31), "hd_adamw_step: too many elements in one call");
+        HD_REQUIRE(wgs < (1ULL << 24), "hd_adamw_step: too many elements in one call");      // a grid holds 2^32 threads
     }
     if (j.n == 0) return HD_OK;
     HD_REQUIRE(exp_avg && exp_avg_sq && (state_bits == 32 || (exp_avg_scale && exp_avg_sq_scale)), "hd_adamw_step: null state");

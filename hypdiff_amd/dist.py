@@ -74,8 +74,9 @@ def allreduce_moments(m, group=None):
 
 
 class GradBucket:
-    """All gradients of a module as ONE flat buffer in fp32 -- or in bf16 / fp16 where all parameters are -- (2.8 M elements for the mlp denoiser at
-    D=512 ~ 11 MB; 6.4 M ~ 25 MB for ddpm.Backbone).
+    """All gradients of a module as ONE flat buffer (2.8 M elements for the mlp denoiser at D=512 ~ 11 MB; 6.4 M ~ 25 MB for
+    ddpm.Backbone), in fp32, or in bf16 / fp16 where all parameters are: ranks then exchange half the bytes, and each
+    addition of the reduction rounds like the gradients themselves are rounded.
 
     The buffer is reduced in a few large chunks rather than per parameter -- xGMI links are
     point-to-point, so a ring all-reduce is per-link bound and few large messages beat many small

@@ -43,9 +43,20 @@ class _Flat:
                 self.buffers[k] = torch.zeros(at, dtype=torch.uint8, device=dev).view(torch.float8_e4m3fn)
                 self.buffers[k + "_scale"] = torch.zeros(at // BLOCK, dtype=torch.float32, device=dev)
         if self.with_master:
-            m = self.buffers["master"] = torch.zeros(at, dtype=torch.float32, device=dev)
-            torch._foreach_copy_([m[a:a + n] for a, n in zip(self.first, self.numels)],
-                                 [p.detach().reshape(-1) for p in self.params])
+            self.buffers["master"] = torch.zeros(at, dtype=torch.float32, device=dev)
+            self.take_masters()
+
+    def take_masters(self):
+        m = self.buffers["master"]
+        torch._foreach_copy_([m[a:a + n] for a, n in zip(self.first, self.numels)], [p.detach().reshape(-1) for p in self.params])
+
+    def clear(self):
+        """as before the first step, in the same memory"""
+        for k, b in self.buffers.items():
+            (b.view(torch.uint8) if b.dtype == torch.float8_e4m3fn else b).zero_()
+        if self.with_master:
+            self.take_masters()
+        self.set_steps([0] * len(self.params))
 
     def view(self, key, i):
         """parameter i's part of a buffer: its shape, or one value per block for the scales"""
@@ -85,7 +96,7 @@ class AdamW(torch.optim.Optimizer):
     Sparse, complex and fp64 parameters, lr as a tensor, amsgrad and maximize are not offered.  A parameter whose gradient
     is None is skipped and does not count the step.  Inside a captured HIP graph the step count lives on the device, so a
     replay has the right bias corrections; lr and the other options are the captured ones.  Run one step (or load a state)
-    before the capture.  state_dict / load_state_dict keep the state's own types; with state_bits=32 a state saved by
+    before the capture; a state loaded later goes into the same arrays, and replays continue from it.  state_dict / load_state_dict keep the state's own types; with state_bits=32 a state saved by
     torch.optim.AdamW loads."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32, master_weights=False):
@@ -130,12 +141,14 @@ class AdamW(torch.optim.Optimizer):
             if torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("AdamW: the state does not exist yet: run one step or load a state before capturing a graph")
             fl = self._flats[gi] = _Flat(group)
-            for i, p in enumerate(fl.params):
-                # an fp32 parameter is its own master
-                fl.states.append(self.state[p])
-                fl.states[-1].update({"step": 0, **{k: fl.view(k, i) for k in fl.buffers
-                                                      if k != "master" or p.dtype != torch.float32}})
+            self._link(fl)
         return fl
+
+    def _link(self, fl):
+        fl.states = [self.state[p] for p in fl.params]
+        for i, (p, st) in enumerate(zip(fl.params, fl.states)):
+            # an fp32 parameter is its own master
+            st.update({"step": fl.steps[i], **{k: fl.view(k, i) for k in fl.buffers if k != "master" or p.dtype != torch.float32}})
 
     def state_buffers(self, group=0):
         """The flat state arrays of a parameter group, the ones that the step updates: exp_avg, exp_avg_sq (fp32), or exp_avg,
@@ -263,45 +276,74 @@ class AdamW(torch.optim.Optimizer):
         return super().state_dict()
 
     def load_state_dict(self, state_dict):
-        saved = state_dict["state"]
-        ids = [i for g in state_dict["param_groups"] for i in g["params"]]
-        mine = [p for g in self.param_groups for p in g["params"]]
-        options = [{k: g[k] for k in _OPTIONS} for g in self.param_groups]
-        super().load_state_dict({**state_dict, "state": {}})
-        for g, o in zip(self.param_groups, options):
-            for k in _OPTIONS:
-                g.setdefault(k, o[k])                     # a state saved by torch.optim.AdamW has no state_bits
-            self._check_options(g)
+        saved, groups = state_dict["state"], state_dict["param_groups"]
+        if len(groups) != len(self.param_groups) or any(len(a["params"]) != len(b["params"]) for a, b in zip(groups, self.param_groups)):
+            raise ValueError("AdamW: the saved state has other parameter groups")
+        # a state saved by torch.optim.AdamW has no state_bits.  Everything is looked at before anything changes
+        options = [{k: g.get(k, mine[k]) for k in _OPTIONS} for g, mine in zip(groups, self.param_groups)]
+        for gi, (g, mine, opt) in enumerate(zip(groups, self.param_groups, options)):
+            self._check_options(opt)
             if g.get("amsgrad") or g.get("maximize"):
                 raise ValueError("AdamW: the saved options ask for amsgrad or maximize, which are not offered")
-        self._flats = {}
-        at = 0
-        for gi, group in enumerate(self.param_groups):
-            part, at = list(zip(ids[at:], mine[at:]))[:len(group["params"])], at + len(group["params"])
-            if not any(pid in saved for pid, _ in part):
-                continue
-            fl = self._flat(gi)
+            if self._captured(gi) and not self._keeps(gi, opt):
+                raise RuntimeError("AdamW: a captured step updates this state; state_bits and master_weights cannot change under it")
+            for pid, p in zip(g["params"], mine["params"]):
+                if saved.get(pid):
+                    self._check_saved(saved[pid], p, opt)
+        # and copied before anything is overwritten: the saved state may be this optimizer's own
+        parts = [[saved.get(pid) and {k: v.detach().clone() if torch.is_tensor(v) and k != "step" else int(v) if k == "step" else v
+                                      for k, v in saved[pid].items()} for pid in g["params"]] for g in groups]
+        super().load_state_dict({**state_dict, "state": {}})
+        for gi, (mine, opt, part) in enumerate(zip(self.param_groups, options, parts)):
+            mine.update(opt)
+            if not self._keeps(gi, opt) or not (any(part) or self._captured(gi)):
+                self._flats.pop(gi, None)
+                if not any(part):
+                    continue                              # made anew at the next step
+            if gi in self._flats:
+                fl = self._flats[gi]                      # the arrays stay where they are: a captured step names them
+                fl.clear()
+                self._link(fl)
+            else:
+                fl = self._flat(gi)
             steps, to, frm = list(fl.steps), [], []
-            for i, (pid, p) in enumerate(part):
-                st = saved.get(pid)
+            for i, (st, p) in enumerate(zip(part, fl.params)):
                 if not st:
                     continue
                 for k in fl.buffers:
                     if k == "master" and (k not in st or p.dtype == torch.float32):
-                        continue                          # taken from the parameter when the flat state was made
-                    if k not in st:
-                        raise ValueError(f"AdamW: the saved state has no {k} (state_bits={fl.bits})")
+                        continue                          # taken from the parameter
                     dst, src = fl.view(k, i), st[k]
-                    if src.numel() != dst.numel():
-                        raise ValueError(f"AdamW: the saved {k} has {src.numel()} elements, not {dst.numel()}")
-                    if (src.dtype == torch.float8_e4m3fn) != (dst.dtype == torch.float8_e4m3fn):
-                        raise ValueError(f"AdamW: the saved {k} is {src.dtype}, not {dst.dtype}")
                     if dst.dtype == torch.float8_e4m3fn:
                         dst, src = dst.view(torch.uint8), src.view(torch.uint8)
                     to.append(dst)
                     frm.append(src.detach().to(dst.device).reshape(dst.shape))
-                steps[i] = int(st["step"])
+                steps[i] = st["step"]
             if to:
                 with torch.no_grad():
                     torch._foreach_copy_(to, frm)
             fl.set_steps(steps)
+
+    def _captured(self, gi):
+        return gi in self._flats and self._flats[gi].device_count
+
+    def _keeps(self, gi, opt):
+        fl = self._flats.get(gi)
+        return fl is not None and (fl.bits, fl.with_master) == (int(opt["state_bits"]), bool(opt["master_weights"]))
+
+    @staticmethod
+    def _check_saved(st, p, opt):
+        n, bits = p.numel(), int(opt["state_bits"])
+        blocks = (n + BLOCK - 1) // BLOCK
+        want = {"exp_avg": n, "exp_avg_sq": n} if bits == 32 else \
+            {"exp_avg": n, "exp_avg_sq_root": n, "exp_avg_scale": blocks, "exp_avg_sq_root_scale": blocks}
+        if opt["master_weights"] and p.dtype != torch.float32 and "master" in st:
+            want["master"] = n
+        for k, count in want.items():
+            if k not in st:
+                raise ValueError(f"AdamW: the saved state has no {k} (state_bits={bits})")
+            if st[k].numel() != count:
+                raise ValueError(f"AdamW: the saved {k} has {st[k].numel()} elements, not {count}")
+            codes = bits == 8 and k in ("exp_avg", "exp_avg_sq_root")
+            if (st[k].dtype == torch.float8_e4m3fn) != codes:
+                raise ValueError(f"AdamW: the saved {k} is {st[k].dtype}, not {torch.float8_e4m3fn if codes else torch.float32}")

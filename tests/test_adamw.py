@@ -271,6 +271,24 @@ def test_loads_a_state_of_torchs_adamw():
 
 
 @gpu
+def test_offsets_beyond_32_bits():
+    """a tensor of 2^32 + 300 elements, alike everywhere: every element takes the step that a small tensor's take"""
+    from hypdiff_amd.optim import AdamW
+    out = []
+    for n in ((1 << 32) + 300, 300):
+        p = torch.nn.Parameter(torch.full((n,), 0.5, device="cuda", dtype=torch.bfloat16))
+        p.grad = torch.full((n,), -0.25, device="cuda", dtype=torch.bfloat16)
+        opt = AdamW([p], state_bits=8, **H)
+        opt.step()
+        opt.step()
+        out.append((p.detach(), opt.state_buffers()["exp_avg"].view(torch.uint8)[:n]))
+    for big, small in zip(*out):
+        assert bool((small == small[0]).all()) and float(small[0]) != 0.5
+        for k in range(0, big.numel(), 1 << 30):
+            assert bool((big[k:k + (1 << 30)] == small[0]).all())
+
+
+@gpu
 @pytest.mark.parametrize("bits", [32, 8])
 def test_captured_step_counts_on_the_device(bits):
     from hypdiff_amd.optim import AdamW
@@ -296,6 +314,62 @@ def test_captured_step_counts_on_the_device(bits):
                 assert torch.equal(o1.state[p][name].view(torch.uint8), o2.state[q][name].view(torch.uint8)), name
     o1.step()                                             # eager again: the device's count goes on
     assert o1.state_dict()["state"][0]["step"] == 6
+
+
+@gpu
+@pytest.mark.parametrize("bits,dtype,master", [(32, torch.float32, False), (8, torch.bfloat16, True)])
+def test_a_state_loaded_after_a_capture_is_the_one_that_replays_continue(bits, dtype, master):
+    from hypdiff_amd.optim import AdamW
+    a, b = _params(dtype, seed=8), _params(dtype, seed=8)
+    make = lambda ps: AdamW(ps, state_bits=bits, master_weights=master, **H)  # noqa: E731
+    o1, o2 = make(a), make(b)
+    o1.step()
+    o2.step()
+    sd, weights = copy.deepcopy(o2.state_dict()), [p.detach().clone() for p in b]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        o1.step()
+    for _ in range(3):
+        graph.replay()
+        o1.replayed()
+    with torch.no_grad():
+        for p, w in zip(a, weights):
+            p.copy_(w)
+    o1.load_state_dict(sd)
+    junk = torch.full((1 << 22,), 7.0, device="cuda")     # would land in memory that the load had let go of
+    assert o1.state_dict()["state"][0]["step"] == 1
+    for k in range(2):
+        graph.replay()
+        o1.replayed()
+        o2.step()
+        for p, q in zip(a, b):                            # as test_captured_step_counts_on_the_device; 16-bit: half a step more
+            u = torch.finfo(p.dtype).eps if p.dtype != torch.float32 else 0.0
+            tol = (8 * 2.0 ** -24 * (k + 1) + u) * torch.clamp(p.abs(), min=H["lr"] * 8).double()
+            assert torch.all((p.double() - q.double()).abs() <= tol)
+            for name in (x for x in o1.state[p] if x not in ("step", "master")):
+                assert torch.equal(o1.state[p][name].view(torch.uint8), o2.state[q][name].view(torch.uint8)), name
+    assert torch.all(junk == 7.0)
+    with pytest.raises(RuntimeError, match="captured"):
+        o1.load_state_dict(AdamW(b, state_bits=40 - bits, **H).state_dict())
+
+
+@gpu
+def test_loading_its_own_state_changes_nothing_and_a_refused_state_neither():
+    from hypdiff_amd.optim import AdamW
+    a = _params(torch.bfloat16, seed=9)
+    opt = AdamW(a, state_bits=8, master_weights=True, **H)
+    opt.step()
+    opt.step()
+    before = {k: v.view(torch.uint8).clone() for k, v in opt.state_buffers().items()}
+    opt.load_state_dict(opt.state_dict())
+    broken = copy.deepcopy(opt.state_dict())
+    del broken["state"][len(a) - 1]["exp_avg_scale"]
+    with pytest.raises(ValueError, match="exp_avg_scale"):
+        opt.load_state_dict(broken)
+    for k, v in opt.state_buffers().items():
+        assert torch.equal(v.view(torch.uint8), before[k]), k
+    assert all(opt.state[p]["step"] == 2 for p in a)
 
 
 def test_refusals_on_the_host():
