@@ -12,9 +12,10 @@
 // also writes), dW (A = dz, B = x, both with k -- the rows of the batch -- as the slow index).
 //
 //   tiles     128 x 192, 128 x 128, 64 x 128 or 64 x 64 of 4 wavefronts, by a cost model (choose_tiles); 32 x 32 with the
-//             contraction split over the wavefronts for few rows (small_gemm); dW 192 x 192 or 64 x 64 (dw_plan).  One slab of 64 k in LDS, not two: a workgroup
-//             waits for its loads, and the 3 to 8 that fit a CU because of it multiply meanwhile (74750 x 800 -> 900: 137 us with
-//             three workgroups of one buffer, 165 with two, 173 with two of two buffers).
+//             contraction split over the wavefronts for few rows (small_gemm); dW 192 x 192 or 64 x 64 (dw_plan).  One slab of 64 k in LDS,
+//             not two: a workgroup waits for its loads, and the 3 to 8 that fit a CU because of it multiply meanwhile.  Two
+//             slabs, the next one's loads in flight during the multiplies, are no faster at any size (74750 x 800 -> 900: 128 x 192
+//             146 us, with two 155; 128 x 128 158 and 175; 4096 x 800 -> 900: 14.1 and 14.2 at 64 x 128), three slower.
 //   staging   16-byte chunks go from memory to LDS without passing registers where every row starts on a 16-byte border and
 //             holds whole chunks; otherwise (an odd width, a sliced matrix) through registers, with the tail masked.  Chunks
 //             beyond the contraction's end come from a page of zeros, rows and columns beyond the matrix from a valid one
