@@ -5,6 +5,7 @@ enqueues HIP kernels of libhypdiff_hip.so on the current stream and returns with
 synchronising.  Inputs must live on the GPU; nothing here computes on the CPU.
 """
 import ctypes
+import functools
 import os
 import weakref
 
@@ -809,12 +810,15 @@ def linear_act(x, weight, bias=None, act="identity", resid=None):
     return _linear_act_fwd(x, weight, bias, resid, code, False)[0]
 
 
-def _matrix(t):
+# The helpers below run where autograd records nothing: inside LinearAct, or on operands that need no gradient.  For a small
+# layer the host's work is the time, so contiguous matrices take the short way through them.
+def _matrix(t, cols):
     """(t as a 2-D matrix with unit column stride and rows that do not overlap, its row pitch)"""
-    t = t.detach()
+    if t.is_contiguous():
+        return (t if t.dim() == 2 else t.reshape(-1, cols)), cols
     if t.dim() != 2:
-        t = t.reshape(-1, t.shape[-1])
-    rows, cols = t.shape
+        t = t.reshape(-1, cols)
+    rows = t.shape[0]
     pitch, step = t.stride()
     if (step != 1 and cols > 1) or (pitch < cols and rows > 1):
         t, pitch = t.contiguous(), cols
@@ -823,32 +827,40 @@ def _matrix(t):
 
 def _linear_act_fwd(x, w, b, resid, act, want_z):
     """(y, z or None, x as a matrix, its pitch, w as a matrix, its pitch)"""
-    x2, ldx = _matrix(x)
-    w2, ldw = _matrix(w)
-    M, (N, K) = x2.shape[0], w2.shape
-    y = x2.new_empty(x.shape[:-1] + (N,))
+    N, K = w.shape
+    x2, ldx = _matrix(x, K)
+    w2, ldw = _matrix(w, K)
+    M = x2.shape[0]
+    y = x2.new_empty((M, N) if x.dim() == 2 else x.shape[:-1] + (N,))
     z = x2.new_empty((M, N), dtype=torch.float16) if want_z else None
     if M:
-        r2, ldr = (None, 0) if resid is None else _pitched(resid.detach().reshape(M, N))
+        if resid is not None:
+            resid, ldr = (resid, N) if resid.is_contiguous() else _pitched(resid.reshape(M, N))
         if b is not None and not b.is_contiguous():
-            b = b.detach().contiguous()
+            b = b.contiguous()
         _lib.call("hd_linear_act_fwd", x2.data_ptr(), ldx, w2.data_ptr(), ldw, None if b is None else b.data_ptr(),
-                  None if r2 is None else r2.data_ptr(), ldr, DT_CODES[x2.dtype], M, N, K, act, y.data_ptr(),
-                  None if z is None else z.data_ptr(), raw_stream())
+                  None if resid is None else resid.data_ptr(), 0 if resid is None else ldr, DT_CODES[x2.dtype], M, N, K, act,
+                  y.data_ptr(), None if z is None else z.data_ptr(), raw_stream())
     return y, z, x2, ldx, w2, ldw
+
+
+@functools.lru_cache(maxsize=256)
+def _linear_act_bwd_bytes(M, N, K, act):
+    return _lib.load().hd_linear_act_bwd_workspace_bytes(M, N, K, act)
 
 
 def _linear_act_bwd(g, z, x2, w2, ldx, ldw, act, x_shape, skip, need_x, need_w, need_b):
     if not (g.get_device() == x2.get_device() == w2.get_device() == _cur_device()):
         _dev(g, x2, w2)                                   # says which one is elsewhere
-    g2, ldg = _matrix(g)
-    M, (N, K) = x2.shape[0], w2.shape
+    N, K = w2.shape
+    g2, ldg = _matrix(g, N)
+    M = x2.shape[0]
     new = x2.new_empty if M else x2.new_zeros
     dx = new(x_shape) if need_x else None
     dw = new((N, K)) if need_w else None
     db = new((N,)) if need_b else None
     if M:
-        nbytes = _lib.load().hd_linear_act_bwd_workspace_bytes(M, N, K, act)
+        nbytes = _linear_act_bwd_bytes(M, N, K, act)
         ws = x2.new_empty((nbytes,), dtype=torch.uint8)
         _lib.call("hd_linear_act_bwd", g2.data_ptr(), ldg, None if z is None else z.data_ptr(), x2.data_ptr(), ldx, w2.data_ptr(), ldw,
                   DT_CODES[x2.dtype], M, N, K, act, g2.data_ptr() if skip and need_x else None, ldg, None if dx is None else dx.data_ptr(),
