@@ -878,24 +878,29 @@ def embedding(idx, table, scale=1.0, add=None, padding_idx=None):
     the rows by token in a fixed order (the same bits on every run), in fp32, and is dense.  The row padding_idx gets no
     gradient (it is looked up like any other, as nn.Embedding does); an index outside [0, T) gives a row of NaN and no
     gradient.  The time embedding of ddpm.py:36-41 is embedding(idx, weight, add=h)."""
-    if table.dtype not in DT_CODES:
-        raise TypeError(f"embedding: a table in float32, bfloat16 or float16, not {table.dtype}")
-    if table.dim() != 2 or table.shape[0] < 1 or table.shape[1] < 1:
-        raise ValueError(f"embedding: a table of shape (T, D), not {tuple(table.shape)}")
-    if idx.dtype not in (torch.int32, torch.int64):
+    dt, ts, shape = table.dtype, table.shape, idx.shape
+    if dt not in DT_CODES:
+        raise TypeError(f"embedding: a table in float32, bfloat16 or float16, not {dt}")
+    if len(ts) != 2 or ts[0] < 1 or ts[1] < 1:
+        raise ValueError(f"embedding: a table of shape (T, D), not {tuple(ts)}")
+    if idx.dtype is not torch.int64 and idx.dtype is not torch.int32:
         raise TypeError(f"embedding: indices in int32 or int64, not {idx.dtype}")
+    dev = table.get_device()
+    same, grad = dev >= 0 and idx.get_device() == dev and dev == _cur_device(), table.requires_grad
     if add is not None:
-        if add.dtype != table.dtype:
-            raise TypeError(f"embedding: add is {add.dtype}, the table {table.dtype}")
-        if tuple(add.shape) != tuple(idx.shape) + (table.shape[1],):
-            raise ValueError(f"embedding: add has shape {tuple(add.shape)}, not {tuple(idx.shape) + (table.shape[1],)}")
+        if add.dtype is not dt:
+            raise TypeError(f"embedding: add is {add.dtype}, the table {dt}")
+        if add.shape != shape + ts[1:]:
+            raise ValueError(f"embedding: add has shape {tuple(add.shape)}, not {tuple(shape) + (ts[1],)}")
+        same, grad = same and add.get_device() == dev, grad or add.requires_grad
     if padding_idx is not None:
         if not -table.shape[0] <= padding_idx < table.shape[0]:
             raise ValueError(f"embedding: padding_idx {padding_idx} is outside a table of {table.shape[0]} rows")
         padding_idx = int(padding_idx) % table.shape[0]
     scale = float(scale)
-    _dev(table, idx, add)
-    if torch.is_grad_enabled() and (table.requires_grad or (add is not None and add.requires_grad)):
+    if not same:
+        _dev(table, idx, add)                             # says which one is elsewhere
+    if grad and torch.is_grad_enabled():
         from . import autograd as hag
         return hag.Embedding.apply(table, add, idx, scale, padding_idx)
     return _embedding_lookup(table, idx, scale, add)
@@ -910,28 +915,29 @@ def _pitched(x2):
 
 def _embedding_lookup(table, idx, scale, add):
     T, D = table.shape
-    tab, ldt = _pitched(table.detach())
-    ix = idx.reshape(-1)
-    ix = ix if ix.is_contiguous() else ix.contiguous()
-    a2, lda = (None, 0) if add is None else _pitched(add.detach().reshape(-1, D))
-    out = torch.empty(tuple(idx.shape) + (D,), dtype=table.dtype, device=table.device)
-    _lib.call("hd_embedding_lookup", _p(tab), ldt, _p(ix), ix.element_size() * 8, _p(a2), lda, scale, DT_CODES[table.dtype], T,
-              ix.numel(), D, _p(out), _stream())
+    tab, ldt = (table, D) if table.is_contiguous() else _pitched(table.detach())
+    ix = idx if idx.is_contiguous() else idx.contiguous()
+    lda = 0
+    if add is not None:
+        add, lda = (add, D) if add.is_contiguous() else _pitched(add.detach().reshape(-1, D))
+    out = tab.new_empty(idx.shape + (D,))
+    _lib.call("hd_embedding_lookup", tab.data_ptr(), ldt, ix.data_ptr(), 64 if ix.dtype is torch.int64 else 32,
+              None if add is None else add.data_ptr(), lda, scale, DT_CODES[table.dtype], T, ix.numel(), D, out.data_ptr(), raw_stream())
     return out
 
 
 def _embedding_sum(g, idx, T, scale, padding_idx):
     D = g.shape[-1]
-    _dev(g, idx)
-    g2, ldg = _pitched(g.detach().reshape(-1, D))
-    ix = idx.reshape(-1)
-    ix = ix if ix.is_contiguous() else ix.contiguous()
-    dt = DT_CODES[g.dtype]
-    nbytes = _lib.load().hd_embedding_sum_workspace_bytes(ix.numel(), D, T, dt)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=g.device)
-    out = torch.empty(T, D, dtype=g.dtype, device=g.device)
-    _lib.call("hd_embedding_sum", _p(g2), ldg, _p(ix), ix.element_size() * 8, -1 if padding_idx is None else padding_idx, scale,
-              dt, T, ix.numel(), D, _p(out), _p(ws), nbytes, _stream())
+    if not (g.get_device() == idx.get_device() == _cur_device()):
+        _dev(g, idx)                                      # says which one is elsewhere
+    g2, ldg = (g, D) if g.is_contiguous() else _pitched(g.detach().reshape(-1, D))
+    ix = idx if idx.is_contiguous() else idx.contiguous()
+    dt, rows = DT_CODES[g.dtype], ix.numel()
+    nbytes = _lib.load().hd_embedding_sum_workspace_bytes(rows, D, T, dt)
+    ws = g2.new_empty((nbytes,), dtype=torch.uint8)
+    out = g2.new_empty((T, D))
+    _lib.call("hd_embedding_sum", g2.data_ptr(), ldg, ix.data_ptr(), 64 if ix.dtype is torch.int64 else 32,
+              -1 if padding_idx is None else padding_idx, scale, dt, T, rows, D, out.data_ptr(), ws.data_ptr(), nbytes, raw_stream())
     return out
 
 
