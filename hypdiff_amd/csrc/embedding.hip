@@ -237,20 +237,17 @@ __global__ __launch_bounds__(256) void segment_sum_k(const T* __restrict__ g, lo
                                                      float scale, int chunk, int log2_lanes, int tiles, unsigned sum_wgs,
                                                      T* __restrict__ out, float* __restrict__ head, float* __restrict__ tail) {
     if (blockIdx.x >= sum_wgs) {                                              // zeros of the table rows that nothing names
-        __shared__ unsigned present[kZeroRows];
-        __shared__ unsigned range[2];
+        // a search for every row's first place: walking the keys of 64 rows instead takes one workgroup 90 us where 75 000 rows
+        // are one token's
+        __shared__ unsigned place[kZeroRows + 1];
         const unsigned t0 = (blockIdx.x - sum_wgs) * kZeroRows;
         const unsigned t1 = n_table - t0 < kZeroRows ? n_table : t0 + kZeroRows;
-        if (threadIdx.x < kZeroRows) present[threadIdx.x] = 0;
-        if (threadIdx.x < 2) range[threadIdx.x] = lower_bound(keys, n, threadIdx.x ? t1 : t0);
-        __syncthreads();
-        const unsigned a = range[0], b = range[1];
-        for (unsigned i = a + threadIdx.x; i < b; i += 256) present[keys[i] - t0] = 1;
+        if (threadIdx.x <= kZeroRows) place[threadIdx.x] = lower_bound(keys, n, t0 + threadIdx.x);
         __syncthreads();
         const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
         const float zero[VEC] = {};
         for (unsigned t = t0 + wave; t < t1; t += 4)
-            if (!present[t - t0])
+            if (place[t - t0] == place[t - t0 + 1])
                 for (int c = lane * VEC; c < dim; c += 64 * VEC)
                     store_row<T, VEC>(out + (long long)t * dim + (c + VEC <= dim ? c : dim - VEC), zero, 1.f);
         return;
