@@ -17,6 +17,8 @@ reduced in chunks as soon as the backward kernels have produced them (last layer
 GEMMs of the earlier layers still run; the tangent all-gather of slab k+1 is on the wire while
 slab k is aggregated.
 """
+import gc
+
 import numpy as np
 import torch
 import torch.distributed as dist
@@ -71,6 +73,19 @@ def allreduce_moments(m, group=None):
     if _collective(group):
         dist.all_reduce(m, op=dist.ReduceOp.SUM, group=group)
     return m
+
+
+def _in_a_live_graph(params):
+    """The parameters whose gradient node (AccumulateGrad) is alive, i.e. held by some graph.  A mark left on the node is
+    found again only if the node outlives the call that made it."""
+    def marked(p):
+        torch.autograd.graph.get_gradient_edge(p).node.metadata["hypdiff_live"] = True
+        return "hypdiff_live" in torch.autograd.graph.get_gradient_edge(p).node.metadata
+    live = [p for p in params if marked(p)]
+    if live:
+        gc.collect()                                  # a dropped graph may wait for the collector in a reference cycle
+        live = [p for p in live if marked(p)]
+    return live
 
 
 class GradBucket:
@@ -300,8 +315,9 @@ class DataParallelTrainer:
         launches of a few microseconds: 2.5 ms issued one by one, 1.3 ms of kernels).  Requirements: loss_fn reads
         the same device tensors on every call, draws its random numbers on the device (torch's CUDA generator is
         graph-safe; ddpm.Model does that while a capture is running), never reads anything back to the host; the
-        optimizer is BucketAdam or optim.AdamW (their step counts live on the device).  With more than one rank (backend nccl = RCCL) the
-        chunked gradient all-reduces are recorded into the graph as well -- they are stream operations -- so the graphed
+        optimizer is BucketAdam or optim.AdamW (their step counts live on the device); no tensor of an earlier eager pass that
+        still carries its autograd graph is alive (refused: the graph's nodes of the parameters are shared, with their stream).
+        With more than one rank (backend nccl = RCCL) the chunked gradient all-reduces are recorded into the graph as well -- they are stream operations -- so the graphed
         step survives data parallelism (every rank must capture and replay in lockstep).
         `warmup` eager steps run first on a side stream (allocations, caches).  The parameters' versions are bumped
         after every replay, as after an eager step."""
@@ -312,6 +328,11 @@ class DataParallelTrainer:
         from . import optim
         if not isinstance(self.opt, (BucketAdam, optim.AdamW)):
             raise TypeError("DataParallelTrainer.capture needs the BucketAdam optimizer or optim.AdamW (device-side step count)")
+        live = _in_a_live_graph(self.bucket.params)
+        if live:
+            raise RuntimeError(f"DataParallelTrainer.capture: {len(live)} parameters still belong to an autograd graph (an earlier loss or "
+                               "output that was kept without detach()): a captured backward pass would wait for that graph's "
+                               "stream.  Drop it first")
         side = torch.cuda.Stream()
         side.wait_stream(torch.cuda.current_stream())
         with torch.cuda.stream(side):

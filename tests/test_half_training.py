@@ -147,6 +147,34 @@ def test_captured_training_step(dtype, state_bits):
             assert float(d.detach()) <= 4 * (k + 1) * half + 1e-3 * 0.05 * (k + 1), float(d.detach())
 
 
+def test_live_graphs_are_found():
+    from hypdiff_amd.dist import _in_a_live_graph
+    p, q = torch.nn.Parameter(torch.randn(3)), torch.nn.Parameter(torch.randn(2))
+    p.register_post_accumulate_grad_hook(lambda t: None)
+    assert _in_a_live_graph([p, q]) == []
+    loss = (p * 2).sum()
+    assert [t is p for t in _in_a_live_graph([p, q])] == [True]
+    loss.backward()
+    assert len(_in_a_live_graph([p, q])) == 1            # the tensor still holds the node
+    kept = loss.detach()
+    ring = [loss]
+    ring.append(ring)                                    # dropped, but only the collector will see it
+    del loss, ring
+    assert _in_a_live_graph([p, q]) == [] and bool(torch.isfinite(kept))
+
+
+@gpu
+def test_capture_is_refused_while_an_eager_graph_lives():
+    model, tr = _trainer(32)
+    x, eps, idx = torch.randn(20, 64, device="cuda"), torch.randn(20, 64, device="cuda"), torch.zeros(20, dtype=torch.int64, device="cuda")
+    kept = model.loss_fn(x, idx=idx, epsilon=eps)
+    with pytest.raises(RuntimeError, match="autograd graph"):
+        tr.capture(lambda: model.loss_fn(x, idx=idx, epsilon=eps), warmup=1)
+    del kept
+    replay = tr.capture(lambda: model.loss_fn(x, idx=idx, epsilon=eps), warmup=1)
+    assert bool(torch.isfinite(replay()))
+
+
 @gpu
 def test_trainer_gives_16_bit_modules_masters():
     from hypdiff_amd import dist as hdist, optim
