@@ -95,7 +95,7 @@ class AdamW(torch.optim.Optimizer):
 
     Sparse, complex and fp64 parameters, lr as a tensor, amsgrad and maximize are not offered.  A parameter whose gradient
     is None is skipped and does not count the step.  Inside a captured HIP graph the step count lives on the device, so a
-    replay has the right bias corrections; lr and the other options are the captured ones.  Run one step (or load a state)
+    replay has the right bias corrections (state_dict reads it back); lr and the other options are the captured ones.  Run one step (or load a state)
     before the capture; a state loaded later goes into the same arrays, and replays continue from it.  state_dict / load_state_dict keep the state's own types; with state_bits=32 a state saved by
     torch.optim.AdamW loads."""
 
@@ -290,9 +290,11 @@ class AdamW(torch.optim.Optimizer):
             for pid, p in zip(g["params"], mine["params"]):
                 if saved.get(pid):
                     self._check_saved(saved[pid], p, opt)
-        # and copied before anything is overwritten: the saved state may be this optimizer's own
-        parts = [[saved.get(pid) and {k: v.detach().clone() if torch.is_tensor(v) and k != "step" else int(v) if k == "step" else v
-                                      for k, v in saved[pid].items()} for pid in g["params"]] for g in groups]
+        # and the saved state may be this optimizer's own: that is copied before it is overwritten
+        own = {b.untyped_storage().data_ptr() for fl in self._flats.values() for b in fl.buffers.values()}
+        kept = lambda v: v.detach().clone() if v.untyped_storage().data_ptr() in own else v.detach()  # noqa: E731
+        parts = [[saved.get(pid) and {k: int(v) if k == "step" else kept(v) if torch.is_tensor(v) else v for k, v in saved[pid].items()}
+                  for pid in g["params"]] for g in groups]
         super().load_state_dict({**state_dict, "state": {}})
         for gi, (mine, opt, part) in enumerate(zip(self.param_groups, options, parts)):
             mine.update(opt)
