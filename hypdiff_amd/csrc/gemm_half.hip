@@ -527,12 +527,12 @@ __global__ __launch_bounds__(256) void small_gemm(const Prod g) {
 }
 
 // dx by small_gemm and dW's slices by 64 x 64 tiles in one launch: with few rows neither fills the chip nor waits for the other
-template <typename T, bool DIRECT, int BK>
+template <typename T, bool DIRECT>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4))) void small_pair(const Prod dx, const Prod dw, int dx_wgs) {
-    constexpr int kTile = kTileLds<true, DIRECT, 64, 64, BK>;
+    constexpr int kTile = kTileLds<true, DIRECT, 64, 64, 64>;
     __shared__ __attribute__((aligned(1024))) char lds[kTile > kSmallLds ? kTile : kSmallLds];
     if ((int)blockIdx.x < dx_wgs) small_item<T>(dx, (int)blockIdx.x, lds);
-    else tile_item<T, true, DIRECT, 64, 64, BK>(dw, (int)blockIdx.x - dx_wgs, lds);
+    else tile_item<T, true, DIRECT, 64, 64, 64>(dw, (int)blockIdx.x - dx_wgs, lds);
 }
 
 // ---- dz = g * act'(z), the column sums of the unrounded products, and W^T ---------------------------------------------------------
@@ -714,7 +714,7 @@ inline void cut(Prod& g, int bm, int bn, int bk, int slices) {
 
 template <typename T, bool TR, int BM, int BN, int OCC>
 void launch_tiles(Prod g, int slices, bool direct, hipStream_t st) {
-    // slabs of 64 k; 32 where a slab passes through registers, which 64 would take from a resident workgroup
+    // slabs of 64 k; 32 where a slab of 192 x 192 passes through registers, of which 64 would need more than there are
     auto go = [&](auto bk, auto tag) {
         constexpr int BK = decltype(bk)::value;
         constexpr bool DIRECT = decltype(tag)::value;
@@ -723,7 +723,7 @@ void launch_tiles(Prod g, int slices, bool direct, hipStream_t st) {
         half_gemm<T, TR, DIRECT, BM, BN, BK, DIRECT ? OCC : 2><<<grid, 256, 0, st>>>(g);
     };
     if (direct) go(std::integral_constant<int, 64>{}, std::true_type{});
-    else go(std::integral_constant<int, 32>{}, std::false_type{});
+    else go(std::integral_constant<int, BM * BN <= 128 * 192 ? 64 : 32>{}, std::false_type{});
 }
 
 inline int64_t tiles_of(int64_t M, int64_t N, int64_t bm, int64_t bn) { return ((M + bm - 1) / bm) * ((N + bn - 1) / bn); }
@@ -732,7 +732,7 @@ inline int64_t tiles_of(int64_t M, int64_t N, int64_t bm, int64_t bn) { return (
 // 2048 x 512 x 512 12.1 against 7.9), up to 64 where rows start off 16-byte borders, whose fragments cost more loads (512 x 800 x
 // 513 16.8 against 9.7).  Above, the least of start + share of the chip per 256 tiles, fitted to K = 800 (bf16, GELU, us; the
 // times at 4096, 8192, 16384 and 74750 rows of 900); the small ones cost 3.6 and 5.4 where slabs pass through registers (7850 x
-// 800 x 513: 29.6 us in 64 x 128 tiles, 25.3 in 128 x 128):
+// 800 x 513: 27.0 us in 64 x 128 tiles, 23.1 in 128 x 128):
 //   1  64 x 64     6 + 2.85, at least 11      16.7   28.4   48.9   240
 //   2  64 x 128    6 + 4.6,  at least 13      15.1   24.5   42.9   179
 //   3  128 x 128   8 + 8.0,  at least 18      18.6   23.0   37.7   145
@@ -858,9 +858,9 @@ int linear_bwd(const T* g, int64_t ldg, const f16* z, const T* x, int64_t ldx, c
     if (dx && dw && !p.dw.large && choose_tiles(q.M, q.N, q.K, true) == 0) {
         const int dx_wgs = (int)tiles_of(M, K, 32, 32);
         q.tiles_n = (q.N + 31) / 32;
-        cut(v, 64, 64, direct ? 64 : 32, p.dw.slices);
-        if (direct) small_pair<T, true, 64><<<(unsigned)(dx_wgs + v.total), 256, 0, s>>>(q, v, dx_wgs);
-        else small_pair<T, false, 32><<<(unsigned)(dx_wgs + v.total), 256, 0, s>>>(q, v, dx_wgs);
+        cut(v, 64, 64, 64, p.dw.slices);
+        if (direct) small_pair<T, true><<<(unsigned)(dx_wgs + v.total), 256, 0, s>>>(q, v, dx_wgs);
+        else small_pair<T, false><<<(unsigned)(dx_wgs + v.total), 256, 0, s>>>(q, v, dx_wgs);
     } else {
         if (dx) launch_product<T>(q, true, s);
         if (dw && p.dw.large) launch_tiles<T, true, 192, 192, 2>(v, p.dw.slices, direct, s);
