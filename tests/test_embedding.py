@@ -167,6 +167,17 @@ def test_captured_and_replayed_with_new_indices():
 
 
 @gpu
+@pytest.mark.parametrize("rows", [511, 512, 513, 1024, 1025, 2049])
+def test_gradient_around_the_borders_of_the_sorts(rows):
+    from hypdiff_amd import ops
+    for T, kind in ((3, "any"), (70000, "hot"), (256, "one")):
+        idx = _idx(rows, T, kind, torch.int64, rows)
+        g = torch.randn(rows, 9, device="cuda", generator=_gen(rows + 1))
+        want, size = _grad64(idx, g, T, 0.5, None)
+        _check(ops._embedding_sum(g, idx, T, 0.5, None), want, size, torch.float32)
+
+
+@gpu
 def test_two_streams_at_once():
     from hypdiff_amd import ops
     sets = [(torch.randint(0, 300, (20000,), device="cuda", generator=_gen(k)), torch.randn(300, 96, device="cuda", generator=_gen(k + 2)),
