@@ -8,9 +8,10 @@
 //   sort    key = token (the padding token and tokens outside the table become T, behind all others), value = row.  Up to
 //           512 rows: one workgroup, bitonic on (key, row) in LDS, three launches fewer (the whole gradient of 200 rows 15.0 us,
 //           by radix 16.3; of 512 17.8 and 16.7 beside the host's part of the launches; of 4096 47 and 21).
-//           More: least-significant-digit radix passes of at most 8 bits; a workgroup counts its own digits' places from the counts of all workgroups (at most 256 of them, one
-//           read of 256 KB): two launches a pass.  (Counting the next pass's digits in the scatter, by atomics on the counts of the
-//           workgroup a row moves to, saved a launch of 3 us and cost 11: the rows of a hot token meet on one counter.)
+//           More: least-significant-digit radix passes of at most 8 bits; a workgroup counts its own digits' places from the
+//           counts of all workgroups (at most 256 of them, one read of 256 KB): two launches a pass.  (Counting the next
+//           pass's digits in the scatter, by atomics on the counts of the workgroup a row moves to, saved a launch of 3 us
+//           and cost 11: the rows of a hot token meet on one counter.)
 //   sum     the sorted rows are cut into chunks of P; a lane owns VEC columns, walks a chunk and writes a table row
 //           whenever a run ends.  A run that crosses a chunk's border leaves a partial sum there, which the next launch
 //           adds up in chunk order: a hot token (18 000 of 75 000 rows) is spread over hundreds of wavefronts.  Further
