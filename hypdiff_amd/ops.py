@@ -926,6 +926,11 @@ def _embedding_lookup(table, idx, scale, add):
     return out
 
 
+@functools.lru_cache(maxsize=256)
+def _embedding_sum_bytes(rows, D, T, dt):
+    return _lib.load().hd_embedding_sum_workspace_bytes(rows, D, T, dt)
+
+
 def _embedding_sum(g, idx, T, scale, padding_idx):
     D = g.shape[-1]
     if not (g.get_device() == idx.get_device() == _cur_device()):
@@ -933,7 +938,7 @@ def _embedding_sum(g, idx, T, scale, padding_idx):
     g2, ldg = (g, D) if g.is_contiguous() else _pitched(g.detach().reshape(-1, D))
     ix = idx if idx.is_contiguous() else idx.contiguous()
     dt, rows = DT_CODES[g.dtype], ix.numel()
-    nbytes = _lib.load().hd_embedding_sum_workspace_bytes(rows, D, T, dt)
+    nbytes = _embedding_sum_bytes(rows, D, T, dt)
     ws = g2.new_empty((nbytes,), dtype=torch.uint8)
     out = g2.new_empty((T, D))
     _lib.call("hd_embedding_sum", g2.data_ptr(), ldg, ix.data_ptr(), 64 if ix.dtype is torch.int64 else 32,
