@@ -250,6 +250,23 @@ class diffusion(nn.Module):
         for k, v in host.items():
             self.register_buffer(k, v.to(device), persistent=False)
 
+    def _apply(self, fn, recurse=True):
+        """.to() / .bfloat16() / .half() / .float(): the tables follow to the device but stay fp64, as the kernels read them"""
+        before = dict(self._buffers)
+        super()._apply(fn, recurse)
+        for k, v in self._host.items():
+            if self._buffers[k] is not before[k]:
+                self._buffers[k] = torch.from_numpy(v.copy()).to(self._buffers[k].device)
+        return self
+
+    def _schedule(self):
+        """(sqrt(abar), sqrt(1 - abar)) for a kernel, which reads fp64 through their pointers"""
+        a, b = self.sqrt_alphas_cumprod, self.minus_alphas_cumprod
+        if a.dtype != torch.float64 or b.dtype != torch.float64 or a.numel() < self.num_timesteps or b.numel() < self.num_timesteps:
+            raise TypeError("diffusion: the schedule tables are %s / %s of %d / %d steps, not float64 of %d"
+                            % (a.dtype, b.dtype, a.numel(), b.numel(), self.num_timesteps))
+        return a, b
+
     @property
     def device(self):
         return self.sqrt_alphas_cumprod.device
@@ -398,10 +415,11 @@ class diffusion(nn.Module):
             signs = self._signs(direction)
             lab = ops.labels_dev(labels, x_start.device)
             k = signs.shape[0]
+        ab, mab = self._schedule()
         out = torch.empty(n, d, dtype=torch.float64, device=x_start.device)
         ops._lib.call("hd_q_sample", ops._p(x_start), 1 if x_start.dtype == torch.float64 else 0, ops._p(noise),
                       1 if noise.dtype == torch.float64 else 0, ops._p(t.contiguous()), ops._p(lab), ops._p(signs), k,
-                      ops._p(self.sqrt_alphas_cumprod), ops._p(self.minus_alphas_cumprod), self.num_timesteps,
+                      ops._p(ab), ops._p(mab), self.num_timesteps,
                       ops._p(out), n, d, 1 if restrict else 0, float(np.sqrt(self.c)), float(self.prior_horizon),
                       float(self.prior), ops._stream())
         return out
@@ -528,13 +546,14 @@ class diffusion(nn.Module):
             m = self.moments(x_start)
             signs = self._signs(direction)
             lab = ops.labels_dev(labels, x.device)
+            ab, mab = self._schedule()
             ld = (n + 1 + 3) // 4 * 4
             target = torch.empty(b, n, dtype=torch.float32, device=x.device)
             h = torch.empty(b, ld, dtype=torch.float32, device=x.device)
             ops._lib.call("hd_q_sample_pack_train", ops._p(x_start), ops._p(m), ops._p(noise),
                           1 if noise.dtype == torch.float64 else 0, 1 if own_noise else 0, ops._p(t.contiguous()), None,
-                          ops._p(lab), ops._p(signs), signs.shape[0], ops._p(self.sqrt_alphas_cumprod),
-                          ops._p(self.minus_alphas_cumprod), self.num_timesteps, ops._p(target), ops._p(h), ld, b, n,
+                          ops._p(lab), ops._p(signs), signs.shape[0], ops._p(ab),
+                          ops._p(mab), self.num_timesteps, ops._p(target), ops._p(h), ld, b, n,
                           float(np.sqrt(self.c)), float(self.prior_horizon), float(self.prior), ops._stream())
             return hag.mse_loss(self.mlp.forward_packed(h, n), target)
         x_start = self.normalization(x_start)

@@ -1,0 +1,92 @@
+"""16-bit denoisers inside the modules around them: schedule tables, inputs, time feature, mixed types, the exchange of
+gradients between ranks."""
+import types
+
+import numpy as np
+import pytest
+import torch
+
+gpu = pytest.mark.gpu
+HALF = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}       # half a step, relative
+TABLES = ("alphas", "alphas_cumprod", "alphas_cumprod_prev", "minus_alphas_cumprod", "sqrt_alphas_cumprod",
+          "sqrt_recip_alphas_cumprod", "sqrt_recipm1_alphas_cumprod")
+
+
+def _diffusion(dim=30, T=1000, device="cpu"):
+    from hypdiff_amd.models.direction_diffusion import diffusion
+    torch.manual_seed(dim)
+    return diffusion(types.SimpleNamespace(r=2.0, t=1.0), dim, num_timesteps=T, device=device)
+
+
+def _set_diffusion(dim=30, T=1000, device="cpu"):
+    from hypdiff_amd.models.direction_diffusionset import diffusionset
+    torch.manual_seed(dim)
+    return diffusionset(types.SimpleNamespace(r=2.0, t=1.0), dim, dim, num_timesteps=T, device=device)
+
+
+@pytest.mark.parametrize("make", [_diffusion, _set_diffusion])
+@pytest.mark.parametrize("cast", [lambda m: m.bfloat16(), lambda m: m.half(), lambda m: m.float(), lambda m: m.double(),
+                                  lambda m: m.to(torch.bfloat16), lambda m: m.bfloat16().float(), lambda m: m.to("cpu"),
+                                  lambda m: m.to_empty(device="cpu")])
+def test_schedule_tables_stay_fp64(make, cast):
+    plain = make()
+    want = {k: getattr(plain, k).clone() for k in TABLES}
+    m = cast(make())
+    for k in TABLES:
+        got = getattr(m, k)
+        assert got.dtype == torch.float64 and torch.equal(got, want[k]), k
+    assert not any(k in m.state_dict() for k in TABLES)
+    m._schedule()
+
+
+def test_a_schedule_of_another_type_is_refused():
+    m = _diffusion()
+    m.sqrt_alphas_cumprod = m.sqrt_alphas_cumprod.float()
+    with pytest.raises(TypeError, match="schedule"):
+        m._schedule()
+
+
+def _rows(n, dim, seed):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    x = torch.randn(n, dim, device="cuda", generator=gen) * 0.05        # inside the unit ball
+    u0 = torch.randn(3, dim, device="cuda", generator=gen) * 0.05
+    labels = torch.randint(0, 3, (n,), device="cuda", generator=gen)
+    noise = torch.randn(n, dim, device="cuda", generator=gen, dtype=torch.float64)
+    return x, u0, labels, noise
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("fused", [True, False])
+def test_diffusion_trains_and_samples_in_16_bits(dtype, fused):
+    """The whole module cast, against an fp32 module with the same (rounded) weights.  Five layers, three half steps each
+    (what is stored, read and multiplied): the denoiser's output is off by e = 15 h of its norm, sqrt(loss) by e times
+    that norm, which is at most sqrt(loss) + 1 (the target is standardised), and the gradients by e for the layers and e
+    |out| / |out - target| for dL/dout."""
+    n, dim, h = 333, 30, HALF[dtype]
+    e = 15 * h
+    half = _diffusion(dim, device="cuda").to(dtype)
+    full = _diffusion(dim, device="cuda")
+    with torch.no_grad():
+        for p, q in zip(full.mlp.parameters(), half.mlp.parameters()):
+            p.copy_(q)
+    half.fuse_prepass = full.fuse_prepass = fused
+    x, u0, labels, noise = _rows(n, dim, 1)
+    t = torch.randint(0, 1000, (n,), device="cuda", generator=torch.Generator(device="cuda").manual_seed(2))
+    loss = {}
+    for name, m in (("half", half), ("full", full)):
+        loss[name] = m(x.clone(), None, labels, u0, graphset=True, t=t, noise=noise.clone())
+        loss[name].backward()
+    a, b = float(loss["half"].detach()) ** 0.5, float(loss["full"].detach()) ** 0.5
+    assert abs(a - b) <= e * (b + 1) + 1e-5
+    for p, q in zip(half.mlp.parameters(), full.mlp.parameters()):
+        assert p.grad.dtype == dtype
+        assert float((p.grad.float() - q.grad).norm()) <= e * (1 + (b + 1) / b) * float(q.grad.norm())
+    with torch.no_grad():
+        direction = full.directions(u0)
+        for step in (0, 1, 500, 999):
+            ga, xa = half.p_sample(x.double(), None, None, half.directions(u0), labels, u0, step, None, True)
+            gb, xb = full.p_sample(x.double(), None, None, direction, labels, u0, step, None, True)
+            assert xa.dtype == torch.float32 and ga.dtype == torch.float64 and bool(torch.isfinite(ga).all())
+            # the clamp behind the denoiser is 1-Lipschitz
+            assert float((xa - xb).norm()) <= e * float(full._denoise(x.double(), None, step, True).norm())
