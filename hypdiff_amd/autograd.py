@@ -40,6 +40,8 @@ def gemm_ex(a, w, bias, resid, aux, c, c2, epi):
     """hd_gemm_f32_ex / hd_gemm_f32_bf16x3 (ops.GEMM_MODE) on fp32 device tensors; a (M,K), w (N,K); c / c2 may be None."""
     M, K = a.shape
     N = w.shape[0]
+    if not (a.dtype is w.dtype is torch.float32) or (bias is not None and bias.dtype is not torch.float32):
+        raise TypeError(f"gemm_ex: fp32 operands, not {a.dtype}, {w.dtype}" + ("" if bias is None else f", {bias.dtype}"))
     if K % 4 or a.stride(0) % 4 or w.stride(0) % 4 or a.data_ptr() % 16 or w.data_ptr() % 16 or a.stride(1) != 1 \
             or w.stride(1) != 1:
         kp = (K + 3) // 4 * 4
@@ -819,6 +821,8 @@ class GCNConvGelu(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, w, b, csr, act):
+        if not (x.dtype is w.dtype is b.dtype is torch.float32):
+            raise TypeError(f"GCNConv: rows, weight and bias in float32, not {x.dtype}, {w.dtype}, {b.dtype}")
         x = x.contiguous()
         wd, bd = w.detach(), b.detach()
         xw = ops.gemm(x, wd)

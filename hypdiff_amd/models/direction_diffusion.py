@@ -96,6 +96,10 @@ class gcndec(nn.Module):
         self.fc3 = nn.Linear(128, input_dim)
 
     def forward(self, x, adj, t):
+        for layer in (self.conv1.lin, self.conv2.lin, self.conv3.lin, self.conv4.lin, self.fc1, self.fc2, self.fc3):
+            if layer.weight.dtype is not torch.float32:
+                raise TypeError(f"gcndec: weights in float32, not {layer.weight.dtype} (only the mlp denoiser, graphset=True, has a "
+                                "16-bit form)")
         ops._dev(x)
         x = x.contiguous()
         n, d = x.shape

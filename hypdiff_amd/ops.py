@@ -328,6 +328,8 @@ def match_padded(x2, m):
 
 def gemm(a, w, bias=None, epi=0, resid=None, out=None):
     """epi(a @ w.T + bias): fp32 on the exact-f32 matrix cores, fp64 on the vector ALU."""
+    if w.dtype is not a.dtype or (bias is not None and bias.dtype is not a.dtype):
+        raise TypeError(f"gemm: rows in {a.dtype}, weight in {w.dtype}, bias in {None if bias is None else bias.dtype}")
     _dev(a, w, bias)
     M, K = a.shape
     N = w.shape[0]

@@ -90,3 +90,25 @@ def test_diffusion_trains_and_samples_in_16_bits(dtype, fused):
             assert xa.dtype == torch.float32 and ga.dtype == torch.float64 and bool(torch.isfinite(ga).all())
             # the clamp behind the denoiser is 1-Lipschitz
             assert float((xa - xb).norm()) <= e * float(full._denoise(x.double(), None, step, True).norm())
+
+
+def test_gcndec_and_fp32_products_refuse_16_bit_weights():
+    from hypdiff_amd import autograd as hag, ops
+    from hypdiff_amd.models.direction_diffusion import gcndec
+    x, adj = torch.zeros(5, 30), torch.zeros(2, 0, dtype=torch.int64)
+    for m in (gcndec(30).bfloat16(), gcndec(30).half()):
+        with pytest.raises(TypeError, match="gcndec"):
+            m(x, adj, 0.5)
+    m = gcndec(30)
+    m.fc2.bfloat16()
+    with pytest.raises(TypeError, match="gcndec"):
+        m(x, adj, 0.5)
+    w, b = torch.zeros(8, 30).bfloat16(), torch.zeros(8).bfloat16()
+    for args in ((x, w), (x, w.float(), b)):
+        with pytest.raises(TypeError, match="gemm"):
+            ops.gemm(*args)
+        with pytest.raises(TypeError, match="gemm_ex"):
+            hag.gemm_ex(*(args + (None,))[:3], None, None, torch.zeros(5, 8), None, 0)
+    for args in ((x, w, b), (x, w.float(), b), (x.bfloat16(), w, b)):
+        with pytest.raises(TypeError, match="GCNConv"):
+            hag.GCNConvGelu.apply(*args, None, True)
