@@ -100,6 +100,7 @@ class gcndec(nn.Module):
             if layer.weight.dtype is not torch.float32:
                 raise TypeError(f"gcndec: weights in float32, not {layer.weight.dtype} (only the mlp denoiser, graphset=True, has a "
                                 "16-bit form)")
+        f64 = ops._is_f64(x)
         ops._dev(x)
         x = x.contiguous()
         n, d = x.shape
@@ -113,7 +114,7 @@ class gcndec(nn.Module):
                 kind, ts = 1, 0.0
         else:
             kind, tp, ts = 2, None, float(t)
-        ops._lib.call("hd_mlp_pack_input", ops._p(x), 1 if x.dtype == torch.float64 else 0, ops._p(tp), kind, ts,
+        ops._lib.call("hd_mlp_pack_input", ops._p(x), f64, ops._p(tp), kind, ts,
                       ops._p(h), n, d, ld, ops._stream())
         w1 = self.conv1.lin.weight
         if ld != d + 1:         # zero-padded copy of the first weight (differentiable slice-assign)
@@ -153,6 +154,7 @@ class mlp(nn.Module):
         return self._w1_cache[1]
 
     def forward(self, x, t):
+        f64 = ops._is_f64(x)
         ops._dev(x); ops._no_grad(x)
         x = x.contiguous()
         n, d = x.shape
@@ -174,14 +176,14 @@ class mlp(nn.Module):
             # inference: the concat goes straight into the limb image of the first GEMM's operand
             img = ops.limb_empty(n, d + 1, x.device, fmt, zero_amax=False)
             if fmt == "f16x2":
-                ops._lib.call("hd_mlp_pack_input_f16x2", ops._p(x), 1 if x.dtype == torch.float64 else 0, ops._p(tp),
+                ops._lib.call("hd_mlp_pack_input_f16x2", ops._p(x), f64, ops._p(tp),
                               kind, ts, ops._p(img.buf), ops._p(img.exp), ops._p(img.amax), n, d, ops._stream())
             else:
-                ops._lib.call("hd_mlp_pack_input_bf16x3", ops._p(x), 1 if x.dtype == torch.float64 else 0, ops._p(tp),
+                ops._lib.call("hd_mlp_pack_input_bf16x3", ops._p(x), f64, ops._p(tp),
                               kind, ts, ops._p(img.buf), n, d, ops._stream())
             return ops.linear_chain(img, chain)
         h = torch.empty(n, ld, dtype=torch.float32, device=x.device)
-        ops._lib.call("hd_mlp_pack_input", ops._p(x), 1 if x.dtype == torch.float64 else 0, ops._p(tp), kind, ts,
+        ops._lib.call("hd_mlp_pack_input", ops._p(x), f64, ops._p(tp), kind, ts,
                       ops._p(h), n, d, ld, ops._stream())
         return self.forward_packed(h, d)
 
@@ -361,14 +363,15 @@ class diffusion(nn.Module):
 
     def tran_direction(self, direction_vector, gaussian_point, labels):
         """:154-163, in place on gaussian_point (one kernel instead of a row loop)"""
+        f64 = ops._is_f64(gaussian_point)
         ops._dev(gaussian_point)
         if not gaussian_point.is_contiguous():
             raise ValueError("tran_direction: the noise tensor must be contiguous (updated in place)")
         signs = self._signs(direction_vector)
         lab = ops.labels_dev(labels, gaussian_point.device)
         n, d = gaussian_point.shape
-        ops._lib.call("hd_tran_direction", ops._p(gaussian_point), 1 if gaussian_point.dtype == torch.float64 else 0,
-                      ops._p(lab), ops._p(signs), signs.shape[0], n, d, ops._stream())
+        ops._lib.call("hd_tran_direction", ops._p(gaussian_point), f64, ops._p(lab), ops._p(signs), signs.shape[0],
+                      n, d, ops._stream())
         return gaussian_point
 
     def normalization(self, x):
@@ -382,12 +385,12 @@ class diffusion(nn.Module):
     def moments(self, h):
         """{sum, sumsq, count} of h as a 3-vector of doubles on the device (shard-local
         in data-parallel runs; all-reduce it before _apply_moments)."""
+        f64 = ops._is_f64(h)
         ops._dev(h)
         h = h.contiguous()
         ws = torch.empty(int(ops._lib.load().hd_moments_workspace_doubles()), dtype=torch.float64, device=h.device)
         m = torch.empty(3, dtype=torch.float64, device=h.device)
-        ops._lib.call("hd_moments", ops._p(h), 1 if h.dtype == torch.float64 else 0, h.numel(), ops._p(ws), ops._p(m),
-                      ops._stream())
+        ops._lib.call("hd_moments", ops._p(h), f64, h.numel(), ops._p(ws), ops._p(m), ops._stream())
         if self.sync_moments is not None:
             from ..dist import allreduce_moments
             allreduce_moments(m, None if self.sync_moments is True else self.sync_moments)
@@ -396,7 +399,7 @@ class diffusion(nn.Module):
     def _apply_moments(self, x, m, inverse):
         x = x.contiguous()
         out = torch.empty_like(x)
-        ops._lib.call("hd_standardize", ops._p(x), ops._p(out), 1 if x.dtype == torch.float64 else 0, x.numel(),
+        ops._lib.call("hd_standardize", ops._p(x), ops._p(out), ops._is_f64(x), x.numel(),
                       ops._p(m), inverse, ops._stream())
         return out
 
@@ -407,8 +410,10 @@ class diffusion(nn.Module):
     def q_sample(self, x_start, t, direction, noise, labels, u0, restrict=False):
         """:198-213.  Returns fp64 (the tables are fp64); `noise` is sign-flipped IN PLACE
         when restrict is set, like the reference's tran_direction."""
-        ops._dev(x_start, t); ops._no_grad(x_start, noise)
+        x64 = ops._is_f64(x_start)
         noise = self.default(noise, lambda: torch.randn_like(x_start))
+        noise64 = ops._is_f64(noise)
+        ops._dev(x_start, t); ops._no_grad(x_start, noise)
         if not noise.is_contiguous():
             raise ValueError("q_sample: noise must be contiguous (it is updated in place)")
         x_start = x_start.contiguous()
@@ -421,11 +426,10 @@ class diffusion(nn.Module):
             k = signs.shape[0]
         ab, mab = self._schedule()
         out = torch.empty(n, d, dtype=torch.float64, device=x_start.device)
-        ops._lib.call("hd_q_sample", ops._p(x_start), 1 if x_start.dtype == torch.float64 else 0, ops._p(noise),
-                      1 if noise.dtype == torch.float64 else 0, ops._p(t.contiguous()), ops._p(lab), ops._p(signs), k,
-                      ops._p(ab), ops._p(mab), self.num_timesteps,
-                      ops._p(out), n, d, 1 if restrict else 0, float(np.sqrt(self.c)), float(self.prior_horizon),
-                      float(self.prior), ops._stream())
+        ops._lib.call("hd_q_sample", ops._p(x_start), x64, ops._p(noise), noise64, ops._p(t.contiguous()), ops._p(lab),
+                      ops._p(signs), k, ops._p(ab), ops._p(mab), self.num_timesteps, ops._p(out), n, d,
+                      1 if restrict else 0, float(np.sqrt(self.c)), float(self.prior_horizon), float(self.prior),
+                      ops._stream())
         return out
 
     def predict_noise_from_start(self, x_t, t, x0):
@@ -456,6 +460,7 @@ class diffusion(nn.Module):
         """:272-291 -> (pred_img_t fp64, x_start fp32 clamped).  Denoiser = 5 GEMM launches,
         everything after it (predict_noise_from_start, clamp_, sign flip, q_sample at t-1)
         = one fused elementwise kernel."""
+        f64 = ops._is_f64(x)
         ops._dev(x); ops._no_grad(x)
         x = x.contiguous()
         n, d = x.shape
@@ -466,7 +471,7 @@ class diffusion(nn.Module):
         lab = ops.labels_dev(labels, x.device)
         out = torch.empty(n, d, dtype=torch.float64, device=x.device)
         H = self._host
-        ops._lib.call("hd_p_sample_update", ops._p(x), 1 if x.dtype == torch.float64 else 0, ops._p(x_start),
+        ops._lib.call("hd_p_sample_update", ops._p(x), f64, ops._p(x_start),
                       ops._p(lab), ops._p(signs), signs.shape[0], float(H["sqrt_recip_alphas_cumprod"][t]),
                       float(H["sqrt_recipm1_alphas_cumprod"][t]), float(H["sqrt_alphas_cumprod"][t2]),
                       float(H["minus_alphas_cumprod"][t2]), t, t2, ops._p(out), n, d, float(np.sqrt(self.c)),
@@ -555,7 +560,7 @@ class diffusion(nn.Module):
             target = torch.empty(b, n, dtype=torch.float32, device=x.device)
             h = torch.empty(b, ld, dtype=torch.float32, device=x.device)
             ops._lib.call("hd_q_sample_pack_train", ops._p(x_start), ops._p(m), ops._p(noise),
-                          1 if noise.dtype == torch.float64 else 0, 1 if own_noise else 0, ops._p(t.contiguous()), None,
+                          ops._is_f64(noise), 1 if own_noise else 0, ops._p(t.contiguous()), None,
                           ops._p(lab), ops._p(signs), signs.shape[0], ops._p(ab),
                           ops._p(mab), self.num_timesteps, ops._p(target), ops._p(h), ld, b, n,
                           float(np.sqrt(self.c)), float(self.prior_horizon), float(self.prior), ops._stream())

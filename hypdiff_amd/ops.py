@@ -69,12 +69,17 @@ def curv(c):
     return HdCurv(c, c ** 0.5, 1.0 / c, (1.0 / c) ** 0.5)
 
 
-def _sfx(t):
-    if t.dtype == torch.float32:
-        return "_f32"
-    if t.dtype == torch.float64:
-        return "_f64"
+def _is_f64(t):
+    """1 for float64 rows, 0 for float32: the type flag of the kernels that read both"""
+    if t.dtype is torch.float32:
+        return 0
+    if t.dtype is torch.float64:
+        return 1
     raise TypeError(f"hypdiff_amd kernels take float32/float64 rows, got {t.dtype}")
+
+
+def _sfx(t):
+    return "_f64" if _is_f64(t) else "_f32"
 
 
 def _dev(*ts):

@@ -63,7 +63,7 @@ def normalize_features(features, device="cuda"):
         x = x.to(torch.float64)
     x = x.contiguous()
     out = torch.empty(x.shape, dtype=torch.float32, device=device)
-    _lib.call("hd_feat_normalize", ops._p(x), 1 if x.dtype == torch.float64 else 0, x.shape[0], x.shape[1], ops._p(out),
+    _lib.call("hd_feat_normalize", ops._p(x), ops._is_f64(x), x.shape[0], x.shape[1], ops._p(out),
               ops._stream())
     return out
 

@@ -112,3 +112,19 @@ def test_gcndec_and_fp32_products_refuse_16_bit_weights():
     for args in ((x, w, b), (x, w.float(), b), (x.bfloat16(), w, b)):
         with pytest.raises(TypeError, match="GCNConv"):
             hag.GCNConvGelu.apply(*args, None, True)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.int64])
+def test_rows_of_another_type_are_refused(dtype):
+    """The kernels around the denoisers read fp32 or fp64 rows; 16-bit weights do not change that."""
+    from hypdiff_amd import ops
+    m = _diffusion().bfloat16()
+    x, t, adj = torch.zeros(5, 30).to(dtype), torch.zeros(5, dtype=torch.int64), torch.zeros(2, 0, dtype=torch.int64)
+    d, lab = [torch.zeros(30)] * 3, [0] * 5
+    for call in (lambda: m.mlp(x, t), lambda: m.gcn.float()(x, adj, t), lambda: m.tran_direction(d, x, lab), lambda: m.moments(x),
+                 lambda: m.normalization(x), lambda: m.q_sample(x, t, d, torch.zeros(5, 30), lab, None, True),
+                 lambda: m.q_sample(x.float(), t, d, x, lab, None, True), lambda: m.p_sample(x, None, None, d, lab, None, 3, None, True),
+                 lambda: _set_diffusion().mlp(x[None], t[:1]), lambda: ops._sfx(x)):
+        with pytest.raises(TypeError, match="float32/float64"):
+            call()
+    assert ops._is_f64(x.float()) == 0 and ops._is_f64(x.double()) == 1
