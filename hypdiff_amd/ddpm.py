@@ -138,8 +138,11 @@ class Model(nn.Module):
             idx = idx.to(device=x.device, dtype=torch.int64).contiguous()
             ab = self._alpha_bars_dev(x.device)
             used_alpha_bars = ab[idx][:, None]
-            epsilon = torch.randn_like(x) if epsilon is None else epsilon
+            # fp32 whatever x and the weights are: the kernel reads fp32 rows, the loss is taken on them
             x = x.to(torch.float32).contiguous()
+            epsilon = torch.randn_like(x) if epsilon is None else epsilon.to(torch.float32)
+            if epsilon.shape != x.shape:
+                raise ValueError(f"Model: epsilon has shape {tuple(epsilon.shape)}, x {tuple(x.shape)}")
             x_tilde = torch.empty_like(x)
             ops._lib.call("hd_ddpm_noise", ops._p(x), ops._p(epsilon.contiguous()), ops._p(idx), ops._p(ab), ab.shape[0],
                           ops._p(x_tilde), x.shape[0], x.shape[1], 1 if restrict else 0, self.deta,

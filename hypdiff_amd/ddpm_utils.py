@@ -25,7 +25,11 @@ class DDPMSampler():
 
     def one_step(self, x, idx, noise=None):
         """one iteration of _one_diffusion_step (ddpm_utils.py:37-45)"""
-        eps = self.diffusion_fn(x, idx, get_target=False)
+        x = x.to(torch.float32).contiguous()              # the kernel reads fp32 rows, 16-bit weights or not
+        noise = None if noise is None else noise.to(torch.float32).contiguous()
+        eps = self.diffusion_fn(x, idx, get_target=False).to(torch.float32).contiguous()
+        if eps.shape != x.shape or (noise is not None and noise.shape != x.shape):
+            raise ValueError("DDPMSampler: the denoiser's output and the noise have x's shape")
         out = torch.empty_like(x)
         ops._lib.call("hd_ddpm_step", ops._p(x), ops._p(eps), ops._p(noise), float(self._c1[idx]), float(self._c2[idx]),
                       float(self._c3[idx]), ops._p(out), x.numel(), ops._stream())

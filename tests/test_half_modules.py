@@ -128,3 +128,30 @@ def test_rows_of_another_type_are_refused(dtype):
         with pytest.raises(TypeError, match="float32/float64"):
             call()
     assert ops._is_f64(x.float()) == 0 and ops._is_f64(x.double()) == 1
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float64])
+@pytest.mark.parametrize("weights", [torch.float32, torch.bfloat16])
+def test_ddpm_takes_inputs_of_any_type(dtype, weights):
+    """x, epsilon and the sampler's noise in another type give what their fp32 values give, bit for bit."""
+    from hypdiff_amd.ddpm import Model
+    from hypdiff_amd.ddpm_utils import DDPMSampler
+    torch.manual_seed(4)
+    model = Model(64, 96, 2, 50, 1e-4, 0.02).cuda().to(weights)
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    new = lambda: torch.randn(40, 64, device="cuda", generator=gen).to(torch.bfloat16 if dtype != torch.float16 else dtype).to(dtype)  # noqa: E731
+    x, eps, noise = new(), new(), new()
+    idx = torch.randint(0, 50, (40,), device="cuda", generator=gen)
+    got, want = model.loss_fn(x, idx=idx, epsilon=eps), model.loss_fn(x.float(), idx=idx, epsilon=eps.float())
+    assert torch.equal(got, want) and bool(torch.isfinite(got.detach()))
+    torch.manual_seed(6)
+    got = model.loss_fn(x, idx=idx)
+    torch.manual_seed(6)
+    assert torch.equal(got, model.loss_fn(x.float(), idx=idx))
+    s = DDPMSampler(1e-4, 0.02, 50, model, "cuda", (64,))
+    with torch.no_grad():
+        assert torch.equal(s.one_step(x, 7, noise), s.one_step(x.float(), 7, noise.float()))
+        assert torch.equal(s.one_step(x.t().contiguous().t(), 7, noise), s.one_step(x.float(), 7, noise.float()))
+    with pytest.raises(ValueError, match="epsilon"):
+        model.loss_fn(x, idx=idx, epsilon=eps[:1])
