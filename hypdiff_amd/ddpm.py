@@ -69,8 +69,13 @@ class Backbone(nn.Module):
         self.linear_model2 = MLP(dim_hidden, dim_hidden, dim_in, num_layer)
 
     def forward(self, x, idx):
+        kind = self.embedding_layer.weight.dtype
+        if not (self.linear_model1.layers[0].weight.dtype is kind is self.linear_model2.layers[0].weight.dtype):
+            # activations of one type would reach an embedding that reads and writes another
+            raise TypeError("Backbone: linear_model1, embedding_layer and linear_model2 have weights of one type, not "
+                            f"{self.linear_model1.layers[0].weight.dtype}, {kind}, {self.linear_model2.layers[0].weight.dtype}")
         ops._dev(x)
-        if self.embedding_layer.weight.dtype in ops.HALF_TYPES:
+        if kind in ops.HALF_TYPES:
             # bf16 / fp16 weights: the result comes back in x's type (the noising and the sampler around it stay in fp32)
             h = self.linear_model1(x)
             h = ops.embedding(idx.to(device=x.device, dtype=torch.int64), self.embedding_layer.weight, add=h)

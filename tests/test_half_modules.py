@@ -155,3 +155,13 @@ def test_ddpm_takes_inputs_of_any_type(dtype, weights):
         assert torch.equal(s.one_step(x.t().contiguous().t(), 7, noise), s.one_step(x.float(), 7, noise.float()))
     with pytest.raises(ValueError, match="epsilon"):
         model.loss_fn(x, idx=idx, epsilon=eps[:1])
+
+
+@pytest.mark.parametrize("part", ["linear_model1", "embedding_layer", "linear_model2"])
+def test_backbone_of_mixed_types_is_refused(part):
+    from hypdiff_amd.ddpm import Backbone
+    for whole, other in ((torch.float32, torch.bfloat16), (torch.bfloat16, torch.float32), (torch.bfloat16, torch.float16)):
+        bb = Backbone(64, 96, 2, 50).to(whole)
+        getattr(bb, part).to(other)
+        with pytest.raises(TypeError, match="one type"):
+            bb(torch.zeros(3, 64), torch.zeros(3, dtype=torch.int64))
