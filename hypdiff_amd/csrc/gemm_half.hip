@@ -201,25 +201,31 @@ struct Stager {
     }
 };
 
-// 0.5 erfc(a / sqrt 2) for a = |x|, as 2^(a P(a) - 1): a weighted minimax fit of log2 erfc, of degree 4 because the result is
-// rounded to 16 bits: GELU comes out within 2e-6 |x| (relative 8e-5 down to x = -3, a sixth of fp16's half step); the fp32 path's
-// degree 7 costs three more operations an element, and the epilogue shares the vector unit with the products' issue.
+// 2^SHIFT * 0.5 erfc(a / sqrt 2) for a = |x|, as 2^(a P(a) - 1 + SHIFT): a weighted minimax fit of log2 erfc.  Degree 8, so that
+// GELU's negative tail is right to a quarter of the half step of the type it is rounded to: relative error 5.5e-5 down to x = -6, where
+// fp16 ends, 3.3e-4 down to -13.3, where bf16 does (a degree of 4 is off by 0.4 % at -4 and by 17 % at -6), and 1.4e-6 |x| anywhere.
 // Beyond 30 it is 0 in any case; the clamp keeps infinities out of the products.
+template <int SHIFT>
 __device__ __forceinline__ float half_erfc16(float x) {
     const float a = fminf(fabsf(x), 30.f);
-    float r = fmaf(-4.9161474e-04f, a, 7.2239037e-03f);
-    r = fmaf(r, a, -5.2209500e-02f);
-    r = fmaf(r, a, -4.5953175e-01f);
-    r = fmaf(r, a, -1.1510228f);
-    return __builtin_amdgcn_exp2f(fmaf(r, a, -1.0f));
+    float r = fmaf(-1.26476807e-09f, a, 1.06469543e-07f);
+    r = fmaf(r, a, -3.80471897e-06f);
+    r = fmaf(r, a, 7.67703314e-05f);
+    r = fmaf(r, a, -9.83094680e-04f);
+    r = fmaf(r, a, 8.56748410e-03f);
+    r = fmaf(r, a, -5.38930967e-02f);
+    r = fmaf(r, a, -4.58624214e-01f);
+    r = fmaf(r, a, -1.15118206e+00f);
+    return __builtin_amdgcn_exp2f(fmaf(r, a, (float)(SHIFT - 1)));
 }
-// GELU(x) = (x + |x|) / 2 - |x| * (0.5 erfc(|x| / sqrt 2)); the first term passes a NaN on and +inf through
+// GELU(x) = (x + |x|) / 2 - |x| * (0.5 erfc(|x| / sqrt 2)); the first term passes a NaN on and +inf through.  The second is
+// formed 2^24 above its value and brought down last: exp2 returns 0 below 2^-126, which x = -12.9 reaches
 __device__ __forceinline__ float gelu16(float x) {
-    return fmaf(-fminf(fabsf(x), 30.f), half_erfc16(x), fmaf(0.5f, fabsf(x), 0.5f * x));
+    return fmaf(fminf(fabsf(x), 30.f) * half_erfc16<24>(x), -0x1p-24f, fmaf(0.5f, fabsf(x), 0.5f * x));
 }
-// Phi(x) + x phi(x)
+// Phi(x) + x phi(x); Phi of a negative x without a difference that would round at 2^-25
 __device__ __forceinline__ float gelu16_slope(float x) {
-    const float Phi = 0.5f + copysignf(0.5f - half_erfc16(x), x);
+    const float q = half_erfc16<0>(x), Phi = x < 0.f ? q : 1.0f - q;
     return fmaf(x, __builtin_amdgcn_exp2f(fmaf(x * -0.72134752044448170368f, x, -1.32574806473615f)), Phi);   // log2(1 / sqrt(2 pi))
 }
 template <int ACT>
