@@ -191,10 +191,15 @@ class mlp(nn.Module):
         """the stack on an already packed input: h = [x.float(), t, 0 ...] rows of pitch (d + 1) rounded up to 4"""
         ld = h.shape[1]
         if self.fc1.weight.dtype in ops.HALF_TYPES:
-            # bf16 / fp16 weights, inference and training: one fused launch a layer; the result in fp32 like the other paths
-            # (t enters in the weights' type: bf16 holds whole steps up to 256 exactly, fp16 up to 2048)
-            y = h[:, : d + 1].to(self.fc1.weight.dtype)
-            for fc in (self.fc1, self.fc2, self.fc3, self.fc4):
+            # bf16 / fp16 weights, inference and training: one fused launch a layer; the result in fp32 like the other paths.
+            # t enters as the sum of two 16-bit columns (t rounded, and what the rounding dropped) against the one weight
+            # column: 17 bits of it count in bf16, 22 in fp16.  Rounded once, bf16 would tell 507 of 1000 steps apart.
+            dt, w1 = self.fc1.weight.dtype, self.fc1.weight
+            y = torch.empty(h.shape[0], d + 2, dtype=dt, device=h.device)
+            y[:, : d + 1].copy_(h[:, : d + 1])
+            torch.sub(h[:, d:d + 1], y[:, d:d + 1], out=y[:, d + 1:])
+            y = ops.linear_act(y, torch.cat([w1, w1[:, d:]], 1), self.fc1.bias, act="gelu")
+            for fc in (self.fc2, self.fc3, self.fc4):
                 y = ops.linear_act(y, fc.weight, fc.bias, act="gelu")
             return ops.linear_act(y, self.fc5.weight, self.fc5.bias).to(torch.float32)
         chain = [(self.fc1.weight, self.fc1.bias, 1), (self.fc2.weight, self.fc2.bias, 1),

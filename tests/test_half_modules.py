@@ -165,3 +165,68 @@ def test_backbone_of_mixed_types_is_refused(part):
         getattr(bb, part).to(other)
         with pytest.raises(TypeError, match="one type"):
             bb(torch.zeros(3, 64), torch.zeros(3, dtype=torch.int64))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("fraction", [False, True])
+def test_every_step_reaches_the_denoiser(dtype, fraction, monkeypatch):
+    """All 1000 steps, as integers (sampling) and as t / T (training), through a first layer that shows t: unit j has the
+    weight s (1, or 1000 for fractions: exact in both types) on t and the bias -4 j, so it holds gelu(s t - 4 j).  t as two
+    16-bit numbers is off by h^2 of itself (the second one's half step); the fractions of fp16 by 2^-25 besides."""
+    from hypdiff_amd import ops
+    from hypdiff_amd.models.direction_diffusion import mlp
+    d, h = 6, HALF[dtype]
+    net = mlp(d).cuda().to(dtype)
+    scale = 1000.0 if fraction else 1.0
+    with torch.no_grad():
+        net.fc1.weight.zero_()
+        net.fc1.weight[:, d] = scale
+        net.fc1.bias.copy_(-4.0 * (torch.arange(800, device="cuda") % 250))
+    first = []
+    inner = ops.linear_act
+
+    def record(*args, **kw):
+        out = inner(*args, **kw)
+        first.append(out.detach())
+        return out
+    monkeypatch.setattr(ops, "linear_act", record)
+    steps = torch.arange(1000, device="cuda")
+    t = steps.double().div(1000).float() if fraction else steps
+    with torch.no_grad():
+        net(torch.zeros(1000, d, device="cuda"), t)
+    z = scale * t.double()[:, None] + net.fc1.bias.detach().double()
+    want = z * 0.5 * torch.erfc(-z / 2.0 ** 0.5)
+    off = 1.13 * scale * (h * h * t.double().abs() + (2.0 ** -25 if dtype == torch.float16 else 0.0))[:, None]
+    got = first[0].double()
+    over = (got - want).abs() - (off + 1.25 * h * (want.abs() + off) + 2.0 ** -25 + 4 * 2.0 ** -24 * z.abs())
+    assert not bool((over > 0).any()), float(over.max())
+    assert torch.unique(first[0], dim=0).shape[0] == 1000
+    net.train()
+    out = net(torch.zeros(1000, d, device="cuda"), t)
+    out.sum().backward()
+    assert net.fc1.weight.grad.shape == net.fc1.weight.shape and bool(torch.isfinite(net.fc1.weight.grad).all())
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_gradient_of_the_step_column(dtype):
+    """The weight column of t sums the gradients of both parts: against fp32 autograd on the same (rounded) weights with t
+    unrounded, at the bound of a five-layer pass (three half steps a layer)."""
+    from hypdiff_amd.models.direction_diffusion import mlp
+    torch.manual_seed(8)
+    d = 13
+    net = mlp(d).cuda().to(dtype)
+    x = torch.randn(500, d, device="cuda")
+    t = torch.rand(500, device="cuda")
+    ps = {n: p.detach().double().requires_grad_(True) for n, p in net.named_parameters()}
+    hid = torch.cat([x, t[:, None]], 1).double()
+    for k in range(1, 6):
+        hid = hid @ ps[f"fc{k}.weight"].t() + ps[f"fc{k}.bias"]
+        hid = hid * 0.5 * torch.erfc(-hid / 2.0 ** 0.5) if k < 5 else hid
+    g = torch.randn(500, d, device="cuda").to(dtype)
+    net(x, t).backward(g.float())
+    hid.backward(g.double())
+    for sl in (slice(0, d), slice(d, d + 1)):
+        got, want = net.fc1.weight.grad[:, sl].double(), ps["fc1.weight"].grad[:, sl]
+        assert float((got - want).norm()) <= 15 * HALF[dtype] * float(want.norm())
