@@ -4,6 +4,8 @@ Stands beside dist.BucketAdam (Adam over the fp32 bucket of the data-parallel tr
 parameters in fp32, bf16 or fp16 with gradients of their own type, with decoupled weight decay and parameter groups.  The
 reference trains with optim.Adam(params, lr) (diff.py:107, diff_graphset.py:66, lp_train.py:41-46).
 """
+import numbers
+
 import numpy as np
 import torch
 
@@ -290,6 +292,8 @@ class AdamW(torch.optim.Optimizer):
             for pid, p in zip(g["params"], mine["params"]):
                 if saved.get(pid):
                     self._check_saved(saved[pid], p, opt)
+            if any(saved.get(pid) for pid in g["params"]):
+                ops._dev(*mine["params"])
         # and the saved state may be this optimizer's own: that is copied before it is overwritten
         own = {b.untyped_storage().data_ptr() for fl in self._flats.values() for b in fl.buffers.values()}
         kept = lambda v: v.detach().clone() if v.untyped_storage().data_ptr() in own else v.detach()  # noqa: E731
@@ -341,9 +345,16 @@ class AdamW(torch.optim.Optimizer):
             {"exp_avg": n, "exp_avg_sq_root": n, "exp_avg_scale": blocks, "exp_avg_sq_root_scale": blocks}
         if opt["master_weights"] and p.dtype != torch.float32 and "master" in st:
             want["master"] = n
+        step = st.get("step")
+        if torch.is_tensor(step):
+            step = step.item() if step.numel() == 1 else None
+        if isinstance(step, bool) or not isinstance(step, numbers.Real) or not 0 <= step < 1 << 53 or step != int(step):
+            raise ValueError(f"AdamW: the saved step is {st.get('step')!r}, not a whole number >= 0")
         for k, count in want.items():
             if k not in st:
                 raise ValueError(f"AdamW: the saved state has no {k} (state_bits={bits})")
+            if not torch.is_tensor(st[k]) or st[k].is_complex():
+                raise TypeError(f"AdamW: the saved {k} is not a tensor of real numbers")
             if st[k].numel() != count:
                 raise ValueError(f"AdamW: the saved {k} has {st[k].numel()} elements, not {count}")
             codes = bits == 8 and k in ("exp_avg", "exp_avg_sq_root")

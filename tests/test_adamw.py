@@ -414,3 +414,63 @@ def test_refusals_of_the_entry_point():
                       (dict(m=None), "null state"), (dict(m=260), "16-byte")):
         with pytest.raises(RuntimeError, match=what):
             call(**bad)
+
+
+BAD_STEPS = [None, -1, 1.5, float("nan"), float("inf"), "3", True, torch.tensor([1.0, 2.0]), torch.tensor(-2.0), torch.tensor(float("nan"))]
+
+
+def _saved_step(sd, k, step):
+    sd = {"state": {i: dict(st) for i, st in sd["state"].items()}, "param_groups": [dict(g, lr=0.5) for g in sd["param_groups"]]}
+    if step is None:
+        del sd["state"][k]["step"]
+    else:
+        sd["state"][k]["step"] = step
+    return sd
+
+
+def test_a_state_without_a_step_is_refused_before_anything_changes():
+    from hypdiff_amd.optim import AdamW
+    p = torch.nn.Parameter(torch.zeros(4))
+    opt = AdamW([p], lr=1e-3)
+    whole = {"state": {0: {"step": 1, "exp_avg": torch.zeros(4), "exp_avg_sq": torch.zeros(4)}}, "param_groups": opt.state_dict()["param_groups"]}
+    for bad in BAD_STEPS:
+        with pytest.raises(ValueError, match="step"):
+            opt.load_state_dict(_saved_step(whole, 0, bad))
+    for entry in (None, 3.0, torch.zeros(4, dtype=torch.complex64)):
+        sd = _saved_step(whole, 0, 1)
+        sd["state"][0]["exp_avg_sq"] = entry
+        with pytest.raises(TypeError, match="exp_avg_sq"):
+            opt.load_state_dict(sd)
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        opt.load_state_dict(_saved_step(whole, 0, torch.tensor(2.0)))
+    assert opt.param_groups[0]["lr"] == 1e-3 and not opt.state
+
+
+@gpu
+@pytest.mark.parametrize("captured", [False, True])
+def test_a_refused_step_changes_nothing_on_the_device(captured):
+    from hypdiff_amd.optim import AdamW
+    a = _params(torch.bfloat16, seed=9)
+    opt = AdamW(a, state_bits=8, master_weights=True, **H)
+    opt.step()
+    opt.step()
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    if captured:
+        with torch.cuda.graph(graph):
+            opt.step()
+        graph.replay()
+    sd = copy.deepcopy(opt.state_dict())
+    before = {k: v.view(torch.uint8).clone() for k, v in opt.state_buffers().items()}
+    table = opt._flats[0].table.clone()
+    for bad in BAD_STEPS:
+        with pytest.raises(ValueError, match="step"):
+            opt.load_state_dict(_saved_step(sd, len(a) - 2, bad))
+    for k, v in opt.state_buffers().items():
+        assert torch.equal(v.view(torch.uint8), before[k]), k
+    assert torch.equal(opt._flats[0].table, table) and opt.param_groups[0]["lr"] == H["lr"]
+    assert opt.state_dict()["state"][0]["step"] == 2 + captured
+    opt.load_state_dict(sd)
+    if captured:
+        graph.replay()
+        assert opt.state_dict()["state"][0]["step"] == 4
