@@ -95,7 +95,7 @@ class AdamW(torch.optim.Optimizer):
         step of the type is lost otherwise).  fp32 parameters are their own.  The masters are taken from the parameters at
         the first step (or from a loaded state): parameters changed by hand afterwards are overwritten.
 
-    Sparse, complex and fp64 parameters, lr as a tensor, amsgrad and maximize are not offered.  A parameter whose gradient
+    The parameters of a group are distinct and share no memory.  Sparse, complex and fp64 parameters, lr as a tensor, amsgrad and maximize are not offered.  A parameter whose gradient
     is None is skipped and does not count the step.  Inside a captured HIP graph the step count lives on the device, so a
     replay has the right bias corrections (state_dict reads it back); lr and the other options are the captured ones.  Run one step (or load a state)
     before the capture; a state loaded later goes into the same arrays, and replays continue from it.  state_dict / load_state_dict keep the state's own types; with state_bits=32 a state saved by
@@ -124,6 +124,8 @@ class AdamW(torch.optim.Optimizer):
         g = self.param_groups[-1]
         try:
             self._check_options(g)
+            if len({id(p) for p in g["params"]}) != len(g["params"]):
+                raise ValueError("AdamW: a parameter stands twice in a group (both updates would run at once)")
             for p in g["params"]:
                 if p.dtype not in _DT:
                     raise TypeError(f"AdamW: parameters in float32, bfloat16 or float16, not {p.dtype}")
@@ -140,11 +142,21 @@ class AdamW(torch.optim.Optimizer):
             if not group["params"]:
                 return None
             ops._dev(*group["params"])
+            self._check_apart(group["params"])
             if torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("AdamW: the state does not exist yet: run one step or load a state before capturing a graph")
             fl = self._flats[gi] = _Flat(group)
             self._link(fl)
         return fl
+
+    @staticmethod
+    def _check_apart(params):
+        """one launch updates all of them: no two may share memory"""
+        end = 0
+        for start, stop in sorted((p.data_ptr(), p.data_ptr() + p.numel() * p.element_size()) for p in params if p.numel()):
+            if start < end:
+                raise ValueError("AdamW: two parameters of a group share memory (both updates would run at once)")
+            end = stop
 
     def _link(self, fl):
         fl.states = [self.state[p] for p in fl.params]

@@ -474,3 +474,38 @@ def test_a_refused_step_changes_nothing_on_the_device(captured):
     if captured:
         graph.replay()
         assert opt.state_dict()["state"][0]["step"] == 4
+
+
+@pytest.mark.filterwarnings("ignore:optimizer contains a parameter group with duplicate")
+def test_a_parameter_twice_is_refused():
+    """one launch would read and write it from two places at once"""
+    from hypdiff_amd.optim import AdamW
+    p, q = (torch.nn.Parameter(torch.zeros(n)) for n in (600, 4))
+    with pytest.raises(ValueError, match="twice"):
+        AdamW([p, q, p])
+    opt = AdamW([p])
+    with pytest.raises(ValueError, match="twice"):
+        opt.add_param_group({"params": [q, q]})
+    assert len(opt.param_groups) == 1
+    base = torch.zeros(600)
+    apart = [torch.nn.Parameter(base[:300]), torch.nn.Parameter(base[300:]), torch.nn.Parameter(torch.zeros(0)), q]
+    AdamW._check_apart(apart)
+    with pytest.raises(ValueError, match="share memory"):
+        AdamW._check_apart(apart + [torch.nn.Parameter(base[299:301])])
+
+
+@gpu
+def test_parameters_that_share_memory_are_refused():
+    from hypdiff_amd.optim import AdamW
+    base = torch.zeros(600, device="cuda")
+    ps = [torch.nn.Parameter(base[:301]), torch.nn.Parameter(base[300:])]
+    for p in ps:
+        p.grad = torch.ones_like(p)
+    with pytest.raises(ValueError, match="share memory"):
+        AdamW(ps).step()
+    assert not base.any()
+    ps = [torch.nn.Parameter(base[:300]), torch.nn.Parameter(base[300:])]
+    for p in ps:
+        p.grad = torch.ones_like(p)
+    AdamW(ps, lr=0.5, weight_decay=0.0).step()          # neighbours in one buffer: m / sqrt(v) = 1
+    assert float((base + 0.5).abs().max()) <= 0.5 * 16 * 2.0 ** -24 + 0.5e-8
