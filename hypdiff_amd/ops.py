@@ -11,6 +11,7 @@ import weakref
 
 import numpy as np
 import torch
+import torch.autograd.forward_ad as _fwd
 
 from . import _lib
 from ._lib import HdCurv
@@ -810,7 +811,7 @@ def linear_act(x, weight, bias=None, act="identity", resid=None):
         same, grad = same and resid.get_device() == dev, grad or resid.requires_grad
     if not same:
         _dev(x, weight, bias, resid)                      # says which one is elsewhere
-    if grad and torch.is_grad_enabled():
+    if (grad and torch.is_grad_enabled()) or _fwd._current_level >= 0:      # inside a dual level: the Function refuses tangents
         from . import autograd as hag
         skip = resid is x                                 # x's two gradients leave as one
         return hag.LinearAct.apply(x, weight, bias, None if skip else resid, code, skip)
@@ -907,7 +908,7 @@ def embedding(idx, table, scale=1.0, add=None, padding_idx=None):
     scale = float(scale)
     if not same:
         _dev(table, idx, add)                             # says which one is elsewhere
-    if grad and torch.is_grad_enabled():
+    if (grad and torch.is_grad_enabled()) or _fwd._current_level >= 0:      # inside a dual level: the Function refuses tangents
         from . import autograd as hag
         return hag.Embedding.apply(table, add, idx, scale, padding_idx)
     return _embedding_lookup(table, idx, scale, add)

@@ -397,3 +397,25 @@ def test_refusals_of_the_entry_points():
         with pytest.raises(RuntimeError, match=what):
             bwd(**bad)
     assert _lib.load().hd_linear_act_bwd_workspace_bytes(1 << 30, 8, 8, 6) == 0
+
+
+@gpu
+@pytest.mark.parametrize("grad", [False, True])
+def test_forward_mode_derivatives_are_refused(grad):
+    """a tangent may not get lost, whether or not an operand requires a gradient; operands without one pass"""
+    import torch.autograd.forward_ad as fwd
+    from hypdiff_amd import ops
+    x, w = (torch.randn(8, 8, device="cuda", dtype=torch.bfloat16) for _ in range(2))
+    idx = torch.arange(8, device="cuda")
+    y, e = ops.linear_act(x, w, act="gelu"), ops.embedding(idx, w, add=x)
+    w.requires_grad_(grad)
+    with fwd.dual_level():
+        assert torch.equal(ops.linear_act(x, w, act="gelu"), y) and torch.equal(ops.embedding(idx, w, add=x), e)
+        dual = fwd.make_dual(x, torch.ones_like(x))
+        for call in (lambda: ops.linear_act(dual, w), lambda: ops.linear_act(x, w, resid=dual), lambda: ops.linear_act(x, dual),
+                     lambda: ops.linear_act(x, w, dual[0]), lambda: ops.linear_act(dual, w, resid=dual),
+                     lambda: ops.embedding(idx, dual), lambda: ops.embedding(idx, w, add=dual)):
+            with pytest.raises(NotImplementedError, match="forward mode"):
+                call()
+            with torch.no_grad(), pytest.raises(NotImplementedError, match="forward mode"):
+                call()
