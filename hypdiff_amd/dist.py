@@ -88,10 +88,24 @@ def _in_a_live_graph(params):
     return live
 
 
+class _WideMean:
+    """Mean over the ranks of a 16-bit buffer, reduced through an fp32 copy: dividing and adding in 16 bits would round once
+    a rank, and lose what falls below fp16's smallest step.  wait() brings the mean back, rounded once."""
+
+    def __init__(self, view, group):
+        self.view, self.wide = view, view.to(torch.float32)
+        self.wide.div_(dist.get_world_size(group))
+        self.work = dist.all_reduce(self.wide, op=dist.ReduceOp.SUM, group=group, async_op=True)
+
+    def wait(self):
+        self.work.wait()
+        self.view.copy_(self.wide)
+
+
 class GradBucket:
     """All gradients of a module as ONE flat buffer (2.8 M elements for the mlp denoiser at D=512 ~ 11 MB; 6.4 M ~ 25 MB for
-    ddpm.Backbone), in fp32, or in bf16 / fp16 where all parameters are: ranks then exchange half the bytes, and each
-    addition of the reduction rounds like the gradients themselves are rounded.
+    ddpm.Backbone), in fp32, or in bf16 / fp16 where all parameters are.  Ranks exchange fp32 either way: a 16-bit chunk
+    is widened when it leaves and rounded once when its mean is back.
 
     The buffer is reduced in a few large chunks rather than per parameter -- xGMI links are
     point-to-point, so a ring all-reduce is per-link bound and few large messages beat many small
@@ -199,6 +213,9 @@ class GradBucket:
                 p.grad = self.flat[lo:hi].view_as(p)
         if not _collective(self._group):      # one process: the bucket is only the sink of the backward kernels
             return
+        if view.dtype != torch.float32:
+            self._works.append(_WideMean(view, self._group))
+            return
         view.div_(dist.get_world_size(self._group))
         self._works.append(dist.all_reduce(view, op=dist.ReduceOp.SUM, group=self._group, async_op=True))
 
@@ -216,6 +233,9 @@ class GradBucket:
         """one blocking all-reduce of the whole bucket (the non-overlapped form)"""
         if not _collective(group):
             return None
+        if self.flat.dtype != torch.float32:
+            work = _WideMean(self.flat, group)
+            return work if async_op else work.wait()
         self.flat.div_(dist.get_world_size(group))
         return dist.all_reduce(self.flat, op=dist.ReduceOp.SUM, group=group, async_op=async_op)
 
