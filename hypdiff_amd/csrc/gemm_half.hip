@@ -891,13 +891,14 @@ extern "C" int hd_linear_act_fwd(const void* x, int64_t ldx, const void* w, int6
     HD_REQUIRE(!resid || ldr >= 0, "hd_linear_act_fwd: negative pitch");
     HD_REQUIRE((((uintptr_t)x | (uintptr_t)w | (uintptr_t)y | (uintptr_t)z | (uintptr_t)bias | (uintptr_t)resid) & 1) == 0,
                "hd_linear_act_fwd: pointer not aligned to the element");
-    HD_REQUIRE(tiles_of(M, N, 64, 64) < (1LL << 24) - 8, "hd_linear_act_fwd: too many tiles");   // a grid holds 2^32 threads
+    const bool direct = direct_ok(x, ldx, K, M) && direct_ok(w, ldw, K, N);
+    const int64_t tile = K < 8 && !direct ? 32 : 64;                          // small_gemm's tiles, whatever their number
+    HD_REQUIRE(tiles_of(M, N, tile, tile) < (1LL << 24) - 8, "hd_linear_act_fwd: too many tiles");   // a grid holds 2^32 threads
     Prod g = {};
     g.A = x; g.lda = ldx; g.B = w; g.ldb = ldw; g.M = (int)M; g.N = (int)N; g.K = (int)K;
     g.C = y; g.bias = bias; g.resid = resid; g.ldr = ldr; g.z = z; g.act = act;
     // a z beside which nothing stays in the 256 MB behind the L2s until the backward pass reads it: 74750 x 900 183 against 200 us
     g.z_past = M * N >= (1LL << 25);
-    const bool direct = direct_ok(x, ldx, K, M) && direct_ok(w, ldw, K, N);
     return dtype == HD_DT_BF16 ? linear_fwd<bf16>(g, direct, (hipStream_t)st) : linear_fwd<f16>(g, direct, (hipStream_t)st);
 }
 

@@ -419,3 +419,15 @@ def test_forward_mode_derivatives_are_refused(grad):
                 call()
             with torch.no_grad(), pytest.raises(NotImplementedError, match="forward mode"):
                 call()
+
+
+def test_grids_beyond_the_limit_are_refused():
+    """an input narrower than a chunk takes 32 x 32 tiles whatever their number: 2^24 of them are 2^32 threads, which no grid
+    holds (no GPU needed: refused before anything is launched)"""
+    from hypdiff_amd import _lib
+
+    def fwd(M, N, K):
+        _lib.call("hd_linear_act_fwd", 256, K, 256, K, None, None, 0, 1, M, N, K, 0, 256, None, None)
+    for M, N, K in ((1 << 24, 1024, 3), (1 << 19, 1 << 15, 7), ((1 << 29) - 1, 33, 1), (1 << 26, 4096, 8), (1 << 26, 4096, 9)):
+        with pytest.raises(RuntimeError, match="too many tiles"):
+            fwd(M, N, K)
