@@ -431,3 +431,38 @@ def test_grids_beyond_the_limit_are_refused():
     for M, N, K in ((1 << 24, 1024, 3), (1 << 19, 1 << 15, 7), ((1 << 29) - 1, 33, 1), (1 << 26, 4096, 8), (1 << 26, 4096, 9)):
         with pytest.raises(RuntimeError, match="too many tiles"):
             fwd(M, N, K)
+
+
+def _tiles(M, N, bm, bn):
+    return -(-M // bm) * -(-N // bn)
+
+
+def _kind(M, N, K, direct):
+    """the kernel that hd_linear_act_fwd takes (csrc/gemm_half.hip, choose_tiles): 0 the 32 x 32 one, then by tile size"""
+    if (K < 8 and not direct) or _tiles(M, N, 32, 32) <= (512 if direct else 64):
+        return 0
+    cost = [max(least, start + (per if direct else odd) / 256 * _tiles(M, N, bm, bn)) for bm, bn, start, per, odd, least in (
+        (64, 64, 6, 2.85, 3.6, 11), (64, 128, 6, 4.6, 5.4, 13), (128, 128, 8, 8, 8, 18), (128, 192, 8, 12, 12, 20))]
+    return 1 + cost.index(min(cost))
+
+
+# every tile size with rows staged straight to LDS (K a multiple of 8) and through registers, none of the sizes a multiple of a tile
+@gpu
+@pytest.mark.parametrize("M,N,K,kind", [(4101, 260, 136, 1), (8055, 264, 72, 2), (5003, 776, 200, 2), (7750, 776, 136, 3),
+                                        (6225, 904, 104, 4), (9003, 906, 64, 4),
+                                        (674, 72, 101, 1), (7994, 201, 67, 2), (5001, 777, 129, 2), (7262, 521, 131, 3), (6164, 905, 77, 4),
+                                        (9001, 907, 70, 4)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_every_tile_size(M, N, K, kind, dtype):
+    assert _kind(M, N, K, K % 8 == 0) == kind
+    _run(M, N, K, dtype, ("gelu", "relu", "identity")[M % 3], True, M % 2 == 0, M)
+
+
+# the weight gradient in 192 x 192 tiles (from 8e9 products and 6 tiles on), rows straight to LDS and through registers; also
+# the input gradient of a wide layer in the larger tiles
+@gpu
+@pytest.mark.parametrize("M,N,K", [(20011, 600, 680), (20011, 601, 681), (12007, 1000, 904), (12007, 905, 1001), (41003, 385, 577)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_large_weight_gradients(M, N, K, dtype):
+    assert M * N * K >= 8e9 and _tiles(N, K, 192, 192) >= 6 and M % 64 and N % 192 and K % 192
+    _run(M, N, K, dtype, "gelu" if M % 2 else "relu", True, False, N)
