@@ -278,3 +278,20 @@ def test_refusals_of_the_entry_points():
     with pytest.raises(RuntimeError, match="null"):
         summed(ws=None)
     assert _lib.load().hd_embedding_sum_workspace_bytes(1 << 31, 8, 4, 0) == 0
+
+
+@gpu
+@pytest.mark.parametrize("T", [(1 << 24) + 5, 1 << 24, (1 << 16) - 1, 1 << 16])
+def test_gradient_at_every_number_of_radix_passes(T):
+    """tokens of 17, 16 and 25 bits (3, 2, 4 passes): the named rows against 64 bits, all others zero"""
+    from hypdiff_amd import ops
+    rows, D = 3000, 2
+    idx = _idx(rows, T, "hot", torch.int64, 50)
+    idx[-1] = T - 1
+    g = torch.randn(rows, D, device="cuda", generator=_gen(51))
+    got = ops._embedding_sum(g, idx, T, 1.0, None)
+    names, at = torch.unique(idx, return_inverse=True)
+    want, size = _grad64(at, g, names.numel(), 1.0, None)
+    _check(got[names], want, size, torch.float32)
+    got[names] = 0
+    assert not bool(got.any())
