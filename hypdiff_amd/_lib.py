@@ -40,11 +40,6 @@ class HdAdamJob(ctypes.Structure):
     _fields_ = [("param", c_void_p), ("offset", c_int64), ("count", c_int64)]
 
 
-class HdAdamWJob(ctypes.Structure):
-    """struct hd_adamw_job of include/hypdiff.h"""
-    _fields_ = [("param", c_void_p), ("grad", c_void_p), ("first", c_int64), ("count", c_int64), ("row", c_int64)]
-
-
 class HdTnJob(ctypes.Structure):
     """struct hd_tn_job of include/hypdiff.h"""
     _fields_ = [("a_img", c_void_p), ("b_img", c_void_p), ("c", c_void_p), ("colsum_a", c_void_p), ("P", c_int64),

@@ -13,6 +13,7 @@ from . import _lib, ops
 
 BLOCK = 256                 # elements of one scale of the 8-bit moments; every tensor's state starts on a multiple of it
 _DT = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+# struct hd_adamw_job of include/hypdiff.h
 _JOB = np.dtype([("param", np.uint64), ("grad", np.uint64), ("first", np.int64), ("count", np.int64), ("row", np.int64)])
 _OPTIONS = ("lr", "betas", "eps", "weight_decay", "state_bits", "master_weights")
 
