@@ -205,3 +205,27 @@ def test_sampler_runs_on_16_bit_weights():
     # one denoiser pass of 9 stages, weights rounded too (one more half step each), scaled into the update of x
     assert float((got - want).norm() / want.norm()) <= 4 * 9 * 2.0 ** -8
     assert final.shape == (30, 64) and bool(torch.isfinite(final).all())
+
+
+@gpu
+def test_capture_of_an_fp32_module_beside_an_eager_graph():
+    """BucketAdam: refused while a loss holds the parameters' nodes (the captured backward pass would join their stream), and
+    nothing has changed by then; captured once it is dropped, detached losses may stay."""
+    from hypdiff_amd import dist as hdist
+    from hypdiff_amd.ddpm import Model
+    torch.manual_seed(11)
+    model = Model(64, 96, 2, 50, 1e-4, 0.02).cuda()
+    tr = hdist.DataParallelTrainer(model)
+    assert isinstance(tr.opt, hdist.BucketAdam)
+    x, eps, idx = torch.randn(20, 64, device="cuda"), torch.randn(20, 64, device="cuda"), torch.zeros(20, dtype=torch.int64, device="cuda")
+    loss_fn = lambda: model.loss_fn(x, idx=idx, epsilon=eps)  # noqa: E731
+    kept, before = loss_fn(), [p.detach().clone() for p in model.parameters()]
+    for _ in range(2):
+        with pytest.raises(RuntimeError, match="autograd graph"):
+            tr.capture(loss_fn, warmup=1)
+    assert all(torch.equal(p, q) for p, q in zip(model.parameters(), before)) and tr.opt.t == 0
+    kept = kept.detach()
+    first = tr.step(loss_fn)
+    assert torch.equal(first, kept)
+    replay = tr.capture(loss_fn, warmup=1)
+    assert bool(torch.isfinite(replay())) and bool(torch.isfinite(first))
