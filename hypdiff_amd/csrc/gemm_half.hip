@@ -14,8 +14,9 @@
 //   tiles     128 x 192, 128 x 128, 64 x 128 or 64 x 64 of 4 wavefronts, by a cost model (choose_tiles); 32 x 32 with the
 //             contraction split over the wavefronts for few rows (small_gemm); dW 192 x 192 or 64 x 64 (dw_plan).  One slab of 64 k in LDS,
 //             not two: a workgroup waits for its loads, and the 3 to 8 that fit a CU because of it multiply meanwhile.  Two
-//             slabs, the next one's loads in flight during the multiplies, are no faster at any size (74750 x 800 -> 900: 128 x 192
-//             146 us, with two 155; 128 x 128 158 and 175; 4096 x 800 -> 900: 14.1 and 14.2 at 64 x 128), three slower.
+//             slabs, the next one's loads in flight during the multiplies, are no faster at any size (with a GELU of four
+//             operations less an element, 74750 x 800 -> 900: 128 x 192 146 us, with two 155; 128 x 128 158 and 175;
+//             4096 x 800 -> 900: 14.1 and 14.2 at 64 x 128), three slower.
 //   staging   16-byte chunks go from memory to LDS without passing registers where every row starts on a 16-byte border and
 //             holds whole chunks; otherwise (an odd width, a sliced matrix) through registers, with the tail masked.  Chunks
 //             beyond the contraction's end come from a page of zeros, rows and columns beyond the matrix from a valid one
@@ -28,9 +29,10 @@
 //             consecutive k of its own column, so nothing is transposed in memory.
 //   split     the contraction of dW is cut into slices, one workgroup each; fp32 partial tiles are summed in slice order by
 //             the last launch, which also finishes db: the same bits on every call.
-// What bounds the large forward (74750 x 800 -> 900, bf16): bytes from L2 into the CUs, beside the products.  A CU takes 64 bytes a
-// clock in whole 128-byte lines (34 TB/s for the chip; 21 where the runs of 128 bytes straddle lines, as with rows of 1600 bytes;
-// 16 in runs of 64 bytes).  Timed alone: products 72 us, loads 70 to 100; stores and GELU cost 25 more than they hide.
+// What bounds the large forward (74750 x 800 -> 900, bf16: 142 to 155 us): no unit alone.  By its counters the matrix pipe is busy
+// 39 % of the cycles, the vector unit issues in 54 % (dx, without GELU, in 29 %), 2.2 GB of L2 lines reach the CUs (15 TB/s; a third
+// more than the operands' bytes, as runs of 128 bytes of 1600-byte rows straddle lines), and 36 % of the wavefronts' time is
+// waiting: the phases of a workgroup (loads, products, write-out) alternate, and the three of a CU overlap them in part.
 #include <math.h>
 #include <type_traits>
 #include "hd_common.cuh"
@@ -243,8 +245,8 @@ __device__ __forceinline__ float through_act(float g, float z) {
 }
 
 // The pre-activation as it is kept for the backward pass: in fp16 for bf16 operands too, whose own 8 bits would add a third of dz's
-// rounding to the gradients (error 1.5 instead of 1.41 roundings).  Only the slope reads it: beyond 30000 that is 0 or 1 (the
-// clamp keeps fp16 finite), and a positive z stays positive for ReLU.  A NaN stays one.
+// rounding to the gradients (error 1.5 instead of 1.41 roundings; for fp16 operands it is 1.47).  Only the slope reads it: beyond
+// 30000 that is 0 or 1 (the clamp keeps fp16 finite), and a positive z stays positive for ReLU.  A NaN stays one.
 __device__ __forceinline__ f16 kept_z(float z) {
     const float c = fminf(fmaxf(z, -30000.f), 30000.f);
     const float p = z > 0.f ? fmaxf(c, 0x1p-24f) : c;
@@ -739,10 +741,12 @@ inline int64_t tiles_of(int64_t M, int64_t N, int64_t bm, int64_t bn) { return (
 // 513 16.8 against 9.7).  Above, the least of start + share of the chip per 256 tiles, fitted to K = 800 (bf16, GELU, us; the
 // times at 4096, 8192, 16384 and 74750 rows of 900); the small ones cost 3.6 and 5.4 where slabs pass through registers (7850 x
 // 800 x 513: 27.0 us in 64 x 128 tiles, 23.1 in 128 x 128):
-//   1  64 x 64     6 + 2.85, at least 11      16.7   28.4   48.9   240
-//   2  64 x 128    6 + 4.6,  at least 13      15.1   24.5   42.9   179
-//   3  128 x 128   8 + 8.0,  at least 18      18.6   23.0   37.7   145
-//   4  128 x 192   8 + 12,   at least 20      20.9   26.3   36.9   137
+//   1  64 x 64     6 + 2.85, at least 11      18.9   30.6   52.2   210
+//   2  64 x 128    6 + 4.6,  at least 13      16.7   27.3   47.7   182
+//   3  128 x 128   8 + 8.0,  at least 18      20.8   25.5   40.8   155
+//   4  128 x 192   8 + 12,   at least 20      23.1   28.9   39.9   142
+// K is not in the rule.  Against all four at K = 64, 65, 333, 512, 513, 800, 801, 4096 and N = 300, 512, 900 its choice is 2 % behind
+// the best in the median and 28 % at most (8192 x 65 -> 900: 18.2 against 14.2).
 inline int choose_tiles(int64_t M, int64_t N, int64_t K, bool direct) {
     if (K < 8 && !direct) return 0;                                           // no 8 elements in a row to load at once
     if (tiles_of(M, N, 32, 32) <= (direct ? 512 : 64)) return 0;

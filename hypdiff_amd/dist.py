@@ -6,7 +6,7 @@ Three shardings:
   * graph sets (configs 1-3): whole graphs per rank, no data-path collective.  The only
     global quantity of the diffusion path is the mean / unbiased std of `normalization`
     (models/direction_diffusion.py:145-153): all-reduce the shard-local (sum, sumsq, count).
-  * data-parallel training: one flat fp32 gradient bucket, one all-reduce per step.
+  * data-parallel training: one flat gradient bucket (fp32, or 16-bit for 16-bit modules), averaged over the ranks in fp32.
   * one large graph (configs 4-5): contiguous row blocks of the CSR; HypLinear / HypAct are
     row-local, HypAgg needs the tangent rows of remote columns -> the (N/P, d) tangent block of
     every rank is all-gathered per layer IN COLUMN SLABS on RCCL's stream while the local SpMM
@@ -279,13 +279,12 @@ class DataParallelTrainer:
     loss -> backward -> Adam on one device; here every rank does that on its own shard of the
     graph set and the gradients are averaged in between).
 
-    All gradients live in one flat fp32 bucket (the HIP backward kernels' outputs are accumulated
-    into views of it).  With `overlap` (default) the bucket leaves in >= 4 MB chunks over RCCL while
+    All gradients live in one flat bucket, fp32 or 16-bit like the parameters (the HIP backward kernels' outputs are
+    accumulated into views of it).  With `overlap` (default) the bucket leaves in >= 4 MB chunks over RCCL while
     backward is still running -- 3 chunks for the mlp at D=512 (11 MB), 6 for ddpm.Backbone (25 MB);
     otherwise as ONE all-reduce after backward.  The optimizer is Adam on every rank (BucketAdam: one launch over the
-    bucket; optim.AdamW without decay and with fp32 masters for 16-bit parameters; torch.optim.Adam for host tensors; or the
-    one passed in) -- identical updates: weights never need a broadcast
-    after the first."""
+    bucket; optim.AdamW without decay and with fp32 masters for 16-bit parameters; torch.optim.Adam for host tensors; or
+    the one passed in) -- identical updates: weights never need a broadcast after the first."""
 
     def __init__(self, module, lr=1e-3, group=None, optimizer=None, broadcast=True, overlap=True):
         self.module, self.group, self.overlap = module, group, overlap
@@ -337,8 +336,9 @@ class DataParallelTrainer:
         graph-safe; ddpm.Model does that while a capture is running), never reads anything back to the host; the
         optimizer is BucketAdam or optim.AdamW (their step counts live on the device); no tensor of an earlier eager pass that
         still carries its autograd graph is alive (refused: the graph's nodes of the parameters are shared, with their stream).
-        With more than one rank (backend nccl = RCCL) the chunked gradient all-reduces are recorded into the graph as well -- they are stream operations -- so the graphed
-        step survives data parallelism (every rank must capture and replay in lockstep).
+        With more than one rank (backend nccl = RCCL) the chunked gradient all-reduces are recorded into the graph as well --
+        they are stream operations -- so the graphed step survives data parallelism (every rank must capture and replay in
+        lockstep).
         `warmup` eager steps run first on a side stream (allocations, caches).  The parameters' versions are bumped
         after every replay, as after an eager step."""
         coll = _collective(self.group)

@@ -96,11 +96,12 @@ class AdamW(torch.optim.Optimizer):
         step of the type is lost otherwise).  fp32 parameters are their own.  The masters are taken from the parameters at
         the first step (or from a loaded state): parameters changed by hand afterwards are overwritten.
 
-    The parameters of a group are distinct and share no memory.  Sparse, complex and fp64 parameters, lr as a tensor, amsgrad and maximize are not offered.  A parameter whose gradient
-    is None is skipped and does not count the step.  Inside a captured HIP graph the step count lives on the device, so a
-    replay has the right bias corrections (state_dict reads it back); lr and the other options are the captured ones.  Run one step (or load a state)
-    before the capture; a state loaded later goes into the same arrays, and replays continue from it.  state_dict / load_state_dict keep the state's own types; with state_bits=32 a state saved by
-    torch.optim.AdamW loads."""
+    The parameters of a group are distinct and share no memory.  Sparse, complex and fp64 parameters, lr as a tensor, amsgrad
+    and maximize are not offered.  A parameter whose gradient is None is skipped and does not count the step.  Inside a
+    captured HIP graph the step count lives on the device, so a replay has the right bias corrections (state_dict reads it
+    back); lr and the other options are the captured ones.  Run one step (or load a state) before the capture; a state loaded
+    later goes into the same arrays, and replays continue from it.  state_dict / load_state_dict keep the state's own types;
+    with state_bits=32 a state saved by torch.optim.AdamW loads; a state that is refused has changed nothing."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32, master_weights=False):
         defaults = dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits,
@@ -292,7 +293,8 @@ class AdamW(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict):
         saved, groups = state_dict["state"], state_dict["param_groups"]
-        if len(groups) != len(self.param_groups) or any(len(a["params"]) != len(b["params"]) for a, b in zip(groups, self.param_groups)):
+        if len(groups) != len(self.param_groups) or any(len(a["params"]) != len(b["params"])
+                                                        for a, b in zip(groups, self.param_groups)):
             raise ValueError("AdamW: the saved state has other parameter groups")
         # a state saved by torch.optim.AdamW has no state_bits.  Everything is looked at before anything changes
         options = [{k: g.get(k, mine[k]) for k in _OPTIONS} for g, mine in zip(groups, self.param_groups)]
@@ -301,7 +303,8 @@ class AdamW(torch.optim.Optimizer):
             if g.get("amsgrad") or g.get("maximize"):
                 raise ValueError("AdamW: the saved options ask for amsgrad or maximize, which are not offered")
             if self._captured(gi) and not self._keeps(gi, opt):
-                raise RuntimeError("AdamW: a captured step updates this state; state_bits and master_weights cannot change under it")
+                raise RuntimeError("AdamW: a captured step updates this state; state_bits and master_weights cannot change "
+                                   "under it")
             for pid, p in zip(g["params"], mine["params"]):
                 if saved.get(pid):
                     self._check_saved(saved[pid], p, opt)
@@ -310,8 +313,8 @@ class AdamW(torch.optim.Optimizer):
         # and the saved state may be this optimizer's own: that is copied before it is overwritten
         own = {b.untyped_storage().data_ptr() for fl in self._flats.values() for b in fl.buffers.values()}
         kept = lambda v: v.detach().clone() if v.untyped_storage().data_ptr() in own else v.detach()  # noqa: E731
-        parts = [[saved.get(pid) and {k: int(v) if k == "step" else kept(v) if torch.is_tensor(v) else v for k, v in saved[pid].items()}
-                  for pid in g["params"]] for g in groups]
+        parts = [[saved.get(pid) and {k: int(v) if k == "step" else kept(v) if torch.is_tensor(v) else v
+                                      for k, v in saved[pid].items()} for pid in g["params"]] for g in groups]
         super().load_state_dict({**state_dict, "state": {}})
         for gi, (mine, opt, part) in enumerate(zip(self.param_groups, options, parts)):
             mine.update(opt)

@@ -450,14 +450,16 @@ int hd_adam_step_f32(const hd_adam_job* jobs, int n_jobs, const void* grad_flat,
  *   z = x W^T + bias,  y = resid + act(z)
  * x (M, K) with row pitch ldx, W (N, K) with row pitch ldw, bias (N) or NULL, resid (M, N) with row pitch ldr (0: one row for
  * all) or NULL, y (M, N) contiguous; act HD_ACT_IDENTITY, HD_ACT_RELU or HD_ACT_GELU.  z (M, N) contiguous or NULL: the
- * pre-activation for the backward pass, in fp16 for both types (clamped to +-30000; the slope there is 0 or 1).  y is rounded once, from fp32.  Any sizes, pitches and element-aligned
- * pointers; rows that start on 16-byte borders and hold a multiple of 8 elements are fastest.  y and z overlap nothing. */
+ * pre-activation for the backward pass, in fp16 for both types (clamped to +-30000; the slope there is 0 or 1).  y is rounded
+ * once, from fp32.  Any pitches and element-aligned pointers, M < 2^29, N and K < 2^22, fewer than 2^24 tiles of 64 x 64 results
+ * (of 32 x 32 where K < 8); rows that start on 16-byte borders and hold a multiple of 8 elements are fastest.  y and z overlap
+ * nothing. */
 int hd_linear_act_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, const void* resid, int64_t ldr,
                       int dtype, int64_t M, int64_t N, int64_t K, int act, void* y, void* z, void* stream);
 /* Its gradients from g = dL/dy (M, N) with row pitch ldg:  dz = g * act'(z);  dx (M, K) = dz W,  dw (N, K) = dz^T x,
- * db (N) = colsum(dz); each contiguous, of the operands' type, or NULL.  dx_add (M, K) with
- * row pitch ld_add, or NULL, is added to dx before its rounding (the gradient that reaches x past the layer, as a skip
- * connection's does).  z may be NULL for HD_ACT_IDENTITY.  M >= 1.
+ * db (N) = colsum(dz); each contiguous, of the operands' type, or NULL.  dx_add (M, K) with row pitch ld_add, or NULL, is added to
+ * dx before its rounding (the gradient that reaches x past the layer, as a skip connection's does).  z may be NULL for
+ * HD_ACT_IDENTITY.  M >= 1.
  * workspace: hd_linear_act_bwd_workspace_bytes bytes, 16-byte aligned, contents arbitrary, not shared between calls in
  * flight.  No atomics: the same bits on every call. */
 int64_t hd_linear_act_bwd_workspace_bytes(int64_t M, int64_t N, int64_t K, int act);

@@ -400,6 +400,7 @@ def test_refusals_of_the_entry_points():
 
 
 @gpu
+@pytest.mark.filterwarnings("ignore:.*torch.jit:DeprecationWarning")
 @pytest.mark.parametrize("grad", [False, True])
 def test_forward_mode_derivatives_are_refused(grad):
     """a tangent may not get lost, whether or not an operand requires a gradient; operands without one pass"""
