@@ -514,9 +514,9 @@ class LinearAct(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, w, b, resid, act, skip):
-        y, z, x2, ldx, w2, ldw = ops._linear_act_fwd(x, w, b, x if skip else resid, act, act != 0)
+        y, z, x2, w2 = ops._linear_act_fwd(x, w, b, x if skip else resid, act, act != 0)
         ctx.save_for_backward(x2, w2, z)
-        ctx.args = (ldx, ldw, act, x.shape, skip)
+        ctx.args = (act, x.shape, skip)
         return y
 
     @staticmethod

@@ -834,7 +834,7 @@ def _matrix(t, cols):
 
 
 def _linear_act_fwd(x, w, b, resid, act, want_z):
-    """(y, z or None, x as a matrix, its pitch, w as a matrix, its pitch)"""
+    """(y, z or None, x as a matrix, w as a matrix)"""
     N, K = w.shape
     x2, ldx = _matrix(x, K)
     w2, ldw = _matrix(w, K)
@@ -849,7 +849,7 @@ def _linear_act_fwd(x, w, b, resid, act, want_z):
         _lib.call("hd_linear_act_fwd", x2.data_ptr(), ldx, w2.data_ptr(), ldw, None if b is None else b.data_ptr(),
                   None if resid is None else resid.data_ptr(), 0 if resid is None else ldr, DT_CODES[x2.dtype], M, N, K, act,
                   y.data_ptr(), None if z is None else z.data_ptr(), raw_stream())
-    return y, z, x2, ldx, w2, ldw
+    return y, z, x2, w2
 
 
 @functools.lru_cache(maxsize=256)
@@ -857,12 +857,20 @@ def _linear_act_bwd_bytes(M, N, K, act):
     return _lib.load().hd_linear_act_bwd_workspace_bytes(M, N, K, act)
 
 
-def _linear_act_bwd(g, z, x2, w2, ldx, ldw, act, x_shape, skip, need_x, need_w, need_b):
+def _linear_act_bwd(g, z, x2, w2, act, x_shape, skip, need_x, need_w, need_b):
     if not (g.get_device() == x2.get_device() == w2.get_device() == _cur_device()):
         _dev(g, x2, w2)                                   # says which one is elsewhere
     N, K = w2.shape
     g2, ldg = _matrix(g, N)
+    # the saved operands' own pitches, not the forward pass's: a hook on saved tensors (save_on_cpu) brings back contiguous copies
+    x2, ldx = _matrix(x2, K)
+    w2, ldw = _matrix(w2, K)
     M = x2.shape[0]
+    if z is not None:
+        z = z.contiguous()
+    if not (x2.dtype is w2.dtype is g2.dtype) or g2.shape[0] != M or (z is not None and (
+            z.dtype is not torch.float16 or z.shape != g2.shape or z.get_device() != x2.get_device())):
+        raise RuntimeError("linear_act: a saved tensor came back with another type, shape or device")
     new = x2.new_empty if M else x2.new_zeros
     dx = new(x_shape) if need_x else None
     dw = new((N, K)) if need_w else None

@@ -422,6 +422,33 @@ def test_forward_mode_derivatives_are_refused(grad):
                 call()
 
 
+@gpu
+@pytest.mark.parametrize("M,N,K,pitch,w_pitch", [(300, 136, 128, 37, 5), (300, 136, 128, 0, 8), (40, 33, 41, 7, 0), (3000, 264, 200, 24, 16)])
+def test_saved_tensors_that_change_their_layout(M, N, K, pitch, w_pitch):
+    """hooks on saved tensors bring back contiguous copies of pitched operands (save_on_cpu), or pitched ones of contiguous: the
+    same gradients; a hook that changes the type is refused"""
+    from hypdiff_amd import ops
+    gen = _gen(16)
+    x = torch.randn(M, K + pitch, device="cuda", generator=gen).bfloat16()[:, :K].detach().requires_grad_(True)
+    w = torch.randn(N, K + w_pitch, device="cuda", generator=gen).bfloat16()[:, :K].detach().requires_grad_(True)
+    g = torch.randn(M, N, device="cuda", generator=gen).bfloat16()
+    run = lambda act: torch.autograd.grad(ops.linear_act(x, w, act=act), [x, w], g)  # noqa: E731
+
+    def widen(t):
+        big = torch.full((t.shape[0], t.shape[1] + 9), float("nan"), device="cuda", dtype=t.dtype)
+        big[:, 3:3 + t.shape[1]] = t
+        return big[:, 3:3 + t.shape[1]]
+    for act in ("gelu", "identity"):
+        want = run(act)
+        for hooks in (torch.autograd.graph.save_on_cpu(), torch.autograd.graph.saved_tensors_hooks(lambda t: t, widen),
+                      torch.autograd.graph.saved_tensors_hooks(lambda t: t.contiguous().clone(), lambda t: t)):
+            with hooks:
+                got = run(act)
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: t.float()), pytest.raises(RuntimeError, match="came back"):
+        run("gelu")
+
+
 def test_grids_beyond_the_limit_are_refused():
     """an input narrower than a chunk takes 32 x 32 tiles whatever their number: 2^24 of them are 2^32 threads, which no grid
     holds (no GPU needed: refused before anything is launched)"""
