@@ -230,3 +230,97 @@ def test_gradient_of_the_step_column(dtype):
     for sl in (slice(0, d), slice(d, d + 1)):
         got, want = net.fc1.weight.grad[:, sl].double(), ps["fc1.weight"].grad[:, sl]
         assert float((got - want).norm()) <= 15 * HALF[dtype] * float(want.norm())
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("T", [20, 40])
+def test_diffusionset_trains_and_samples_in_16_bits(dtype, T):
+    """as test_diffusion_trains_and_samples_in_16_bits, with the graph axis.  The schedule of 20 steps ends at beta = 50 * 0.02 = 1,
+    hence abar = 0, from which no sampling starts (1 / abar): not in fp32 either.
+
+    The unscaled gradients of a mean over 4440 elements reach fp16's smallest numbers, where a stored value is off by u0 = 2^-25
+    however small it is.  In Frobenius norms, R rows, layer l of N x K: dL/dout is off by d5 = u0 sqrt(R N); dx of layer l by
+    d_l |W_l|_2 + u0 sqrt(R K); dz of the layer below by 1.13 of that + u0 sqrt(R K); dW_l by d_l |h_l|_2 + u0 sqrt(N K); db_l by
+    d_l sqrt(R) + u0 sqrt(N)."""
+    g, n, dim, e = 4, 37, 30, 15 * HALF[dtype]
+    half, full = _set_diffusion(dim, T=T, device="cuda").to(dtype), _set_diffusion(dim, T=T, device="cuda")
+    with torch.no_grad():
+        for p, q in zip(full.mlp.parameters(), half.mlp.parameters()):
+            p.copy_(q)
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    x = torch.randn(g, n, dim, device="cuda", generator=gen) * 0.05
+    u0 = torch.randn(g, 3, dim, device="cuda", generator=gen) * 0.05
+    labels = torch.randint(0, 3, (g, n), device="cuda", generator=gen)
+    noise = torch.randn(g, n, dim, device="cuda", generator=gen, dtype=torch.float64)
+    t = torch.randint(0, 20, (g,), device="cuda", generator=gen)
+    loss, seen = [], []
+    full.mlp.register_forward_pre_hook(lambda mod, args: seen.append(args))
+    for m in (half, full):
+        out = m(x.clone(), None, labels, u0, restrict=True, graphset=True, t=t, noise=noise.clone())
+        out.backward()
+        loss.append(float(out.detach()) ** 0.5)
+    assert abs(loss[0] - loss[1]) <= e * (loss[1] + 1) + 1e-5
+    xt, tf = seen[0]
+    layers = [getattr(full.mlp, f"fc{k}") for k in range(1, 6)]
+    with torch.no_grad():
+        h = [torch.cat([xt.reshape(g * n, dim), tf.repeat_interleave(n)[:, None]], 1).double()]
+        for layer in layers[:-1]:
+            z = h[-1] @ layer.weight.double().t() + layer.bias.double()
+            h.append(z * 0.5 * torch.erfc(-z / 2.0 ** 0.5))
+        u0_, R = 2.0 ** -25 if dtype == torch.float16 else 0.0, g * n
+        d, small = u0_ * (R * dim) ** 0.5, {}
+        for layer, rows in zip(reversed(layers), reversed(h)):
+            N, K = layer.weight.shape
+            small[layer.weight] = d * float(torch.linalg.matrix_norm(rows, 2)) + u0_ * (N * K) ** 0.5
+            small[layer.bias] = d * R ** 0.5 + u0_ * N ** 0.5
+            d = 1.13 * (d * float(torch.linalg.matrix_norm(layer.weight.double(), 2)) + u0_ * (R * K) ** 0.5) + u0_ * (R * K) ** 0.5
+    for p, q in zip(half.mlp.parameters(), full.mlp.parameters()):
+        assert float((p.grad.float() - q.grad).norm()) <= e * (1 + (loss[1] + 1) / loss[1]) * float(q.grad.norm()) + small[q]
+    assert bool(half.alphas_cumprod[-1] == 0) == (T == 20)
+    img = torch.randn(g, n, dim, device="cuda", generator=gen)
+    with torch.no_grad():
+        out, ref = (m.p_sample_loop(x.clone().double(), None, labels, u0, graphset=True, img=img) for m in (half, full))
+    assert out.shape == (g, n, dim) and torch.equal(torch.isfinite(out), torch.isfinite(ref))
+    assert bool(torch.isfinite(out).all()) == (T == 40)
+
+
+@gpu
+@pytest.mark.parametrize("dtype,overlap", [(torch.bfloat16, True), (torch.float16, False)])
+def test_captured_training_step_of_the_direction_denoiser(dtype, overlap):
+    """the direction diffusion's loss, backward and AdamW as one graph, new rows between replays, against eager steps of an
+    identical module: a replay's corrections are one fp32 step off at most, which may move a stored weight by one of its steps"""
+    from hypdiff_amd import dist as hdist
+    x, u0, labels, noise = _rows(300, 30, 7)
+    labels = labels.to(torch.int32)
+    t = torch.randint(0, 200, (300,), device="cuda")
+    mods, trs = [], []
+    for _ in range(2):
+        m = _diffusion(30, T=200, device="cuda").to(dtype).train()
+        mods.append(m)
+        trs.append(hdist.DataParallelTrainer(m.mlp, lr=1e-3, overlap=overlap))
+    loss = [lambda m=m: m(x, None, labels, u0, restrict=True, graphset=True, t=t, noise=noise.clone()) for m in mods]
+    replay = trs[0].capture(loss[0], warmup=1)
+    trs[1].step(loss[1])
+    for k in range(3):
+        gen = torch.Generator(device="cuda").manual_seed(k)
+        x.copy_(torch.randn(300, 30, device="cuda", generator=gen) * 0.05)
+        t.copy_(torch.randint(0, 200, (300,), device="cuda", generator=gen))
+        la, lb = replay(), trs[1].step(loss[1])
+        torch.cuda.synchronize()
+        assert abs(float(la) - float(lb)) <= 0.02 * abs(float(lb))
+        for p, q in zip(mods[0].mlp.parameters(), mods[1].mlp.parameters()):
+            d = float((p.detach().double() - q.detach().double()).norm() / q.detach().double().norm())
+            assert d <= 4 * (k + 1) * HALF[dtype] + 1e-3 * 0.05 * (k + 1), d
+
+
+@gpu
+def test_no_rows_in_16_bits():
+    from hypdiff_amd.ddpm import Backbone
+    from hypdiff_amd.models.direction_diffusion import mlp
+    net, bb = mlp(30).cuda().bfloat16(), Backbone(64, 96, 2, 50).cuda().bfloat16()
+    for out, params in ((net(torch.zeros(0, 30, device="cuda"), torch.zeros(0, device="cuda")), net.parameters()),
+                        (bb(torch.zeros(0, 64, device="cuda"), torch.zeros(0, dtype=torch.int64, device="cuda")), bb.parameters())):
+        assert out.shape[0] == 0
+        out.sum().backward()
+        assert not any(p.grad.any() for p in params)
