@@ -144,8 +144,8 @@ class Model(nn.Module):
             ab = self._alpha_bars_dev(x.device)
             used_alpha_bars = ab[idx][:, None]
             # fp32 whatever x and the weights are: the kernel reads fp32 rows, the loss is taken on them
+            epsilon = torch.randn_like(x, dtype=torch.float32) if epsilon is None else epsilon.to(torch.float32)
             x = x.to(torch.float32).contiguous()
-            epsilon = torch.randn_like(x) if epsilon is None else epsilon.to(torch.float32)
             if epsilon.shape != x.shape:
                 raise ValueError(f"Model: epsilon has shape {tuple(epsilon.shape)}, x {tuple(x.shape)}")
             x_tilde = torch.empty_like(x)

@@ -149,6 +149,11 @@ def test_ddpm_takes_inputs_of_any_type(dtype, weights):
     got = model.loss_fn(x, idx=idx)
     torch.manual_seed(6)
     assert torch.equal(got, model.loss_fn(x.float(), idx=idx))
+    turned = x.t().contiguous().t()                      # the draw follows x's layout in memory, as randn_like does
+    torch.manual_seed(6)
+    got = model.loss_fn(turned, idx=idx)
+    torch.manual_seed(6)
+    assert torch.equal(got, model.loss_fn(x, idx=idx, epsilon=torch.randn_like(turned.float())))
     s = DDPMSampler(1e-4, 0.02, 50, model, "cuda", (64,))
     with torch.no_grad():
         assert torch.equal(s.one_step(x, 7, noise), s.one_step(x.float(), 7, noise.float()))
